@@ -589,6 +589,128 @@ int sd_verify_batch(const void* draft, int64_t draft_stride_b, int64_t draft_str
                     uint8_t* accept_mask, void* workspace, size_t workspace_bytes,
                     void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Decoding in 4 bits: a KV cache of 4-bit codes and a linear with 4-bit
+ * weights. No counterpart in the reference, whose cache is 16-bit and whose
+ * quantized weights are int8.
+ *
+ * Cache: `codes` (num_blocks, block_size, num_kv_heads, 128 bytes) and `scales`
+ * (num_blocks, block_size, num_kv_heads, 4 NG) of dtype, both by strides of
+ * block, position and head (bytes, resp. elements; the last axis contiguous).
+ * A row holds one token's key (bytes 0 .. 63) and value (64 .. 127) of one kv
+ * head, head_dim 128, in NG = 128 / group_size groups of 32, 64 or 128 dims;
+ * its scales are (scale, zero) of each key group, then of each value group:
+ *   lo = min x, hi = max x;  zero = dtype(lo);  scale = dtype(max(hi - zero, 0) / 15)
+ *   code = clamp(round_half_even((x - zero) / scale), 0, 15) (0 where scale is 0)
+ *   value = zero + scale * code
+ * A group with a NaN or an infinity, or whose range leaves dtype's, comes back
+ * as NaN. Key dword 4 g + i, nibble p holds dim 32 i + 8 g + 2 (p % 4) + p / 4;
+ * value dword r, nibble t holds dim 16 t + r (g, i < 4; p, t < 8; r < 16).
+ * Code rows are 16-byte aligned, scale rows 16-byte aligned (8 bytes for
+ * group_size 128). num_blocks * block_size < 2^31.
+ * ------------------------------------------------------------------------- */
+
+/*
+ * Row i of key / value (num_tokens, num_kv_heads, 128) quantized to slot
+ * slot_mapping[i] (position s % block_size of block s / block_size); slots
+ * outside the cache, -1 among them, are skipped. The slots of one call must
+ * differ. dtype bf16/f16; num_tokens * num_kv_heads <= 2^27.
+ */
+int sd_store_kvcache_int4(const void* key, int64_t key_stride_tok, int64_t key_stride_head,
+                          const void* value, int64_t value_stride_tok, int64_t value_stride_head,
+                          void* codes, int64_t codes_stride_block, int64_t codes_stride_pos,
+                          int64_t codes_stride_head, void* scales, int64_t scales_stride_block,
+                          int64_t scales_stride_pos, int64_t scales_stride_head,
+                          int32_t group_size, const int32_t* slot_mapping, int64_t num_tokens,
+                          int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                          int64_t num_blocks, int32_t dtype, void* stream);
+
+/*
+ * A step's append: per-head RMSNorm with q_weight / k_weight ((128,) dtype, both
+ * NULL: none) and rotate-half RoPE of q (num_tokens, num_q_heads, 128) and k
+ * (num_tokens, num_kv_heads, 128) at `positions`, in fp32 throughout:
+ *   y = x / sqrt(mean(x^2) + eps) * w;  (y1 cos - y2 sin, y2 cos + y1 sin)
+ * q_out (num_tokens, num_q_heads, 128) and k_out (num_tokens, num_kv_heads, 128;
+ * may be NULL), contiguous, receive the results rounded once (sd_qk_norm_rope
+ * rounds after each of the module's steps instead); the unrounded key and v are
+ * quantized to slot_mapping as by sd_store_kvcache_int4. A token whose position
+ * is outside [0, max_position) is normed and not rotated. q_out and k_out may
+ * share no memory with q, k, v or the cache. Rows 16-byte aligned;
+ * num_tokens * (num_q_heads + num_kv_heads) <= 2^27.
+ */
+int sd_qk_norm_rope_store_int4(const void* q, int64_t q_stride_tok, int64_t q_stride_head,
+                               const void* k, int64_t k_stride_tok, int64_t k_stride_head,
+                               const void* v, int64_t v_stride_tok, int64_t v_stride_head,
+                               int64_t num_tokens, int32_t num_q_heads, int32_t num_kv_heads,
+                               int32_t head_dim, const void* q_weight, const void* k_weight,
+                               float eps, const int64_t* positions, const float* cos_sin,
+                               int64_t cos_sin_stride, int64_t max_position, void* q_out,
+                               void* k_out, void* codes, int64_t codes_stride_block,
+                               int64_t codes_stride_pos, int64_t codes_stride_head, void* scales,
+                               int64_t scales_stride_block, int64_t scales_stride_pos,
+                               int64_t scales_stride_head, int32_t group_size, int64_t num_blocks,
+                               int32_t block_size, const int32_t* slot_mapping, int32_t dtype,
+                               void* stream);
+
+/*
+ * The rows at slot_mapping (num_rows,) read back: key / value (num_rows,
+ * num_kv_heads, 128) dtype, contiguous, 16-byte aligned; rows of slots outside
+ * the cache are zero. num_rows * num_kv_heads <= 2^27.
+ */
+int sd_load_kvcache_int4(const void* codes, int64_t codes_stride_block, int64_t codes_stride_pos,
+                         int64_t codes_stride_head, const void* scales,
+                         int64_t scales_stride_block, int64_t scales_stride_pos,
+                         int64_t scales_stride_head, int32_t group_size,
+                         const int32_t* slot_mapping, int64_t num_rows, int32_t num_kv_heads,
+                         int32_t head_dim, int32_t block_size, int64_t num_blocks, int32_t dtype,
+                         void* key, void* value, void* stream);
+
+/*
+ * Paged decode / verify attention over the 4-bit cache: sequences, rows, masks,
+ * clamps and limits as sd_paged_attention ((num_q_heads / num_kv_heads) *
+ * max_qlen <= 32; rows without a visible key are zero; rows at or beyond
+ * total_q are neither read nor written). Sums and softmax in fp32, one
+ * rounding at the end. Keys that a row does not see may hold anything.
+ * workspace: >= sd_paged_attention_int4_workspace_size(...) bytes (0: none
+ * needed), 16-byte aligned, queried on the same device; num_splits 0 = library
+ * default, n > 0 = n workgroups per (sequence, kv head) on average. The result
+ * of a call is the same bits every time.
+ */
+size_t sd_paged_attention_int4_workspace_size(int32_t num_seqs, int32_t max_qlen,
+                                              int32_t num_q_heads, int32_t num_kv_heads,
+                                              int64_t max_ctx, int32_t num_splits);
+int sd_paged_attention_int4(const void* q, int64_t q_stride_tok, int64_t q_stride_head,
+                            const void* codes, int64_t codes_stride_block,
+                            int64_t codes_stride_pos, int64_t codes_stride_head,
+                            const void* scales, int64_t scales_stride_block,
+                            int64_t scales_stride_pos, int64_t scales_stride_head,
+                            int32_t group_size, int64_t num_blocks, int32_t block_size,
+                            const int32_t* block_table, int64_t bt_stride,
+                            int32_t max_blocks_per_seq, const int32_t* context_lens,
+                            const int32_t* cu_seqlens_k, const int32_t* cu_seqlens_q,
+                            int32_t max_qlen, int64_t total_q, int32_t num_seqs,
+                            int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                            float scale, int32_t dtype, void* out, int64_t out_stride_tok,
+                            int64_t out_stride_head, void* workspace, size_t workspace_bytes,
+                            int32_t num_splits, void* stream);
+
+/*
+ * W4A16 linear: y = x @ w^T (+ bias), w[n, k] = (code - 8) * scale[n, k / group_size].
+ *   x     : (M, K) dtype (bf16/f16), row stride x_stride_m, 16-byte aligned rows
+ *   w     : (N, K / 2) bytes, row stride w_stride_n bytes, 16-byte aligned rows;
+ *           byte j holds the codes of columns 2 j (low half) and 2 j + 1
+ *   scale : (N, K / group_size) row-major, scale_dtype bf16/f16/f32
+ *   bias  : (N,) dtype or NULL
+ *   y     : (M, N) dtype, row stride y_stride_m, sharing no byte with x
+ * group_size: a multiple of 32 that divides K. fp32 sums, one rounding. A row of
+ * x with an infinity, or with values past 2^120, gives NaN where a product with
+ * the weight alone would give an infinity (the sums are of code + 16, less 24 sum x).
+ */
+int sd_w4a16_linear(const void* x, int64_t x_stride_m, const uint8_t* w, int64_t w_stride_n,
+                    const void* scale, int32_t scale_dtype, int32_t group_size, const void* bias,
+                    void* y, int64_t y_stride_m, int64_t M, int64_t N, int64_t K, int32_t dtype,
+                    void* stream);
+
 #ifdef __cplusplus
 }
 #endif

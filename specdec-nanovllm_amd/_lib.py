@@ -138,6 +138,39 @@ SIGNATURES["sd_paged_attention_store"] = (ctypes.c_int, [
     _p,                             # slot_mapping
     *SIGNATURES["sd_paged_attention"][1]])
 
+_cache4 = [_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i32]  # codes, strides, scales, strides, group
+SIGNATURES.update({
+    "sd_store_kvcache_int4": (ctypes.c_int, [
+        _p, _i64, _i64, _p, _i64, _i64,  # key, strides (tok, head), value, strides
+        *_cache4, _p, _i64,              # the cache, slots, tokens
+        _i32, _i32, _i32, _i64,          # num_kv_heads, head_dim, block_size, num_blocks
+        _i32, _p]),                      # dtype, stream
+    "sd_qk_norm_rope_store_int4": (ctypes.c_int, [
+        _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64,  # q, k, v and strides
+        _i64, _i32, _i32, _i32, _p, _p, _f32,  # tokens, Hq, Hkv, head_dim, q_w, k_w, eps
+        _p, _p, _i64, _i64, _p, _p,      # positions, cos_sin, stride, max_position, q_out, k_out
+        *_cache4, _i64, _i32, _p,        # the cache, num_blocks, block_size, slots
+        _i32, _p]),                      # dtype, stream
+    "sd_load_kvcache_int4": (ctypes.c_int, [
+        *_cache4, _p, _i64,              # the cache, slots, rows
+        _i32, _i32, _i32, _i64, _i32,    # num_kv_heads, head_dim, block_size, num_blocks, dtype
+        _p, _p, _p]),                    # key, value, stream
+    "sd_paged_attention_int4_workspace_size": (_sz, [_i32, _i32, _i32, _i32, _i64, _i32]),
+    "sd_paged_attention_int4": (ctypes.c_int, [
+        _p, _i64, _i64,                  # q, strides (tok, head)
+        *_cache4, _i64, _i32,            # the cache, num_blocks, block_size
+        _p, _i64, _i32,                  # block_table, bt_stride, max_blocks
+        _p, _p, _p,                      # context_lens, cu_seqlens_k, cu_seqlens_q
+        _i32, _i64, _i32, _i32, _i32, _i32,  # max_qlen, total_q, seqs, hq, hkv, head_dim
+        _f32, _i32, _p, _i64, _i64,      # scale, dtype, out, strides
+        _p, _sz, _i32, _p]),             # workspace, bytes, num_splits, stream
+    "sd_w4a16_linear": (ctypes.c_int, [
+        _p, _i64, _p, _i64,              # x, x_stride, w, w_stride
+        _p, _i32, _i32, _p,              # scale, scale_dtype, group_size, bias
+        _p, _i64, _i64, _i64, _i64,      # y, y_stride, M, N, K
+        _i32, _p]),                      # dtype, stream
+})
+
 _lib = None
 
 

@@ -562,6 +562,226 @@ def w8a16_gate_up_silu(x: torch.Tensor, qweight: torch.Tensor, scale: torch.Tens
     return y.view(shape)
 
 
+# ------------------------------------------------------------------- 4-bit KV cache
+def int4_kvcache(num_blocks: int, block_size: int, num_kv_heads: int, group_size: int = 64,
+                 dtype: torch.dtype = torch.bfloat16,
+                 device: torch.device | str = "cuda") -> tuple[torch.Tensor, torch.Tensor]:
+    """An empty 4-bit KV cache for heads of 128 dims: (kv_codes (num_blocks, block_size,
+    num_kv_heads, 128) uint8, kv_scales (..., 512 // group_size) of ``dtype``, the activations').
+
+    A row of codes is one token's key (64 bytes) and value of one head; a scale and a zero per
+    group of 32, 64 or 128 dims: value = zero + scale * code (include/specdec_amd.h has the
+    order of the half bytes). The tensors are views of head-major memory (a head's rows of a
+    page side by side), which attention reads in the longest runs; any strides with aligned rows
+    work. 144 bytes a token and head at group 64, against 512 in 16 bits."""
+    assert group_size in (32, 64, 128), f"group_size must be 32, 64 or 128, got {group_size}"
+    codes = torch.zeros((num_blocks, num_kv_heads, block_size, 128), dtype=torch.uint8, device=device)
+    scales = torch.zeros((num_blocks, num_kv_heads, block_size, 512 // group_size), dtype=dtype,
+                         device=device)
+    return codes.transpose(1, 2), scales.transpose(1, 2)
+
+
+def _cache4(kv_codes: torch.Tensor, kv_scales: torch.Tensor, dtype: torch.dtype) -> tuple:
+    """The C ABI's arguments of a 4-bit cache (codes, strides, scales, strides, group size)."""
+    assert kv_codes.dim() == 4 and kv_codes.dtype == torch.uint8 and kv_codes.shape[3] == 128, \
+        "kv_codes must be (num_blocks, block_size, num_kv_heads, 128) uint8"
+    assert kv_scales.dim() == 4 and kv_scales.shape[:3] == kv_codes.shape[:3] and \
+        kv_scales.shape[3] in (4, 8, 16), "kv_scales must be kv_codes' blocks, 512 / group_size each"
+    assert kv_scales.dtype == dtype, f"kv_scales must be {dtype}, as the activations"
+    cs, ss = kv_codes.stride(), kv_scales.stride()
+    assert cs[3] == 1 and ss[3] == 1
+    return (kv_codes.data_ptr(), cs[0], cs[1], cs[2], kv_scales.data_ptr(), ss[0], ss[1], ss[2],
+            512 // kv_scales.shape[3])
+
+
+def store_kvcache_int4(key: torch.Tensor, value: torch.Tensor, kv_codes: torch.Tensor,
+                       kv_scales: torch.Tensor, slot_mapping: torch.Tensor) -> None:
+    """``store_kvcache`` into a 4-bit cache (``int4_kvcache``): key / value (N, num_kv_heads,
+    128) quantized to ``slot_mapping`` (slots of one call differ; -1 skips the row)."""
+    assert key.dim() == 3 and key.shape == value.shape and key.dtype == value.dtype
+    N, Hkv, D = key.shape
+    cache = _cache4(kv_codes, kv_scales, key.dtype)
+    assert kv_codes.shape[2] == Hkv and slot_mapping.numel() == N
+    assert key.stride(2) == 1 and value.stride(2) == 1
+    slots = _i32(slot_mapping.reshape(-1))
+    dev = _lib.require_device(key, value, kv_codes, kv_scales, slots)
+    if N == 0:
+        return
+    with _lib.on_device(dev):
+        rc = _lib.load().sd_store_kvcache_int4(
+            key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(), value.stride(0),
+            value.stride(1), *cache, slots.data_ptr(), N, Hkv, D, kv_codes.shape[1],
+            kv_codes.shape[0], _lib.dtype_code(key.dtype), _lib.stream_ptr(dev))
+    _lib.check(rc)
+
+
+def qk_norm_rope_store_int4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                            positions: torch.Tensor, cos_sin_cache: torch.Tensor,
+                            kv_codes: torch.Tensor, kv_scales: torch.Tensor,
+                            slot_mapping: torch.Tensor, q_weight: torch.Tensor | None = None,
+                            k_weight: torch.Tensor | None = None, eps: float = 1e-6,
+                            key_out: bool = True):
+    """A step's append to a 4-bit cache in one launch: per-head RMSNorm of q (T, Hq, 128) and
+    k (T, Hkv, 128) (skipped without weights), rotate-half RoPE at ``positions`` from
+    ``cos_sin_cache`` (max_pos, [1,] 128) fp32 = [cos | sin], then the rotated key and v
+    (T, Hkv, 128) quantized to ``slot_mapping``. Strided views of a qkv projection work and are
+    left as they are; returns (q, k) as new contiguous tensors (k None with ``key_out=False``,
+    for decode, where attention reads the cache). fp32 throughout, each output rounded once
+    (``qk_norm_rope`` keeps the module's own roundings); the key is quantized unrounded."""
+    assert q.dim() == 3 and k.dim() == 3 and q.shape[0] == k.shape[0] and v.shape == k.shape
+    assert q.stride(2) == 1 and k.stride(2) == 1 and v.stride(2) == 1
+    assert q.dtype == k.dtype == v.dtype and q.shape[2] == k.shape[2]
+    assert (q_weight is None) == (k_weight is None)
+    T, Hq, D = q.shape
+    Hkv = k.shape[1]
+    cache = _cache4(kv_codes, kv_scales, k.dtype)
+    assert kv_codes.shape[2] == Hkv
+    cs = cos_sin_cache if cos_sin_cache.dim() == 2 else \
+        cos_sin_cache.reshape(cos_sin_cache.shape[0], -1)
+    assert cs.dtype == torch.float32 and cs.shape[1] >= 128 and cs.stride(1) == 1
+    pos = positions.reshape(-1)
+    if pos.dtype != torch.int64:
+        pos = pos.to(torch.int64)
+    pos = pos.contiguous()
+    slots = _i32(slot_mapping.reshape(-1))
+    assert pos.numel() == T and slots.numel() == T
+    qw = kw = None
+    if q_weight is not None:
+        assert q_weight.shape == (D,) and k_weight.shape == (D,)
+        qw, kw = q_weight.to(q.dtype).contiguous(), k_weight.to(q.dtype).contiguous()
+    dev = _lib.require_device(q, k, v, pos, cs, kv_codes, kv_scales, slots, qw, kw)
+    q_out = torch.empty((T, Hq, D), dtype=q.dtype, device=dev)
+    k_out = torch.empty((T, Hkv, D), dtype=q.dtype, device=dev) if key_out else None
+    if T == 0:
+        return q_out, k_out
+    with _lib.on_device(dev):
+        rc = _lib.load().sd_qk_norm_rope_store_int4(
+            q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
+            v.data_ptr(), v.stride(0), v.stride(1), T, Hq, Hkv, D, _ptr(qw), _ptr(kw), float(eps),
+            pos.data_ptr(), cs.data_ptr(), cs.stride(0), cs.shape[0], q_out.data_ptr(), _ptr(k_out),
+            *cache, kv_codes.shape[0], kv_codes.shape[1], slots.data_ptr(),
+            _lib.dtype_code(q.dtype), _lib.stream_ptr(dev))
+    _lib.check(rc)
+    return q_out, k_out
+
+
+def load_kvcache_int4(kv_codes: torch.Tensor, kv_scales: torch.Tensor,
+                      slot_mapping: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """The rows of a 4-bit cache at ``slot_mapping`` (N,) in the activations' type: (key, value),
+    each (N, num_kv_heads, 128); rows of slot -1 are zero. Prefill over a cached prefix reads its
+    pages this way."""
+    cache = _cache4(kv_codes, kv_scales, kv_scales.dtype)
+    slots = _i32(slot_mapping.reshape(-1))
+    dev = _lib.require_device(kv_codes, kv_scales, slots)
+    N, Hkv = slots.numel(), kv_codes.shape[2]
+    k = torch.empty((N, Hkv, 128), dtype=kv_scales.dtype, device=dev)
+    v = torch.empty((N, Hkv, 128), dtype=kv_scales.dtype, device=dev)
+    if N == 0:
+        return k, v
+    with _lib.on_device(dev):
+        rc = _lib.load().sd_load_kvcache_int4(
+            *cache, slots.data_ptr(), N, Hkv, 128, kv_codes.shape[1], kv_codes.shape[0],
+            _lib.dtype_code(kv_scales.dtype), k.data_ptr(), v.data_ptr(), _lib.stream_ptr(dev))
+    _lib.check(rc)
+    return k, v
+
+
+def paged_attention_int4(q: torch.Tensor, kv_codes: torch.Tensor, kv_scales: torch.Tensor,
+                         block_table: torch.Tensor, scale: float, *,
+                         context_lens: torch.Tensor | None = None,
+                         cu_seqlens_k: torch.Tensor | None = None,
+                         cu_seqlens_q: torch.Tensor | None = None, max_seqlen_q: int = 1,
+                         num_splits: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``paged_attention`` over a 4-bit cache (``int4_kvcache``): decode (one query row per
+    sequence) or speculative verify (``cu_seqlens_q``, bottom-right causal), GQA, split over the
+    keys; (num_q_heads // num_kv_heads) * max_seqlen_q <= 32. q (total_q, num_q_heads, 128)."""
+    if q.dim() != 3:
+        raise ValueError(f"q must be (tokens, heads, head_dim), got {tuple(q.shape)}")
+    total_q, Hq, D = q.shape
+    cache = _cache4(kv_codes, kv_scales, q.dtype)
+    num_blocks, block_size, Hkv = kv_codes.shape[:3]
+    assert Hq % Hkv == 0, f"GQA needs num_q_heads divisible by num_kv_heads: {Hq} vs {Hkv}"
+    assert q.stride(2) == 1
+    assert block_table.dim() == 2, "block_table must be (num_seqs, max_blocks)"
+    if (context_lens is None) == (cu_seqlens_k is None):
+        raise ValueError("give exactly one of context_lens / cu_seqlens_k")
+    bt, ctx, cuk, cuq = _i32(block_table), _i32(context_lens), _i32(cu_seqlens_k), _i32(cu_seqlens_q)
+    num_seqs, max_blocks = bt.shape
+    assert ctx is None or ctx.numel() == num_seqs
+    assert cuk is None or cuk.numel() == num_seqs + 1
+    if cuq is None:
+        max_seqlen_q = 1
+        if total_q != num_seqs:
+            raise ValueError(f"decode expects one query row per sequence: q has {total_q} rows, "
+                             f"block_table {num_seqs}")
+    else:
+        assert cuq.numel() == num_seqs + 1
+    dev = _lib.require_device(q, kv_codes, kv_scales, bt, ctx, cuk, cuq, out)
+    if out is None:
+        out = torch.empty_like(q)
+    else:
+        assert out.shape == q.shape and out.dtype == q.dtype and out.stride(2) == 1
+    if total_q == 0 or num_seqs == 0:
+        return out
+    lib = _lib.load()
+    qs, os = q.stride(), out.stride()
+    max_seqlen_q = int(max_seqlen_q)
+    with _lib.on_device(dev):
+        # the plan (and so the workspace) depends on the device's compute units
+        ws_bytes = lib.sd_paged_attention_int4_workspace_size(
+            num_seqs, max_seqlen_q, Hq, Hkv, max_blocks * block_size, int(num_splits))
+        # (past the library's limits the size is the largest there is: the call says what is wrong)
+        ws = _workspace(ws_bytes, dev) if ws_bytes < 1 << 60 else None
+        rc = lib.sd_paged_attention_int4(
+            q.data_ptr(), qs[0], qs[1], *cache, num_blocks, block_size, bt.data_ptr(), bt.stride(0),
+            max_blocks, _ptr(ctx), _ptr(cuk), _ptr(cuq), max_seqlen_q, total_q, num_seqs, Hq, Hkv,
+            D, float(scale), _lib.dtype_code(q.dtype), out.data_ptr(), os[0], os[1], _ptr(ws),
+            ws_bytes if ws is not None else 0, int(num_splits), _lib.stream_ptr(dev))
+    _lib.check(rc)
+    return out
+
+
+# ---------------------------------------------------------------------------- w4a16
+def w4a16_linear(x: torch.Tensor, qweight: torch.Tensor, scale: torch.Tensor,
+                 bias: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """y = x @ w^T + bias with 4-bit weights, w[n, k] = (code - 8) * scale[n, k // group].
+
+    x: (..., K) fp16/bf16; qweight: (N, K // 2) uint8, byte j the codes of columns 2j (low half)
+    and 2j + 1; scale: (N, K // group) bf16/fp16/fp32, the group a multiple of 32. Returns
+    (..., N) in x.dtype; fp32 sums, rounded once (``layers.quant.quantize_weight_int4`` makes
+    the weights)."""
+    assert qweight.dtype == torch.uint8, f"qweight must be uint8, got {qweight.dtype}"
+    assert qweight.dim() == 2 and scale.dim() == 2
+    N, K = qweight.shape[0], 2 * qweight.shape[1]
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    M = x2.shape[0]
+    assert x2.shape[1] == K, f"K mismatch: x {tuple(x2.shape)} vs w {tuple(qweight.shape)}"
+    groups = scale.shape[1]
+    assert scale.shape[0] == N and groups and K % groups == 0, "scale must be (N, K // group)"
+    if x2.stride(1) != 1 or x2.data_ptr() % 16 or (M > 1 and x2.stride(0) % 8):
+        x2 = x2.contiguous()
+    qw = qweight if qweight.is_contiguous() else qweight.contiguous()
+    sc = scale if scale.is_contiguous() else scale.contiguous()
+    b = None
+    if bias is not None:
+        assert bias.shape == (N,), "bias must be (N,)"
+        b = bias.to(x.dtype).contiguous()
+    dev = _lib.require_device(x2, qw, sc, b, out)
+    if out is None:
+        y = torch.empty((M, N), device=dev, dtype=x.dtype)
+    else:
+        y = out.view(M, N)
+        assert y.dtype == x.dtype and (N == 1 or y.stride(1) == 1)
+    if M:
+        with _lib.on_device(dev):
+            rc = _lib.load().sd_w4a16_linear(
+                x2.data_ptr(), x2.stride(0), qw.data_ptr(), qw.stride(0), sc.data_ptr(),
+                _lib.dtype_code(sc.dtype), K // groups, _ptr(b), y.data_ptr(), y.stride(0), M, N, K,
+                _lib.dtype_code(x.dtype), _lib.stream_ptr(dev))
+        _lib.check(rc)
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
+
+
 def quantize_int8(w: torch.Tensor, group_size: int = 0):
     """Symmetric int8 quantization of a 2-D weight on the GPU (the W8A16
     format's producer, nanovllm/layers/quant.py:123-148): per row (group_size

@@ -23,16 +23,25 @@ template <> struct Magic<_Float16> {
   static constexpr uint32_t kMask = 0x03C003C0u, kBase = 0x4C004C00u;
 };
 
+// kBase in a vector register, once a kernel: v_and_or_b32 takes one scalar operand, so with the mask
+// and the base both in scalar registers the pair costs an and and an or.
+template <typename T> __device__ __forceinline__ uint32_t code_base() {
+  uint32_t v = Magic<T>::kBase;
+  asm("" : "+v"(v));
+  return v;
+}
+
 // The codes at bits P .. P + 3 and 16 + P .. 16 + P + 3 of w as two T of 16 + u.
-template <typename T, int P> __device__ __forceinline__ uint32_t code_pair(uint32_t w) {
+template <typename T, int P> __device__ __forceinline__ uint32_t code_pair(uint32_t w, uint32_t base) {
   constexpr int kShift = Magic<T>::kBit - P;
   const uint32_t s = kShift >= 0 ? w << (kShift & 31) : w >> (-kShift & 31);
-  return (s & Magic<T>::kMask) | Magic<T>::kBase;
+  return (s & Magic<T>::kMask) | base;
 }
 
 // The 8 codes of a dword as 8 T of 16 + u, in the order nibble 0, 4, 1, 5, 2, 6, 3, 7.
-template <typename T> __device__ __forceinline__ u32x4 unpack8(uint32_t w) {
-  return u32x4{code_pair<T, 0>(w), code_pair<T, 4>(w), code_pair<T, 8>(w), code_pair<T, 12>(w)};
+template <typename T> __device__ __forceinline__ u32x4 unpack8(uint32_t w, uint32_t base) {
+  return u32x4{code_pair<T, 0>(w, base), code_pair<T, 4>(w, base), code_pair<T, 8>(w, base),
+               code_pair<T, 12>(w, base)};
 }
 
 }  // namespace sd

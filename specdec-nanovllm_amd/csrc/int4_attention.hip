@@ -12,15 +12,26 @@
 // parts (hi + lo, 2^-17 relative), since a single rounding would double the output's error.
 //
 // Work: a pair is one (sequence, kv head), a chunk 128 keys of one pair: 32 for each of the 4 waves
-// of a workgroup. All chunks, laid end to end, are cut into equal runs, one a workgroup, whatever
+// of a workgroup (64 keys where a pair has two 16-row tiles: two waves then take the same keys, one
+// tile each, and share what they load in the caches; one wave with both tiles has no registers left
+// for a second wave on its SIMD and measured 32 us instead of XXX us for 8 x 7 rows). All chunks, laid end to end, are cut into equal runs, one a workgroup, whatever
 // the length mix (context lengths are read on the device). When a pair or the run ends, the waves
 // merge their softmax states in LDS; a pair that several runs share leaves partials in the workspace
 // (two slots a run: the pair it starts in, the pair it ends in), which the combine kernel merges.
 // Where the table admits few chunks a pair, a run is one whole pair and there is no second launch.
 //
-// Bound by the bytes of the cache: 128 + 8 NG per key and kv head. A wave keeps kAhead steps of
-// loads in flight in registers (18 dwords a step at NG = 2).
+// A step's rows go from memory to LDS without registers (global_load_lds, 5 instructions a step), up
+// to kAhead steps ahead; the 16-byte units of a row are permuted by the lanes' global addresses so
+// that the operand reads hit all banks. Scales pass once more through LDS as fp32.
+//
+// Bound by the bytes of the cache, 128 + 8 NG per key and kv head, and close behind by vector issue:
+// unpacking costs 144 instructions a step of 32 keys (two a code pair), the softmax of a 16-row tile
+// as much again. Where a pair has at most 4 rows (decode with up to 4 query heads a kv head), 12 of
+// the tile's 16 columns are empty; there each lane takes 2 of the 8 scores that lanes 0 .. 3 of its
+// row of 16 hold (moves within the row), which leaves a quarter of the softmax (R4 below).
 #include <math.h>
+
+#include <type_traits>
 
 #include "int4.h"
 
@@ -32,19 +43,17 @@ using sd::u32x4;
 constexpr int kD = 128;
 constexpr int kWaves = 4;
 constexpr int kStep = 32;               // keys of a wave's step
-constexpr int kChunk = kWaves * kStep;  // keys of a workgroup's step
-constexpr int kPitch = kD + 4;          // floats of a row's state in LDS: acc, then m and l
-constexpr int kWholeChunks = 4;         // up to this many chunks a pair: no splitting of pairs
+constexpr int kPitch = kD + 4;          // floats of a row's state: acc, then m and l
+constexpr int kMergeRows = 8;           // rows of a tile the waves merge at a time
+constexpr int kWholeKeys = 512;         // tables of up to this many keys: no splitting of pairs
 
 struct Params {
   const uint16_t* q;
   int64_t q_stok, q_shead;
   const uint8_t* codes;
-  int64_t c_sblk, c_shead;  // bytes
-  uint32_t c_spos;          // bytes
+  uint32_t c_sblk, c_spos, c_shead;  // bytes
   const uint8_t* scales;
-  int64_t s_sblk, s_shead;  // bytes
-  uint32_t s_spos;          // bytes
+  uint32_t s_sblk, s_spos, s_shead;  // bytes
   int32_t num_blocks, block_size;
   int32_t bs_shift;  // log2(block_size), -1 where it is no power of two
   int32_t max_ctx;
@@ -63,67 +72,56 @@ struct Params {
   int32_t runs;   // workgroups of the main kernel
   int32_t whole;  // a run is one whole pair
   int32_t rmax;
+  int32_t chunk_shift;  // log2 of a chunk's keys
 };
 
-__device__ __forceinline__ int seq_keys(const Params& p, int b) {
-  const int L = p.ctx ? p.ctx[b] : p.cu_k[b + 1] - p.cu_k[b];
-  return min(max(L, 0), p.max_ctx);
-}
-__device__ __forceinline__ int seq_keys_uniform(const Params& p, int b) {
-  const int L = p.ctx ? sd::load_scalar_i32(p.ctx + b)
-                      : sd::load_scalar_i32(p.cu_k + b + 1) - sd::load_scalar_i32(p.cu_k + b);
-  return min(max(L, 0), p.max_ctx);
-}
-__device__ __forceinline__ int chunks_of(int L) { return (L + kChunk - 1) / kChunk; }
-
-// Chunks (of one head) of all sequences before `upto`, by a whole wave.
-__device__ int chunks_before(const Params& p, int upto) {
-  const int lane = threadIdx.x & 63;
-  int sum = 0;
-  for (int c = lane; c < upto; c += 64) sum += chunks_of(seq_keys(p, c));
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off);
-  return __builtin_amdgcn_readfirstlane(sum);
+typedef const __attribute__((address_space(4))) int32_t* ScalarPtr;
+// Load through the scalar cache of a wave-uniform word that nothing writes while the kernel runs.
+__device__ __forceinline__ int scalar_load(const int32_t* p) {
+  return *(ScalarPtr)(reinterpret_cast<uintptr_t>(p));
 }
 
-// The sequence that holds chunk s of the layout (b major, then head, then chunk), and the chunks of
-// one head before it. s < hkv * all chunks.
-__device__ void locate(const Params& p, int s, int& b, int& before) {
-  const int lane = threadIdx.x & 63;
-  int run = 0;
-  for (int c = 0; c < p.num_seqs; c += 64) {
-    const int n = c + lane < p.num_seqs ? chunks_of(seq_keys(p, c + lane)) : 0;
-    const int incl = sd::wave_inclusive_sum(n);
-    const int excl = run + incl - n;
-    const unsigned long long hit =
-        __ballot(n > 0 && excl * p.hkv <= s && s < (excl + n) * p.hkv);
-    if (hit) {
-      const int src = __ffsll(hit) - 1;
-      b = c + src;
-      before = __builtin_amdgcn_readlane(excl, src);
-      return;
-    }
-    run += __builtin_amdgcn_readlane(incl, 63);
-  }
-  b = p.num_seqs - 1;
-  before = run;
+__device__ __forceinline__ int chunks_of(const Params& p, int L) {
+  return (L + (1 << p.chunk_shift) - 1) >> p.chunk_shift;
 }
 
-struct Rows {
-  int64_t q0;
-  int nq;
+// A sequence: its keys, query rows and the first of these.
+struct Seq {
+  int L, nq, q0;
 };
-__device__ __forceinline__ Rows seq_rows(const Params& p, int b) {
-  if (!p.cu_q) return Rows{b, 1};
-  const int a = sd::load_scalar_i32(p.cu_q + b), e = sd::load_scalar_i32(p.cu_q + b + 1);
-  return Rows{a, min(max(e - a, 0), p.max_qlen)};
+__device__ __forceinline__ Seq seq_of(const Params& p, int k0, int k1, int q0, int q1, int b) {
+  Seq s;
+  s.L = min(max(p.ctx ? k0 : k1 - k0, 0), p.max_ctx);
+  s.nq = p.cu_q ? min(max(q1 - q0, 0), p.max_qlen) : 1;
+  s.q0 = p.cu_q ? q0 : b;
+  return s;
+}
+// Sequence b on each lane. All four words are loaded whatever the arrays: loads under branches would
+// wait for each other.
+__device__ __forceinline__ Seq lane_seq(const Params& p, int b) {
+  const int32_t* kp = p.ctx ? p.ctx : p.cu_k;
+  const int32_t* qp = p.cu_q ? p.cu_q : kp;
+  const int kn = p.ctx ? 0 : 1, qn = p.cu_q ? 1 : 0;
+  const int k0 = kp[b], k1 = kp[b + kn], q0 = qp[b], q1 = qp[b + qn];
+  return seq_of(p, k0, k1, q0, q1, b);
+}
+__device__ __forceinline__ Seq uniform_seq(const Params& p, int b) {
+  const int32_t* kp = p.ctx ? p.ctx : p.cu_k;
+  const int32_t* qp = p.cu_q ? p.cu_q : kp;
+  const int kn = p.ctx ? 0 : 1, qn = p.cu_q ? 1 : 0;
+  return seq_of(p, scalar_load(kp + b), scalar_load(kp + b + kn), scalar_load(qp + b),
+                scalar_load(qp + b + qn), b);
+}
+__device__ __forceinline__ Seq seq_from_lane(const Seq& s, int lane) {
+  return Seq{__builtin_amdgcn_readlane(s.L, lane), __builtin_amdgcn_readlane(s.nq, lane),
+             __builtin_amdgcn_readlane(s.q0, lane)};
 }
 
 template <typename T>
-__device__ __forceinline__ void store_row4(const Params& p, const Rows& sr, int h, int row, int c,
+__device__ __forceinline__ void store_row4(const Params& p, const Seq& sq, int h, int row, int c,
                                            f32x4 v) {
   const int qi = row / p.gq, g = row - qi * p.gq;
-  const int64_t qt = sr.q0 + qi;
+  const int64_t qt = static_cast<int64_t>(sq.q0) + qi;
   if (qt < 0 || qt >= p.total_q) return;
   uint2 w;
   w.x = sd::pack2<T>(v.x, v.y);
@@ -131,312 +129,434 @@ __device__ __forceinline__ void store_row4(const Params& p, const Rows& sr, int 
   *reinterpret_cast<uint2*>(p.out + qt * p.o_stok + static_cast<int64_t>(h * p.gq + g) * p.o_shead + 4 * c) = w;
 }
 
-// Position in the layout: chunk j of the n chunks of pair (b, h), whose sequence has L keys.
-struct Pos {
-  int b, h, j, n, L;
-};
-__device__ __forceinline__ void next_pair(const Params& p, Pos& a) {
-  a.j = 0;
-  if (a.h + 1 < p.hkv) {
-    ++a.h;
-    return;
-  }
-  a.h = 0;
-  do {
-    if (++a.b >= p.num_seqs) {
-      a.n = 0;
-      return;
-    }
-    a.L = seq_keys_uniform(p, a.b);
-    a.n = chunks_of(a.L);
-  } while (a.n == 0);
+// 16 (4) bytes per lane to LDS byte 16 (4) * lane of the wave-uniform address l. In assembly for the
+// scalar-base form and because the compiler makes LDS reads wait for every such load in flight; the
+// loop waits for its own. No register is written.
+__device__ __forceinline__ uint32_t lds_addr(const void* l) {
+  return static_cast<uint32_t>(
+      reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) void*)l));
+}
+__device__ __forceinline__ void to_lds16(const uint8_t* base, uint32_t off, uint32_t l) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+               ::"s"(l), "v"(off), "s"(base) : "memory", "m0");
+}
+__device__ __forceinline__ void to_lds16(const uint8_t* at, uint32_t l) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+               ::"s"(l), "v"(at) : "memory", "m0");
+}
+__device__ __forceinline__ void to_lds4(const uint8_t* at, uint32_t l) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
+               ::"s"(l), "v"(at) : "memory", "m0");
 }
 
-// One wave's step as loaded: lane (lr, lg) holds the key half bytes 32 lg .. 32 lg + 31 of keys lr
-// and 16 + lr, dword lr of the values of keys 4 lg + j and 16 + 4 lg + j, and of key lane / 2 the
-// scales of its keys (even lanes) or values.
-template <int NG> struct Step {
-  u32x4 k[2];
-  uint32_t v[8];
-  uint32_t s[NG];
-};
+// CTRL's lane moves of a value; lanes outside BANKS (four lanes a bit) keep `old`.
+template <int CTRL, int BANKS> __device__ __forceinline__ float merge_dpp(float old, float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(
+                                       __builtin_bit_cast(int, old), __builtin_bit_cast(int, v), CTRL,
+                                       0xF, BANKS, false));
+}
+template <int CTRL> __device__ __forceinline__ uint32_t move_dpp(uint32_t v) {
+  return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, 0xF, 0xF, true));
+}
+constexpr int kShl4 = 0x104, kShl8 = 0x108, kShl12 = 0x10C, kShr4 = 0x114, kShr8 = 0x118, kShr12 = 0x11C;
+constexpr int kRor4 = 0x124, kRor8 = 0x128;
 
-template <typename T, int NG, int RT, bool ONE_PAGE>
-__global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(RT == 1 ? 2 : 1)))
+// How pages meet a wave's 32 keys: they lie in one page, each half does, or anything.
+enum Pages { kOnePage, kHalfPages, kAnyPages };
+
+// Position in the layout: chunk j of the n chunks of pair (b, h); blk: the pages of the wave's keys.
+struct Pos {
+  int b, h, j, n, L;
+  int blk[2];
+};
+// 32 x 32 -> 64 bits (two scalar multiplies)
+__device__ __forceinline__ uint64_t wide(uint32_t a, uint32_t b) { return static_cast<uint64_t>(a) * b; }
+
+// LDS of one wave: kAhead slots of a step (32 rows of 128 bytes, then their scales), fp32 scales.
+template <int NG> constexpr int ahead() { return NG == 4 ? 2 : 3; }
+template <int NG> constexpr int slot_bytes() { return kStep * (kD + 8 * NG); }
+template <int NG> constexpr int wave_bytes() { return ahead<NG>() * slot_bytes<NG>() + kStep * 16 * NG; }
+
+template <typename T, int NG, int TS, bool R4, Pages PAGES>
+__global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2)))
 void int4_attn_main(Params p) {
-  constexpr int kAhead = 3;
-  constexpr int kRow = 4 * NG;  // floats of a key's scales in LDS
-  __shared__ __attribute__((aligned(16))) float lds_s[kWaves][kStep][kRow];
-  __shared__ __attribute__((aligned(16))) float lds_m[kWaves][RT * 16][kPitch];
+  static_assert(!R4 || TS == 1, "four rows fit one tile");
+  constexpr int kChunk = kWaves / TS * kStep;
+  constexpr int kAhead = ahead<NG>();
+  constexpr int kLoads = 5;  // vector memory instructions of a step
+  constexpr int NE = R4 ? 2 : 8;  // scores of a row tile on a lane
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kWaves][wave_bytes<NG>()];
+  __shared__ __attribute__((aligned(16))) float lds_m[kWaves][kMergeRows][kPitch];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 15, lg = lane >> 4;
+  const int ks = wave / TS, ts = wave % TS;  // this wave's keys of a chunk, its row tile
 
-  // ---- this run's chunks [s0, s1) and where they begin
+  // ---- this run's chunks and where they begin
   Pos cur;
-  int left;
+  Seq seqs{0, 1, 0};  // up to 64 sequences: sequence `lane`
+  Seq sq;
+  const bool in_lanes = p.num_seqs <= 64;
+  int left, s0 = 0;
   bool entered = false;  // the current pair began in an earlier run
   const int run = blockIdx.x;
+  auto seq_at = [&](int b) { return in_lanes ? seq_from_lane(seqs, b) : uniform_seq(p, b); };
+  if (in_lanes) seqs = lane_seq(p, min(lane, p.num_seqs - 1));
   if (p.whole) {
     cur.b = run / p.hkv;
     cur.h = run - cur.b * p.hkv;
     cur.j = 0;
-    cur.L = seq_keys_uniform(p, cur.b);
-    cur.n = left = chunks_of(cur.L);
+    sq = seq_at(cur.b);
+    cur.L = sq.L;
+    cur.n = left = chunks_of(p, cur.L);
     if (left == 0) {
-      const Rows sr = seq_rows(p, cur.b);
-      for (int i = tid; i < p.gq * sr.nq * 32; i += kWaves * 64)
-        store_row4<T>(p, sr, cur.h, i / 32, i % 32, f32x4{0.f, 0.f, 0.f, 0.f});
+      for (int i = tid; i < p.gq * sq.nq * 32; i += kWaves * 64)
+        store_row4<T>(p, sq, cur.h, i / 32, i % 32, f32x4{0.f, 0.f, 0.f, 0.f});
       return;
     }
   } else {
-    const int total = chunks_before(p, p.num_seqs) * p.hkv;
-    const int S = (total + p.runs - 1) / p.runs;
-    const int s0 = run * S;
-    if (s0 >= total) return;
-    left = min(S, total - s0);
+    int total = 0;  // chunks of one head
     int before = 0;
-    locate(p, s0, cur.b, before);
+    cur.b = 0;
+    if (in_lanes) {
+      const int n = lane < p.num_seqs ? chunks_of(p, seqs.L) : 0;
+      const int incl = sd::wave_inclusive_sum(n);
+      total = __builtin_amdgcn_readlane(incl, 63);
+      const int S = (total * p.hkv + p.runs - 1) / p.runs;
+      s0 = run * S;
+      left = min(S, total * p.hkv - s0);
+      if (left <= 0) return;
+      const unsigned long long hit =
+          __ballot(n > 0 && (incl - n) * p.hkv <= s0 && s0 < incl * p.hkv);
+      cur.b = __ffsll(hit) - 1;
+      before = __builtin_amdgcn_readlane(incl - n, cur.b);
+    } else {
+      for (int c = lane; c < p.num_seqs; c += 64) total += chunks_of(p, lane_seq(p, c).L);
+      for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off);
+      total = __builtin_amdgcn_readfirstlane(total);
+      const int S = (total * p.hkv + p.runs - 1) / p.runs;
+      s0 = run * S;
+      left = min(S, total * p.hkv - s0);
+      if (left <= 0) return;
+      for (int c = 0, sum = 0; c < p.num_seqs; c += 64) {
+        const int n = c + lane < p.num_seqs ? chunks_of(p, lane_seq(p, c + lane).L) : 0;
+        const int incl = sum + sd::wave_inclusive_sum(n);
+        const unsigned long long hit =
+            __ballot(n > 0 && (incl - n) * p.hkv <= s0 && s0 < incl * p.hkv);
+        if (hit) {
+          const int src = __ffsll(hit) - 1;
+          cur.b = c + src;
+          before = __builtin_amdgcn_readlane(incl - n, src);
+          break;
+        }
+        sum = __builtin_amdgcn_readlane(incl, 63);
+      }
+    }
     cur.b = __builtin_amdgcn_readfirstlane(cur.b);
-    cur.L = seq_keys_uniform(p, cur.b);
-    cur.n = chunks_of(cur.L);
+    sq = seq_at(cur.b);
+    cur.L = sq.L;
+    cur.n = chunks_of(p, cur.L);
     const int in = s0 - before * p.hkv;
     cur.h = in / cur.n;
     cur.j = in - cur.h * cur.n;
     entered = cur.j > 0;
   }
-  Pos ahead = cur;  // what load_step loads next
-  int ahead_left = left;
-  bool first_pair = true;
 
-  auto page_base = [&](int b, int tok) {
-    int pg = p.bs_shift >= 0 ? tok >> p.bs_shift : tok / p.block_size;
-    int blk = p.bt[b * p.bt_stride + pg];
-    return min(max(blk, 0), p.num_blocks - 1);
+  auto next_pair = [&](Pos& a) {
+    a.j = 0;
+    if (a.h + 1 < p.hkv) {
+      ++a.h;
+      return;
+    }
+    a.h = 0;
+    do {
+      if (++a.b >= p.num_seqs) {
+        a.n = 0;
+        return;
+      }
+      a.L = seq_at(a.b).L;
+      a.n = chunks_of(p, a.L);
+    } while (a.n == 0);
   };
+
+  // ---- loads: a step's rows, 8 a instruction, lane l unit (l % 8) ^ (l / 8) of row l / 8; its scales
+  uint8_t* const mine = lds[wave];
+  const uint32_t mine_at = __builtin_amdgcn_readfirstlane(lds_addr(mine));
+  const uint32_t unit = ((lane & 7) ^ (lane >> 3)) * 16;
+  uint32_t row_off[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) row_off[r] = static_cast<uint32_t>(8 * r + (lane >> 3)) * p.c_spos + unit;
+  // the key whose scales this lane loads and the byte of them (16 bytes a lane; NG = 1: 4)
+  const int s_key = NG == 4 ? lane >> 1 : NG == 2 ? lane & 31 : lane >> 1;
+  const uint32_t s_byte = NG == 4 ? 16 * (lane & 1) : NG == 2 ? 0 : 4 * (lane & 1);
+
+  auto page_of = [&](int tok) { return p.bs_shift >= 0 ? tok >> p.bs_shift : tok / p.block_size; };
   auto in_page = [&](int tok) {
     return p.bs_shift >= 0 ? tok & (p.block_size - 1) : tok % p.block_size;
   };
-  // Loads the next step (the same loads whatever the lengths: positions past the end read the last
-  // key, past the run the last chunk again) and moves on.
-  auto load_step = [&](Step<NG>& st) {
-    const int last = ahead.L - 1;
-    const int t0 = min(ahead.j * kChunk + wave * kStep, last);
-    const int64_t hc = ahead.h * p.c_shead, hs = ahead.h * p.s_shead;
-    const int kv = min(t0 + (lane >> 1), last);  // the key whose scales this lane loads
-    if constexpr (ONE_PAGE) {
-      int pg = p.bs_shift >= 0 ? t0 >> p.bs_shift : t0 / p.block_size;
-      int blk = sd::load_scalar_i32(p.bt + ahead.b * p.bt_stride + pg);
-      blk = min(max(blk, 0), p.num_blocks - 1);
-      const int off = in_page(t0);
-      const uint8_t* cp = p.codes + blk * p.c_sblk + hc + static_cast<int64_t>(off) * p.c_spos;
-      const uint8_t* sp = p.scales + blk * p.s_sblk + hs + static_cast<int64_t>(off) * p.s_spos;
-#pragma unroll
-      for (int tt = 0; tt < 2; ++tt)
-        st.k[tt] = sd::load16_stream(cp + static_cast<uint32_t>(min(t0 + 16 * tt + lr, last) - t0) * p.c_spos + 16 * lg);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int tok = min(t0 + (j < 4 ? 4 * lg + j : 12 + 4 * lg + j), last);
-        st.v[j] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(
-            cp + static_cast<uint32_t>(tok - t0) * p.c_spos + 64 + 4 * lr));
-      }
-      const uint32_t* s32 = reinterpret_cast<const uint32_t*>(
-          sp + static_cast<uint32_t>(kv - t0) * p.s_spos) + NG * (lane & 1);
-#pragma unroll
-      for (int g = 0; g < NG; ++g) st.s[g] = s32[g];
-    } else {
-      auto code_row = [&](int tok) {
-        return p.codes + page_base(ahead.b, tok) * p.c_sblk + hc + static_cast<int64_t>(in_page(tok)) * p.c_spos;
-      };
-#pragma unroll
-      for (int tt = 0; tt < 2; ++tt)
-        st.k[tt] = sd::load16_stream(code_row(min(t0 + 16 * tt + lr, last)) + 16 * lg);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int tok = min(t0 + (j < 4 ? 4 * lg + j : 12 + 4 * lg + j), last);
-        st.v[j] = *reinterpret_cast<const uint32_t*>(code_row(tok) + 64 + 4 * lr);
-      }
-      const uint32_t* s32 = reinterpret_cast<const uint32_t*>(
-          p.scales + page_base(ahead.b, kv) * p.s_sblk + hs + static_cast<int64_t>(in_page(kv)) * p.s_spos) + NG * (lane & 1);
-#pragma unroll
-      for (int g = 0; g < NG; ++g) st.s[g] = s32[g];
+  auto first_key = [&](const Pos& a) { return min(a.j * kChunk + ks * kStep, a.L - 1); };
+  // Table lookups of a position's pages, a step ahead of their use.
+  auto find_pages = [&](Pos& a) {
+    if constexpr (PAGES != kAnyPages) {
+      const int t0 = first_key(a);
+      const int32_t* row = p.bt + a.b * p.bt_stride;
+      a.blk[0] = scalar_load(row + page_of(t0));
+      if constexpr (PAGES == kHalfPages) a.blk[1] = scalar_load(row + page_of(min(t0 + 16, a.L - 1)));
     }
-    if (ahead_left > 1) {
-      --ahead_left;
-      if (++ahead.j == ahead.n) next_pair(p, ahead);
+  };
+  Pos pos = cur;  // what load_step loads next
+  int pos_left = left;
+  find_pages(pos);
+  // The same instructions whatever the lengths: rows past the end read the last key, steps past the
+  // run its last chunk again.
+  auto load_step = [&](int slot) {
+    const uint32_t l = mine_at + slot * slot_bytes<NG>(), ls = l + kStep * kD;
+    const int last = pos.L - 1, t0 = first_key(pos);
+    const uint8_t* const hc = p.codes + wide(pos.h, p.c_shead);
+    const uint8_t* const hs = p.scales + wide(pos.h, p.s_shead);
+    const uint8_t* s_at;
+    if constexpr (PAGES == kOnePage) {
+      const int blk = min(max(pos.blk[0], 0), p.num_blocks - 1), off = in_page(t0);
+      const uint8_t* cp = hc + wide(blk, p.c_sblk) + wide(off, p.c_spos);
+      const uint32_t most = static_cast<uint32_t>(last - t0) * p.c_spos + unit;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) to_lds16(cp, min(row_off[r], most), l + 1024 * r);
+      s_at = hs + wide(blk, p.s_sblk) + wide(off, p.s_spos) +
+             (static_cast<uint32_t>(min(s_key, last - t0)) * p.s_spos + s_byte);
+    } else if constexpr (PAGES == kHalfPages) {
+      const uint8_t* sp[2];
+#pragma unroll
+      for (int f = 0; f < 2; ++f) {
+        const int t = min(t0 + 16 * f, last);
+        const int blk = min(max(pos.blk[f], 0), p.num_blocks - 1), off = in_page(t);
+        const uint8_t* cp = hc + wide(blk, p.c_sblk) + wide(off, p.c_spos);
+        const uint32_t most = static_cast<uint32_t>(last - t) * p.c_spos + unit;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) to_lds16(cp, min(row_off[r], most), l + 2048 * f + 1024 * r);
+        sp[f] = hs + wide(blk, p.s_sblk) + wide(off, p.s_spos) +
+                (static_cast<uint32_t>(min(s_key & 15, last - t)) * p.s_spos + s_byte);
+      }
+      s_at = s_key < 16 ? sp[0] : sp[1];
+    } else {
+      const int32_t* table = p.bt + pos.b * p.bt_stride;
+      auto block = [&](int tok) { return min(max(table[page_of(tok)], 0), p.num_blocks - 1); };
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int tok = min(t0 + 8 * r + (lane >> 3), last);
+        to_lds16(hc + wide(block(tok), p.c_sblk) + wide(in_page(tok), p.c_spos) + unit, l + 1024 * r);
+      }
+      const int tok = min(t0 + s_key, last);
+      s_at = hs + wide(block(tok), p.s_sblk) + wide(in_page(tok), p.s_spos) + s_byte;
+    }
+    if constexpr (NG == 1) to_lds4(s_at, ls);
+    else if (NG == 4 || lane < 32) to_lds16(s_at, ls);
+    if (pos_left > 1) {
+      --pos_left;
+      if (++pos.j == pos.n) next_pair(pos);
+      find_pages(pos);
     }
   };
 
-  // ---- state of the current pair
-  u32x4 qop[RT][4];
-  float qsum[RT][NG];
-  int lim[RT], causal = 0;
-  float m_run[RT], l_run[RT], zsum[RT][NG];
-  f32x4 acc[RT][8];
-  Rows sr{0, 0};
+  // ---- state of the current pair. R4: a lane's scores are row lr % 4's, keys 16 (lr / 8) + 4 lg +
+  //      2 (lr / 4 % 2) and the next; its accumulators still row lr's (rows 4 .. 15: nothing).
+  u32x4 qop[4];
+  float qsum[NG], zsum[NG], m_run, l_run;
+  int lim, causal = 0;
+  f32x4 acc[8];
+  auto key_of = [&](int e) {  // of score e, within the step
+    return R4 ? 16 * (lr >> 3) + 4 * lg + 2 * ((lr >> 2) & 1) + e : e < 4 ? 4 * lg + e : 12 + 4 * lg + e;
+  };
 
   auto begin_pair = [&]() {
-    sr = seq_rows(p, cur.b);
-    causal = cur.L - sr.nq;
+    causal = cur.L - sq.nq;
+    // R4: the columns of rows 4 .. 15 repeat rows 0 .. 3 (their scores stay unread)
+    const int row = R4 ? lr & 3 : ts * 16 + lr;
+    const int qi = row / p.gq, gq = row - qi * p.gq;
+    const int64_t qt = static_cast<int64_t>(sq.q0) + qi;
+    const bool valid = qi < sq.nq && qt >= 0 && qt < p.total_q;
+    lim = valid ? min(causal + qi, cur.L - 1) : -1;
+    const uint16_t* qp = p.q + (valid ? qt * p.q_stok + static_cast<int64_t>(cur.h * p.gq + gq) * p.q_shead : 0) + 8 * lg;
+    float part[4];
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      const int row = rt * 16 + lr;
-      const int qi = row / p.gq, g = row - qi * p.gq;
-      const int64_t qt = sr.q0 + qi;
-      const bool valid = qi < sr.nq && qt >= 0 && qt < p.total_q;
-      lim[rt] = valid ? min(causal + qi, cur.L - 1) : -1;
-      const uint16_t* qp = p.q + (valid ? qt * p.q_stok + static_cast<int64_t>(cur.h * p.gq + g) * p.q_shead : 0) + 8 * lg;
-      float part[4];
+    for (int i = 0; i < 4; ++i) {
+      qop[i] = valid ? sd::load16(qp + 32 * i) : u32x4{0u, 0u, 0u, 0u};
+      const uint32_t one = __is_same(T, __bf16) ? 0x3F803F80u : 0x3C003C00u;
+      part[i] = 0.f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        qop[rt][i] = valid ? sd::load16(qp + 32 * i) : u32x4{0u, 0u, 0u, 0u};
-        const uint32_t w[4] = {qop[rt][i].x, qop[rt][i].y, qop[rt][i].z, qop[rt][i].w};
-        float s = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) s += sd::from_bits<T>(static_cast<uint16_t>(w[e / 2] >> (16 * (e & 1))));
-        part[i] = s;
-      }
-#pragma unroll
-      for (int g2 = 0; g2 < NG; ++g2) {
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (i * NG / 4 == g2) s += part[i];
-        qsum[rt][g2] = sd::sum_over_groups(s);
-        zsum[rt][g2] = 0.f;
-      }
-      m_run[rt] = -INFINITY;
-      l_run[rt] = 0.f;
-#pragma unroll
-      for (int t = 0; t < 8; ++t) acc[rt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int e = 0; e < 4; ++e) part[i] = sd::dot2<T>(qop[i][e], one, part[i]);
     }
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i * NG / 4 == g) s += part[i];
+      qsum[g] = sd::sum_over_groups(s);
+      zsum[g] = 0.f;
+    }
+    m_run = -INFINITY;
+    l_run = 0.f;
+#pragma unroll
+    for (int t = 0; t < 8; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
   };
 
-  auto compute_step = [&](const Step<NG>& st) {
-    const int tb = cur.j * kChunk + wave * kStep;
-    if (tb >= cur.L) return;  // wave-uniform
-    // ---- scales to LDS in fp32: key (s c, (z - 16 s) c) with c = softmax scale * log2(e), value
-      //    (s, z - 16 s); lane 2 k (2 k + 1) holds key k's key (value) scales
-    {
-      float* d = &lds_s[wave][lane >> 1][2 * NG * (lane & 1)];
-      const float f = lane & 1 ? 1.f : p.scale_log2;
+  // ---- LDS addresses of the operand reads (see the loads for the order of a row's units)
+  const uint32_t k_at = lr * 128 + ((lg ^ (lr & 7)) * 16);
+  uint32_t v_at[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    v_at[j] = (4 * lg + j) * 128 + (((lr >> 2) ^ j) + 4 * (1 ^ (lg & 1))) * 16 + 4 * (lr & 3);
+  float* const sf = reinterpret_cast<float*>(mine + kAhead * slot_bytes<NG>());  // [key][4 NG]
+  const uint32_t kbase = sd::code_base<T>(), vbase = sd::code_base<__bf16>();
+
+  auto compute = [&](const u32x4 (&kw)[2], const uint32_t (&vw)[8], int tb, auto full_) {
+    constexpr bool kFull = decltype(full_)::value;
+    // ---- scores in log2 units, from the products with the codes: there a lane holds keys
+    //      16 tt + 4 lg + i of row lr
+    float sc[NE];
+    f32x4 dot[NG][2];
+    auto score = [&](int e, int tt, int i) {
+      const float* s = sf + key_of(e) * 4 * NG;
+      float v = 0.f;
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
-        const float s = sd::from_bits<T>(static_cast<uint16_t>(st.s[g]));
-        const float z = sd::from_bits<T>(static_cast<uint16_t>(st.s[g] >> 16));
-        d[g] = s * f;
-        d[NG + g] = (z - 16.f * s) * f;
+        float d = dot[g][tt][i];
+        if constexpr (R4) {
+          d = merge_dpp<kShr4, 0x2>(d, dot[g][0][2 + e]);
+          d = merge_dpp<kShr8, 0x4>(d, dot[g][1][e]);
+          d = merge_dpp<kShr12, 0x8>(d, dot[g][1][2 + e]);
+        }
+        v = fmaf(s[g], d, fmaf(s[NG + g], qsum[g], v));
       }
-    }
-    sd::wave_lds_sync();
-    // ---- scores (log2 units): lane holds key tb + 16 tt + 4 lg + i of row lr
-    float sc[RT][8];
+      sc[e] = kFull || tb + key_of(e) <= lim ? v : -INFINITY;
+    };
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt) {
-      u32x4 ka[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) ka[i] = sd::unpack8<T>(st.k[tt][i]);
-      f32x4 dot[RT][NG];
+      for (int g = 0; g < NG; ++g) {
+        f32x4 c = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
+        for (int i = 0; i < 4; ++i)
+          if (i * NG / 4 == g) c = sd::Elem<T>::mfma(sd::unpack8<T>(kw[tt][i], kbase), qop[i], c);
+        dot[g][tt] = c;
+      }
+      if constexpr (!R4) {
 #pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          f32x4 c = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (i * NG / 4 == g) c = sd::Elem<T>::mfma(ka[i], qop[rt][i], c);
-          dot[rt][g] = c;
-        }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float* ks = lds_s[wave][16 * tt + 4 * lg + i];
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          float s = 0.f;
-#pragma unroll
-          for (int g = 0; g < NG; ++g) s = fmaf(ks[g], dot[rt][g][i], fmaf(ks[NG + g], qsum[rt][g], s));
-          sc[rt][4 * tt + i] = s;
-        }
+        for (int i = 0; i < 4; ++i) score(4 * tt + i, tt, i);
       }
     }
-    const bool full = tb + kStep - 1 <= min(causal, cur.L - 1);
-    if (!full) {
+    if constexpr (R4) {
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int tok = tb + (e < 4 ? 4 * lg + e : 12 + 4 * lg + e);
-          sc[rt][e] = tok <= lim[rt] ? sc[rt][e] : -INFINITY;
-        }
+      for (int e = 0; e < 2; ++e) score(e, 0, e);
     }
     // ---- online softmax; the running maximum moves only when a score exceeds it by more than 8
     //      (log2 units): p <= 2^8 otherwise, well inside fp32 and the bf16 parts
-    u32x4 hi[RT][NG], lo[RT][NG];
+    float mloc = sc[0];
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      float mloc = sc[rt][0];
-#pragma unroll
-      for (int e = 1; e < 8; ++e) mloc = fmaxf(mloc, sc[rt][e]);
-      if (__any(mloc > m_run[rt] + 8.f)) {
-        const float mnew = fmaxf(m_run[rt], sd::max_over_groups(mloc));
-        const float alpha = sd::fast_exp2(m_run[rt] - (mnew == -INFINITY ? 0.f : mnew));
-        l_run[rt] *= alpha;
-#pragma unroll
-        for (int g = 0; g < NG; ++g) zsum[rt][g] *= alpha;
-#pragma unroll
-        for (int t = 0; t < 8; ++t) acc[rt][t] *= alpha;
-        m_run[rt] = mnew;
+    for (int e = 1; e < NE; ++e) mloc = fmaxf(mloc, sc[e]);
+    if (__any(mloc > m_run + 8.f)) {
+      mloc = sd::max_over_groups(mloc);
+      if constexpr (R4) {
+        mloc = fmaxf(mloc, __uint_as_float(move_dpp<kRor4>(__float_as_uint(mloc))));
+        mloc = fmaxf(mloc, __uint_as_float(move_dpp<kRor8>(__float_as_uint(mloc))));
       }
-      const float mb = m_run[rt] == -INFINITY ? 0.f : m_run[rt];
-      float pv[8], ps[NG][8];
+      const float mnew = fmaxf(m_run, mloc);
+      const float alpha = sd::fast_exp2(m_run - (mnew == -INFINITY ? 0.f : mnew));
+      l_run *= alpha;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        pv[e] = sd::fast_exp2(sc[rt][e] - mb);
-        l_run[rt] += pv[e];
-        const float* vs = &lds_s[wave][e < 4 ? 4 * lg + e : 12 + 4 * lg + e][2 * NG];
+      for (int g = 0; g < NG; ++g) zsum[g] *= alpha;
+#pragma unroll
+      for (int t = 0; t < 8; ++t) acc[t] *= alpha;
+      m_run = mnew;
+    }
+    const float mb = m_run == -INFINITY ? 0.f : m_run;
+    u32x4 hi[NG], lo[NG];
+#pragma unroll
+    for (int e2 = 0; e2 < NE / 2; ++e2) {
+      float ps[2][NG];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int e = 2 * e2 + u;
+        const float pv = sd::fast_exp2(sc[e] - mb);
+        l_run += pv;
+        const float* s = sf + key_of(e) * 4 * NG + 2 * NG;
+        const bool seen = kFull || tb + key_of(e) <= lim;
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-          float s = vs[g], z = vs[NG + g];
-          if (!full) {  // a key that this row does not see may hold anything
-            const bool seen = tb + (e < 4 ? 4 * lg + e : 12 + 4 * lg + e) <= lim[rt];
-            s = seen ? s : 0.f;
-            z = seen ? z : 0.f;
-          }
-          ps[g][e] = pv[e] * s;
-          zsum[rt][g] = fmaf(pv[e], z, zsum[rt][g]);
+          // a key that this row does not see may hold anything
+          ps[u][g] = pv * (seen ? s[g] : 0.f);
+          zsum[g] = fmaf(pv, seen ? s[NG + g] : 0.f, zsum[g]);
         }
       }
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
-        uint32_t h[4], l[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sd::split_pack<__bf16>(ps[g][2 * e], ps[g][2 * e + 1], h[e], l[e]);
-        hi[rt][g] = u32x4{h[0], h[1], h[2], h[3]};
-        lo[rt][g] = u32x4{l[0], l[1], l[2], l[3]};
+        uint32_t h, l;
+        sd::split_pack<__bf16>(ps[0][g], ps[1][g], h, l);
+        if constexpr (R4) {
+          hi[g] = u32x4{h, move_dpp<kShl4>(h), move_dpp<kShl8>(h), move_dpp<kShl12>(h)};
+          lo[g] = u32x4{l, move_dpp<kShl4>(l), move_dpp<kShl8>(l), move_dpp<kShl12>(l)};
+        } else {
+          hi[g][e2] = h;
+          lo[g][e2] = l;
+        }
       }
     }
     // ---- O^T += V^T P^T: byte b of the 8 value dwords holds tiles 2 b (low half) and 2 b + 1
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
-      uint32_t even[4], odd[4];
+      u32x4 va, vb;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         // byte b of keys 2 e and 2 e + 1, each in the low byte of a half
-        const uint32_t z = __builtin_amdgcn_perm(st.v[2 * e + 1], st.v[2 * e],
-                                                 0x0c040c00u + 0x00010001u * b);
-        even[e] = sd::code_pair<__bf16, 0>(z);
-        odd[e] = sd::code_pair<__bf16, 4>(z);
+        const uint32_t z = __builtin_amdgcn_perm(vw[2 * e + 1], vw[2 * e], 0x0c040c00u + 0x00010001u * b);
+        va[e] = sd::code_pair<__bf16, 0>(z, vbase);
+        vb[e] = sd::code_pair<__bf16, 4>(z, vbase);
       }
-      const u32x4 va = {even[0], even[1], even[2], even[3]}, vb = {odd[0], odd[1], odd[2], odd[3]};
       const int g = b * NG / 4;
+      acc[2 * b] = sd::Elem<__bf16>::mfma(va, hi[g], acc[2 * b]);
+      acc[2 * b + 1] = sd::Elem<__bf16>::mfma(vb, hi[g], acc[2 * b + 1]);
+      acc[2 * b] = sd::Elem<__bf16>::mfma(va, lo[g], acc[2 * b]);
+      acc[2 * b + 1] = sd::Elem<__bf16>::mfma(vb, lo[g], acc[2 * b + 1]);
+    }
+  };
+
+  bool first_pair = true;
+  auto step = [&](int slot) {
+    const int tb = cur.j * kChunk + ks * kStep;
+    // the oldest step in flight has landed (anything issued after the newer ones only waits longer)
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kAhead - 1) * kLoads) : "memory");
+    const uint8_t* d = mine + slot * slot_bytes<NG>();
+    uint32_t raw[NG];
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        acc[rt][2 * b] = sd::Elem<__bf16>::mfma(va, hi[rt][g], acc[rt][2 * b]);
-        acc[rt][2 * b + 1] = sd::Elem<__bf16>::mfma(vb, hi[rt][g], acc[rt][2 * b + 1]);
-        acc[rt][2 * b] = sd::Elem<__bf16>::mfma(va, lo[rt][g], acc[rt][2 * b]);
-        acc[rt][2 * b + 1] = sd::Elem<__bf16>::mfma(vb, lo[rt][g], acc[rt][2 * b + 1]);
+    for (int g = 0; g < NG; ++g) raw[g] = reinterpret_cast<const uint32_t*>(d + kStep * kD)[lane * NG + g];
+    u32x4 kw[2];
+    uint32_t vw[8];
+#pragma unroll
+    for (int tt = 0; tt < 2; ++tt) kw[tt] = sd::load16(d + k_at + 2048 * tt);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      vw[j] = *reinterpret_cast<const uint32_t*>(d + v_at[j & 3] + 2048 * (j >> 2));
+    // ---- scales to LDS in fp32: key (s c, (z - 16 s) c) with c = softmax scale * log2(e), value
+    //      (s, z - 16 s); lane 2 k (2 k + 1) holds key k's key (value) scales
+    {
+      float* o = sf + lane * 2 * NG;
+      const float f = lane & 1 ? 1.f : p.scale_log2;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const float s = sd::from_bits<T>(static_cast<uint16_t>(raw[g]));
+        const float z = sd::from_bits<T>(static_cast<uint16_t>(raw[g] >> 16));
+        o[g] = s * f;
+        o[NG + g] = fmaf(-16.f, s, z) * f;
       }
+    }
+    // the slot's words are in registers: its next step may land
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    load_step(slot);
+    if (tb < cur.L) {  // wave-uniform
+      sd::wave_lds_sync();
+      if (tb + kStep - 1 <= min(causal, cur.L - 1)) compute(kw, vw, tb, std::true_type{});
+      else compute(kw, vw, tb, std::false_type{});
     }
     sd::wave_lds_sync();  // every lane has read the scales before the next step writes its own
   };
@@ -444,143 +564,200 @@ void int4_attn_main(Params p) {
   // Merges the waves' states of the current pair: rows of out where this run saw the whole pair, a
   // partial otherwise. Every wave comes here.
   auto flush = [&](bool whole_pair) {
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      const int row = rt * 16 + lr;
-      const float l = sd::sum_over_groups(l_run[rt]);
-      float* d = lds_m[wave][row];
-#pragma unroll
-      for (int g = 0; g < NG; ++g) zsum[rt][g] = sd::sum_over_groups(zsum[rt][g]);
-#pragma unroll
-      for (int t = 0; t < 8; ++t)
-        sd::store16(d + 16 * t + 4 * lg, __builtin_bit_cast(u32x4, acc[rt][t] + zsum[rt][t * NG / 8]));
-      if (lg == 0) {
-        d[kD] = m_run[rt];
-        d[kD + 1] = l;
-      }
-    }
-    __syncthreads();
-    const int rows = p.gq * sr.nq;
     float* slot = p.ws + (2 * static_cast<int64_t>(run) + (first_pair ? 0 : 1)) * p.rmax * kPitch;
-    for (int i = tid; i < rows * 32; i += kWaves * 64) {
-      const int row = i >> 5, c = i & 31;
-      float M = -INFINITY, l = 0.f;
+    const int rows = p.gq * sq.nq;
+    float l = sd::sum_over_groups(l_run);
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) M = fmaxf(M, lds_m[w][row][kD]);
-      f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int g = 0; g < NG; ++g) zsum[g] = sd::sum_over_groups(zsum[g]);
+    if constexpr (R4) {  // the four lanes of a row that share its scores
+      l = sd::dpp_add<kRor8>(sd::dpp_add<kRor4>(l));
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        const float m = lds_m[w][row][kD];
-        // no finite score: l is 0 (nothing seen), or NaN, which stays
-        const float f = m == -INFINITY ? lds_m[w][row][kD + 1] : exp2f(m - M);
-        l = fmaf(f, lds_m[w][row][kD + 1], l);
-        o += f * __builtin_bit_cast(f32x4, sd::load16(&lds_m[w][row][4 * c]));
-      }
-      if (whole_pair) {
-        // l is 0 only for a row that sees no key (NaN stays NaN)
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        store_row4<T>(p, sr, cur.h, row, c, o * inv);
-      } else {
-        float* d = slot + row * kPitch;
-        sd::store16(d + 4 * c, __builtin_bit_cast(u32x4, o));
-        if (c == 0) {
-          d[kD] = M;
+      for (int g = 0; g < NG; ++g) zsum[g] = sd::dpp_add<kRor8>(sd::dpp_add<kRor4>(zsum[g]));
+    }
+    for (int r8 = 0; r8 < 16 / kMergeRows && r8 * kMergeRows < rows; ++r8) {
+      if (lr / kMergeRows == r8) {
+        float* d = lds_m[wave][lr % kMergeRows];
+#pragma unroll
+        for (int t = 0; t < 8; ++t)
+          sd::store16(d + 16 * t + 4 * lg, __builtin_bit_cast(u32x4, acc[t] + zsum[t * NG / 8]));
+        if (lg == 0) {
+          d[kD] = m_run;
           d[kD + 1] = l;
         }
       }
+      __syncthreads();
+      const int r = tid >> 5, c = tid & 31;
+      static_assert(kMergeRows * 32 == kWaves * 64, "a thread takes 4 dims of a row of each tile");
+#pragma unroll
+      for (int t = 0; t < TS; ++t) {
+        const int row = 16 * t + kMergeRows * r8 + r;
+        if (row >= rows) continue;
+        float M = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int w = t; w < kWaves; w += TS) M = fmaxf(M, lds_m[w][r][kD]);
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = t; w < kWaves; w += TS) {
+          const float m = lds_m[w][r][kD], lw = lds_m[w][r][kD + 1];
+          // no finite score: l is 0 (nothing seen), or NaN, which stays
+          const float f = m == -INFINITY ? lw : exp2f(m - M);
+          sum = fmaf(f, lw, sum);
+          o += f * __builtin_bit_cast(f32x4, sd::load16(&lds_m[w][r][4 * c]));
+        }
+        if (whole_pair) {
+          // the sum is 0 only for a row that sees no key (NaN stays NaN)
+          store_row4<T>(p, sq, cur.h, row, c, o * (sum == 0.f ? 0.f : 1.f / sum));
+        } else {
+          float* d = slot + row * kPitch;
+          sd::store16(d + 4 * c, __builtin_bit_cast(u32x4, o));
+          if (c == 0) {
+            d[kD] = M;
+            d[kD + 1] = sum;
+          }
+        }
+      }
+      __syncthreads();
     }
-    __syncthreads();
   };
 
-  Step<NG> ring[kAhead];
 #pragma unroll
-  for (int i = 0; i < kAhead; ++i) load_step(ring[i]);
+  for (int i = 0; i < kAhead; ++i) load_step(i);
   begin_pair();
-  while (true) {
-    bool done = false;
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      compute_step(ring[i]);
-      load_step(ring[i]);
-      ++cur.j;
-      --left;
-      const bool ends = cur.j == cur.n;
-      if (ends || left == 0) {
-        flush(ends && !entered);
-        if (left == 0) {
-          done = true;
-          break;
-        }
-        entered = first_pair = false;
-        next_pair(p, cur);
-        begin_pair();
-      }
+  for (int slot = 0;; slot = slot + 1 == kAhead ? 0 : slot + 1) {
+    step(slot);
+    ++cur.j;
+    --left;
+    if (cur.j == cur.n || left == 0) {
+      flush(cur.j == cur.n && !entered);
+      if (left == 0) break;
+      entered = first_pair = false;
+      next_pair(cur);
+      sq = seq_at(cur.b);
+      begin_pair();
     }
-    if (done) break;
   }
+  // the loads that ran ahead land before the workgroup's LDS is another's
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
-// One workgroup a pair: rows of pairs that several runs share from their partials, zeros for
-// sequences without keys; a pair that one run saw whole is written already.
+// Rows of pairs that several runs share from their partials, zeros for sequences without keys; a
+// pair that one run saw whole is written already. 4 dims of a row a thread.
 template <typename T> __global__ __launch_bounds__(256) void int4_attn_combine(Params p) {
+  __shared__ __attribute__((aligned(16))) float part[8][kPitch];
+  const int tid = threadIdx.x, lane = tid & 63;
   const int b = blockIdx.x / p.hkv, h = blockIdx.x - b * p.hkv;
-  const int n = chunks_of(seq_keys_uniform(p, b));
-  const Rows sr = seq_rows(p, b);
-  const int rows = p.gq * sr.nq;
+  int total = 0, before = 0;
+  Seq sq;
+  if (p.num_seqs <= 64) {
+    const Seq s = lane_seq(p, min(lane, p.num_seqs - 1));
+    const int n = lane < p.num_seqs ? chunks_of(p, s.L) : 0;
+    const int incl = sd::wave_inclusive_sum(n);
+    total = __builtin_amdgcn_readlane(incl, 63);
+    before = __builtin_amdgcn_readlane(incl - n, b);
+    sq = seq_from_lane(s, b);
+  } else {
+    for (int c = lane; c < p.num_seqs; c += 64) {
+      const int n = chunks_of(p, lane_seq(p, c).L);
+      total += n;
+      before += c < b ? n : 0;
+    }
+    for (int off = 32; off > 0; off >>= 1) {
+      total += __shfl_xor(total, off);
+      before += __shfl_xor(before, off);
+    }
+    sq = uniform_seq(p, b);
+  }
+  const int n = chunks_of(p, sq.L), rows = p.gq * sq.nq;
+  const int half = tid >> 5, c = tid & 31;
   if (n == 0) {
-    for (int i = threadIdx.x; i < rows * 32; i += 256)
-      store_row4<T>(p, sr, h, i >> 5, i & 31, f32x4{0.f, 0.f, 0.f, 0.f});
+    for (int row = blockIdx.y * 8 + half; row < rows; row += gridDim.y * 8)
+      store_row4<T>(p, sq, h, row, c, f32x4{0.f, 0.f, 0.f, 0.f});
     return;
   }
-  const int S = (chunks_before(p, p.num_seqs) * p.hkv + p.runs - 1) / p.runs;
-  const int first = chunks_before(p, b) * p.hkv + h * n;
+  const int S = (total * p.hkv + p.runs - 1) / p.runs;
+  const int first = before * p.hkv + h * n;
   const int r0 = first / S, r1 = (first + n - 1) / S;
   if (r0 == r1) return;
-  for (int i = threadIdx.x; i < rows * 32; i += 256) {
-    const int row = i >> 5, c = i & 31;
+  // few partials: a half wave takes a row; many: the half waves share a row's
+  const bool share = r1 - r0 >= 8;
+  for (int row = share ? blockIdx.y : blockIdx.y * 8 + half; row < rows; row += share ? gridDim.y : gridDim.y * 8) {
+    float M = -INFINITY, l = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
     auto state = [&](int r) {
       return p.ws + ((2 * static_cast<int64_t>(r) + (first > r * S ? 1 : 0)) * p.rmax + row) * kPitch;
     };
-    float M = -INFINITY, l = 0.f;
-    for (int r = r0; r <= r1; ++r) M = fmaxf(M, state(r)[kD]);
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int r = r0; r <= r1; ++r) {
-      const float* s = state(r);
-      const float f = s[kD] == -INFINITY ? s[kD + 1] : exp2f(s[kD] - M);
-      l = fmaf(f, s[kD + 1], l);
-      o += f * __builtin_bit_cast(f32x4, sd::load16(s + 4 * c));
+    auto add = [&](float m2, float l2, f32x4 o2) {
+      const float m = fmaxf(M, m2);
+      // no finite score: l is 0 (nothing seen), or NaN, which stays
+      const float f = M == -INFINITY ? l : exp2f(M - m), f2 = m2 == -INFINITY ? l2 : exp2f(m2 - m);
+      l = l * f + l2 * f2;
+      o = o * f + o2 * f2;
+      M = m;
+    };
+    constexpr int kOnce = 4;  // loads in flight
+    const int by = share ? 8 : 1;
+    for (int r = share ? r0 + half : r0; r <= r1; r += by * kOnce) {
+      float2 ml[kOnce];
+      f32x4 v[kOnce];
+#pragma unroll
+      for (int i = 0; i < kOnce; ++i) {
+        const float* s = state(min(r + by * i, r1));
+        ml[i] = *reinterpret_cast<const float2*>(s + kD);
+        v[i] = __builtin_bit_cast(f32x4, sd::load16(s + 4 * c));
+      }
+#pragma unroll
+      for (int i = 0; i < kOnce; ++i)
+        if (r + by * i <= r1) add(ml[i].x, ml[i].y, v[i]);
     }
-    store_row4<T>(p, sr, h, row, c, o * (l == 0.f ? 0.f : 1.f / l));
+    if (!share) {
+      store_row4<T>(p, sq, h, row, c, o * (l == 0.f ? 0.f : 1.f / l));
+      continue;
+    }
+    sd::store16(&part[half][4 * c], __builtin_bit_cast(u32x4, o));
+    if (c == 0) {
+      part[half][kD] = M;
+      part[half][kD + 1] = l;
+    }
+    __syncthreads();
+    if (half == 0) {
+#pragma unroll
+      for (int i = 1; i < 8; ++i)
+        add(part[i][kD], part[i][kD + 1], __builtin_bit_cast(f32x4, sd::load16(&part[i][4 * c])));
+      store_row4<T>(p, sq, h, row, c, o * (l == 0.f ? 0.f : 1.f / l));
+    }
+    __syncthreads();
   }
 }
+
+// Keys of a chunk: fewer where two waves share them
+int64_t chunk_keys(int64_t rows) { return kStep * kWaves / (rows <= 16 ? 1 : 2); }
 
 struct Plan {
   int64_t runs;
   bool whole;
-  int rmax, RT;
+  int rmax;
 };
 
 Plan make_plan(int num_seqs, int max_qlen, int hq, int hkv, int64_t max_ctx, int num_splits) {
   Plan pl;
   pl.rmax = hq / hkv * max_qlen;
-  pl.RT = pl.rmax <= 16 ? 1 : 2;
   const int64_t pairs = static_cast<int64_t>(num_seqs) * hkv;
-  const int64_t most = (max_ctx + kChunk - 1) / kChunk;  // chunks of a pair
-  pl.whole = num_splits == 0 && most <= kWholeChunks;
+  pl.whole = num_splits == 0 && max_ctx <= kWholeKeys;
   if (pl.whole) {
     pl.runs = pairs;
   } else {
-    // one resident set of workgroups: 4 waves each, RT == 1 two workgroups a compute unit
-    pl.runs = num_splits > 0 ? pairs * num_splits : static_cast<int64_t>(sd::device_cus()) * (pl.RT == 1 ? 2 : 1);
-    if (pl.runs > pairs * most) pl.runs = pairs * most;
+    // one resident set of workgroups of 4 waves, two a compute unit
+    const int64_t chunk = chunk_keys(pl.rmax), most = pairs * ((max_ctx + chunk - 1) / chunk);
+    pl.runs = num_splits > 0 ? pairs * num_splits : 2ll * sd::device_cus();
+    if (pl.runs > most) pl.runs = most;
   }
   return pl;
 }
 
 bool plan_fits(int num_seqs, int hkv, int64_t max_ctx, int num_splits) {
-  const int64_t pairs = static_cast<int64_t>(num_seqs) * hkv;
+  const int64_t pairs = static_cast<int64_t>(num_seqs) * hkv, chunk = kStep * kWaves / 2;
   return max_ctx <= (1ll << 30) && pairs <= (1ll << 23) && num_splits <= (1 << 16) &&
-         pairs * ((max_ctx + kChunk - 1) / kChunk) <= (1ll << 30) &&
+         pairs * ((max_ctx + chunk - 1) / chunk) <= (1ll << 30) &&
          (num_splits == 0 || pairs * num_splits <= (1ll << 22));
 }
 
@@ -588,26 +765,32 @@ size_t ws_bytes(const Plan& pl) {
   return pl.whole ? 0 : static_cast<size_t>(2 * pl.runs) * pl.rmax * kPitch * sizeof(float);
 }
 
-template <typename T, int NG, int RT> void launch_main(const Params& p, hipStream_t st) {
+template <typename T, int NG, int TS, bool R4> void launch_main(const Params& p, hipStream_t st) {
+  const dim3 grid(p.runs), block(kWaves * 64);
   if (p.block_size % kStep == 0)
-    hipLaunchKernelGGL((int4_attn_main<T, NG, RT, true>), dim3(p.runs), dim3(kWaves * 64), 0, st, p);
+    hipLaunchKernelGGL((int4_attn_main<T, NG, TS, R4, kOnePage>), grid, block, 0, st, p);
+  else if (p.block_size % (kStep / 2) == 0)
+    hipLaunchKernelGGL((int4_attn_main<T, NG, TS, R4, kHalfPages>), grid, block, 0, st, p);
   else
-    hipLaunchKernelGGL((int4_attn_main<T, NG, RT, false>), dim3(p.runs), dim3(kWaves * 64), 0, st, p);
+    hipLaunchKernelGGL((int4_attn_main<T, NG, TS, R4, kAnyPages>), grid, block, 0, st, p);
+}
+
+template <typename T, int NG> void launch_rows(const Params& p, hipStream_t st) {
+  if (p.rmax <= 4) launch_main<T, NG, 1, true>(p, st);
+  else if (p.rmax <= 16) launch_main<T, NG, 1, false>(p, st);
+  else launch_main<T, NG, 2, false>(p, st);
 }
 
 template <typename T> int launch(const Params& p, const Plan& pl, int group, hipStream_t st) {
-  if (pl.RT == 1) {
-    if (group == 32) launch_main<T, 4, 1>(p, st);
-    else if (group == 64) launch_main<T, 2, 1>(p, st);
-    else launch_main<T, 1, 1>(p, st);
-  } else {
-    if (group == 32) launch_main<T, 4, 2>(p, st);
-    else if (group == 64) launch_main<T, 2, 2>(p, st);
-    else launch_main<T, 1, 2>(p, st);
-  }
+  if (group == 32) launch_rows<T, 4>(p, st);
+  else if (group == 64) launch_rows<T, 2>(p, st);
+  else launch_rows<T, 1>(p, st);
   const int rc = sd::check_launch("paged_attention_int4 main");
   if (rc != SD_OK || pl.whole) return rc;
-  hipLaunchKernelGGL((int4_attn_combine<T>), dim3(p.num_seqs * p.hkv), dim3(256), 0, st, p);
+  const int pairs = p.num_seqs * p.hkv;
+  // a workgroup a row while the pairs alone leave the device idle
+  const dim3 grid(pairs, pairs <= 1024 ? p.rmax : 1);
+  hipLaunchKernelGGL((int4_attn_combine<T>), grid, dim3(256), 0, st, p);
   return sd::check_launch("paged_attention_int4 combine");
 }
 
@@ -697,8 +880,12 @@ extern "C" int sd_paged_attention_int4(
     return SD_ERR_UNSUPPORTED;
   }
   if (codes_stride_pos < 0 || scales_stride_pos < 0 || codes_stride_pos > (1ll << 25) ||
-      scales_stride_pos > (1ll << 25)) {
-    sd::set_error("%s: position strides of the cache must lie in [0, 2^25]", what);
+      scales_stride_pos > (1ll << 24) || codes_stride_block < 0 || codes_stride_head < 0 ||
+      scales_stride_block < 0 || scales_stride_head < 0 || codes_stride_block >= (1ll << 32) ||
+      codes_stride_head >= (1ll << 32) || scales_stride_block >= (1ll << 31) ||
+      scales_stride_head >= (1ll << 31)) {
+    sd::set_error("%s: position strides of the cache must lie in [0, 2^25] bytes, block and head "
+                  "strides in [0, 2^32) bytes", what);
     return SD_ERR_UNSUPPORTED;
   }
   const Plan pl = make_plan(num_seqs, max_qlen, num_q_heads, num_kv_heads, max_ctx, num_splits);
@@ -713,12 +900,12 @@ extern "C" int sd_paged_attention_int4(
   p.q_stok = q_stride_tok;
   p.q_shead = q_stride_head;
   p.codes = static_cast<const uint8_t*>(codes);
-  p.c_sblk = codes_stride_block;
-  p.c_shead = codes_stride_head;
+  p.c_sblk = static_cast<uint32_t>(codes_stride_block);
+  p.c_shead = static_cast<uint32_t>(codes_stride_head);
   p.c_spos = static_cast<uint32_t>(codes_stride_pos);
   p.scales = static_cast<const uint8_t*>(scales);
-  p.s_sblk = 2 * scales_stride_block;
-  p.s_shead = 2 * scales_stride_head;
+  p.s_sblk = static_cast<uint32_t>(2 * scales_stride_block);
+  p.s_shead = static_cast<uint32_t>(2 * scales_stride_head);
   p.s_spos = static_cast<uint32_t>(2 * scales_stride_pos);
   p.num_blocks = static_cast<int32_t>(num_blocks);
   p.block_size = block_size;
@@ -742,6 +929,7 @@ extern "C" int sd_paged_attention_int4(
   p.runs = static_cast<int32_t>(pl.runs);
   p.whole = pl.whole;
   p.rmax = pl.rmax;
+  p.chunk_shift = __builtin_ctzll(chunk_keys(pl.rmax));
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == SD_BF16) return launch<__bf16>(p, pl, group_size, st);
   return launch<_Float16>(p, pl, group_size, st);

@@ -105,6 +105,7 @@ __global__ __launch_bounds__(W * 64) void w4a16_gemv(Args a) {
     for (int f = 0; f < 4 / FOLD; ++f)
       d.s[f] = load_scale(a, n * a.groups + min(kb + 32 * FOLD * f, a.K - 32) / a.group);
   };
+  const uint32_t base = sd::code_base<T>();
   const u32x4 m24 = {minus24<T>(), minus24<T>(), minus24<T>(), minus24<T>()};
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   auto compute = [&](const Block& d, int blk) {
@@ -119,7 +120,7 @@ __global__ __launch_bounds__(W * 64) void w4a16_gemv(Args a) {
         u32x4 x = reorder(d.x[i]);
         if (kb + 32 * i >= a.K) x = u32x4{0u, 0u, 0u, 0u};  // past the last column
         t = sd::Elem<T>::mfma(x, m24, t);
-        t = sd::Elem<T>::mfma(x, sd::unpack8<T>(w[i]), t);
+        t = sd::Elem<T>::mfma(x, sd::unpack8<T>(w[i], base), t);
       }
       acc += scale_value(a, d.s[f]) * t;
     }
@@ -204,6 +205,7 @@ __global__ __launch_bounds__(256) void w4a16_gemm(Args a) {
     }
   };
 
+  const uint32_t base = sd::code_base<T>();
   f32x4 acc[MT][NT];
 #pragma unroll
   for (int i = 0; i < MT; ++i)
@@ -222,7 +224,7 @@ __global__ __launch_bounds__(256) void w4a16_gemm(Args a) {
     for (int t = 0; t < NT; ++t) {
       const u32x4 w = turn(wr[t]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) wf[t][i] = sd::unpack8<T>(w[i]);
+      for (int i = 0; i < 4; ++i) wf[t][i] = sd::unpack8<T>(w[i], base);
 #pragma unroll
       for (int f = 0; f < NF; ++f) sv[t][f] = scale_value(a, sr[t][f]);
     }

@@ -164,11 +164,12 @@ SIGNATURES.update({
         _i32, _i64, _i32, _i32, _i32, _i32,  # max_qlen, total_q, seqs, hq, hkv, head_dim
         _f32, _i32, _p, _i64, _i64,      # scale, dtype, out, strides
         _p, _sz, _i32, _p]),             # workspace, bytes, num_splits, stream
+    "sd_w4a16_workspace_size": (_sz, [_i64, _i64, _i64, _i32]),
     "sd_w4a16_linear": (ctypes.c_int, [
         _p, _i64, _p, _i64,              # x, x_stride, w, w_stride
         _p, _i32, _i32, _p,              # scale, scale_dtype, group_size, bias
         _p, _i64, _i64, _i64, _i64,      # y, y_stride, M, N, K
-        _i32, _p]),                      # dtype, stream
+        _i32, _p, _sz, _p]),             # dtype, workspace, bytes, stream
 })
 
 _lib = None

@@ -10,9 +10,15 @@
 // columns (one group at a time), and the order 0, 4, 1, 5, 2, 6, 3, 7 that unpack8 leaves is met
 // by putting the activations in the same order.
 //
-// Up to 16 rows (w4a16_gemv): bound by the weights' bytes, N K / 2. A workgroup takes 16 weight rows,
-// its waves the 128-column blocks in turn; their sums meet in LDS. Above (w4a16_gemm): a tile of
-// activation rows goes to LDS once for the four waves, each with its own weight rows in registers.
+// Up to 32 rows (w4a16_rows): bound by the weights' bytes, N K / 2. A workgroup takes tiles of 16 weight
+// rows, its waves the columns in turn; their sums meet in LDS and are added in wave order.
+// Activations read by every wave from the caches instead of from LDS kept the address units busy: 75 us
+// at 1 x 151936 x 1024 against XXX.
+// Above (w4a16_gemm): a tile of activation rows goes straight to LDS for the workgroup's waves
+// (global_load_lds, one step of 128 columns ahead), weights to registers; K is split over workgroups
+// where the tiles alone leave compute units idle, and w4a16_reduce adds the slices in order.
+#include <type_traits>
+
 #include "int4.h"
 
 namespace {
@@ -26,25 +32,32 @@ struct Args {
   const uint8_t* w;
   int64_t ws;  // bytes
   const void* scale;
-  int32_t scale_dtype;
-  int32_t groups;  // per weight row
-  int32_t group;
+  int32_t scale_f16, scale_f32;  // the scales' type (neither: bf16)
+  int32_t groups;     // per weight row
+  uint64_t inv32;     // ceil(2^32 / (columns per group / 32))
   const uint16_t* bias;
   uint16_t* y;
   int64_t ys;
   int64_t M, N;
   int32_t K;
+  int32_t tiles;  // w4a16_rows: groups of weight tiles a workgroup
+  float* part;    // K slices: [slices][M][N] sums
+  int32_t tiles_m, tiles_n, slices;
 };
 
-// Raw bits of one scale (its conversion waits for the load only where it is used).
-__device__ __forceinline__ uint32_t load_scale(const Args& a, int64_t at) {
-  return a.scale_dtype == SD_F32 ? static_cast<const uint32_t*>(a.scale)[at]
-                                 : static_cast<const uint16_t*>(a.scale)[at];
+// Group of column k: k / 32 is below 2^15 and a group below 2^20 columns, where the product with the
+// rounded-up reciprocal is exact (the error stays below 2^15 * 2^15 / 2^32 of a group).
+__device__ __forceinline__ int group_of(const Args& a, int k) {
+  return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(k) >> 5) * a.inv32) >> 32);
 }
-__device__ __forceinline__ float scale_value(const Args& a, uint32_t bits) {
-  if (a.scale_dtype == SD_F32) return __uint_as_float(bits);
-  if (a.scale_dtype == SD_BF16) return __uint_as_float(bits << 16);
-  return sd::from_bits<_Float16>(static_cast<uint16_t>(bits));
+// S32: 32-bit scales. Raw bits: the conversion waits for the load only where it is used.
+template <bool S32> __device__ __forceinline__ uint32_t load_scale(const Args& a, int64_t at) {
+  if constexpr (S32) return static_cast<const uint32_t*>(a.scale)[at];
+  else return static_cast<const uint16_t*>(a.scale)[at];
+}
+template <bool S32> __device__ __forceinline__ float scale_value(const Args& a, uint32_t bits) {
+  if constexpr (S32) return __uint_as_float(bits);
+  else return a.scale_f16 ? sd::from_bits<_Float16>(static_cast<uint16_t>(bits)) : __uint_as_float(bits << 16);
 }
 
 // Dword i of lane group lg becomes dword lg of lane group i.
@@ -77,216 +90,540 @@ template <typename T> __device__ __forceinline__ uint32_t minus24() {  // two T 
   return __is_same(T, __bf16) ? 0xC1C0C1C0u : 0xCE00CE00u;
 }
 
-constexpr int kBlock = 128;  // columns of a step: one 16-byte load of weights a lane
+constexpr int kBlock = 128;  // columns of a step: 16 bytes of weights a lane
 
-// FOLD: MFMAs (32 columns each) between two scalings, 4, 2 or 1.
-template <typename T, int FOLD, int W>
-__global__ __launch_bounds__(W * 64) void w4a16_gemv(Args a) {
-  __shared__ float red[W][16][17];
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int lr = lane & 15, lg = lane >> 4;
-  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * 16;
-  const int64_t n = min(n0 + lr, a.N - 1);
-  const uint8_t* wrow = a.w + n * a.ws;
-  const uint16_t* xrow = a.x + min(static_cast<int64_t>(lr), a.M - 1) * a.xs;
-  const int blocks = (a.K + kBlock - 1) / kBlock;
+__device__ __forceinline__ void to_lds16(const void* base, uint32_t off, uint32_t l) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+               ::"s"(l), "v"(off), "s"(base) : "memory", "m0");
+}
+__device__ __forceinline__ uint32_t lds_addr(const void* l) {
+  return __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(
+      reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) void*)l)));
+}
 
-  struct Block {
-    u32x4 w, x[4];
-    uint32_t s[4 / FOLD];
-  };
-  auto load = [&](Block& d, int blk) {
-    const int kb = min(blk, blocks - 1) * kBlock;
-    d.w = sd::load16_stream(wrow + min(kb + 32 * lg, a.K - 32) / 2);
+// The 8 codes of a dword as 8 T of 16 + u in their own order (10 instructions where unpack8 takes 8,
+// for activations that cannot be reordered on their way to LDS).
+template <typename T> __device__ __forceinline__ u32x4 unpack8_in_order(uint32_t w, uint32_t base) {
+  // low (high) half bytes at the mantissa bits of a byte each; fp16: within a half, after the perm
+  if constexpr (__is_same(T, __bf16)) {
+    const uint32_t lo = w << 3, hi = w >> 1;
+    u32x4 r;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) d.x[i] = sd::load16(xrow + min(kb + 32 * i + 8 * lg, a.K - 8));
+    for (int b = 0; b < 4; ++b)
+      r[b] = (__builtin_amdgcn_perm(hi, lo, 0x0c040c00u + 0x00010001u * b) & sd::Magic<T>::kMask) | base;
+    return r;
+  } else {
+    const uint32_t hi = w >> 4;
+    u32x4 r;
 #pragma unroll
-    for (int f = 0; f < 4 / FOLD; ++f)
-      d.s[f] = load_scale(a, n * a.groups + min(kb + 32 * FOLD * f, a.K - 32) / a.group);
-  };
-  const uint32_t base = sd::code_base<T>();
-  const u32x4 m24 = {minus24<T>(), minus24<T>(), minus24<T>(), minus24<T>()};
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  auto compute = [&](const Block& d, int blk) {
-    const int kb = blk * kBlock;
-    const u32x4 w = turn(d.w);
-#pragma unroll
-    for (int f = 0; f < 4 / FOLD; ++f) {
-      f32x4 t = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int j = 0; j < FOLD; ++j) {
-        const int i = f * FOLD + j;
-        u32x4 x = reorder(d.x[i]);
-        if (kb + 32 * i >= a.K) x = u32x4{0u, 0u, 0u, 0u};  // past the last column
-        t = sd::Elem<T>::mfma(x, m24, t);
-        t = sd::Elem<T>::mfma(x, sd::unpack8<T>(w[i], base), t);
-      }
-      acc += scale_value(a, d.s[f]) * t;
-    }
-  };
-  constexpr int kAhead = 2;
-  Block ring[kAhead];
-#pragma unroll
-  for (int i = 0; i < kAhead; ++i) load(ring[i], wave + i * W);
-  for (int blk = wave; blk < blocks; blk += kAhead * W) {
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      if (blk + i * W < blocks) compute(ring[i], blk + i * W);
-      load(ring[i], blk + (i + kAhead) * W);
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) red[wave][4 * lg + i][lr] = acc[i];
-  __syncthreads();
-  for (int i = tid; i < 256; i += W * 64) {
-    const int m = i >> 4, c = i & 15;
-    if (m >= a.M || n0 + c >= a.N) continue;
-    float s = 0.f;
-#pragma unroll
-    for (int v = 0; v < W; ++v) s += red[v][m][c];
-    if (a.bias) s += sd::from_bits<T>(a.bias[n0 + c]);
-    a.y[m * a.ys + n0 + c] = sd::to_bits<T>(s);
+    for (int b = 0; b < 4; ++b)
+      r[b] = sd::code_pair<T, 0>(__builtin_amdgcn_perm(hi, w, 0x0c040c00u + 0x00010001u * b), base);
+    return r;
   }
 }
 
-// BM = 16 MT activation rows by BN = 64 NT weight rows; wave v has weight rows 16 NT v .. + 16 NT.
-template <typename T, int FOLD, int MT, int NT>
-__global__ __launch_bounds__(256) void w4a16_gemm(Args a) {
-  constexpr int BM = 16 * MT, BN = 64 * NT, NF = 4 / FOLD;
-  __shared__ __attribute__((aligned(16))) u32x4 lx[2][BM * 16];     // rows of 16 units of 8 columns
-  __shared__ __attribute__((aligned(16))) float lsum[2][NF][BM];    // -24 sum x of a fold's columns
+// Up to 2 XI rows. FOLD: MFMAs (32 columns each) between two scalings, 4, 2 or 1. A workgroup takes
+// `tiles` groups of NT tiles of 16 weight rows, one after another; its waves take a group's stages of 256
+// columns in turn. A stage's weights (whole 128-byte lines of each row) and activations go straight to
+// the wave's own LDS, kAhead stages ahead and on into the next group, so that the waves meet only where
+// their sums do. The scales of all rows lie in LDS in fp32.
+constexpr int kStage = 256;                   // columns of a stage
+constexpr int kTileBytes = 16 * kStage / 2;   // of a tile's weights in a stage
+constexpr int stage_bytes(int xi, int nt) { return nt * kTileBytes + xi * 1024; }
+constexpr int rows_ahead(int xi, int nt) { return xi == 1 && nt == 1 ? 3 : 2; }
+
+template <typename T, int FOLD, int XI, int NT>
+__global__ __launch_bounds__(XI == 16 ? 512 : 1024) void w4a16_rows(Args a) {
+  constexpr int NF = 4 / FOLD, MT = (XI + 7) / 8, R = 16 * MT;
+  constexpr int kAhead = rows_ahead(XI, NT), kBytes = stage_bytes(XI, NT);
+  extern __shared__ __attribute__((aligned(1024))) char sm[];
+  const int W = blockDim.x >> 6;
+  float* const red = reinterpret_cast<float*>(sm + W * kAhead * kBytes);  // [wave][tile][R][16]
+  float* const lscale = red + W * NT * R * 16;                            // [row of a group][pitch]
+  const int M = static_cast<int>(a.M), pitch = a.groups | 1;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 15, lg = lane >> 4;
-  const int64_t m0 = static_cast<int64_t>(blockIdx.x) * BM, n0 = static_cast<int64_t>(blockIdx.y) * BN;
-  const int blocks = (a.K + kBlock - 1) / kBlock;
+  const int first = blockIdx.x * a.tiles;
+  const int tiles = min(a.tiles, a.tiles_n - first);
+  const int64_t n0 = static_cast<int64_t>(first) * (16 * NT);
+  const int stages = (a.K + kStage - 1) / kStage;
 
-  // ---- activations: unit u of row r by the 16 threads u of each row
-  const int u = tid & 15, r0 = tid >> 4;
-  u32x4 xr[MT];
-  auto load_x = [&](int blk) {
-    const int k = min(blk * kBlock + 8 * u, a.K - 8);
+  // ---- loads. Weights: 8 rows an instruction, lane l unit (l % 8) ^ (l / 8) of row l / 8. Activations: 2
+  //      rows an instruction, lane l unit (l % 32) ^ (row % 16); rows past M repeat the last.
+  const uint32_t ws = static_cast<uint32_t>(a.ws);
+  const uint32_t unit = 16 * ((lane & 7) ^ (lane >> 3)), row0 = (lane >> 3) * ws;
+  uint32_t x_off[XI];
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
-      xr[i] = sd::load16(a.x + min(m0 + 16 * i + r0, a.M - 1) * a.xs + k);
-  };
-  auto put_x = [&](int blk, int buf) {
-    const bool in = blk * kBlock + 8 * u < a.K;
+  for (int i = 0; i < XI; ++i)
+    x_off[i] = static_cast<uint32_t>(min(2 * i + (lane >> 5), M - 1)) * static_cast<uint32_t>(2 * a.xs);
+  const char* const x0 = reinterpret_cast<const char*>(a.x);
+  char* const mine = sm + wave * kAhead * kBytes;
+  const uint32_t mine_at = lds_addr(mine);
+  int load_tile = 0, load_stage = wave;
+  auto load = [&](int slot) {  // past the last group: its last stage again, into a slot nobody reads
+    const int t = min(load_tile, tiles - 1), s = min(load_stage, stages - 1);
+    const int64_t n = n0 + static_cast<int64_t>(16 * NT) * t;
+    const uint8_t* base = a.w + n * a.ws + s * (kStage / 2);
+    const uint32_t most = static_cast<uint32_t>(min(a.N - 1 - n, static_cast<int64_t>(16 * NT - 1))) * ws;
+    const uint32_t u = min(unit, static_cast<uint32_t>(a.K / 2 - 16 - s * (kStage / 2)));
+    const uint32_t l = mine_at + slot * kBytes;
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      const u32x4 v = in ? reorder(xr[i]) : u32x4{0u, 0u, 0u, 0u};
-      const int r = 16 * i + r0;
-      lx[buf][r * 16 + (u ^ (r & 15))] = v;
-      float s = 0.f;
+    for (int i = 0; i < 2 * NT; ++i) to_lds16(base, min(row0 + 8 * i * ws, most) + u, l + 1024 * i);
+    const uint32_t last = static_cast<uint32_t>(2 * a.K - 16 - s * (2 * kStage));
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s = sd::dot2<T>(v[e], minus24<T>(), s);
-      s = sd::dpp_add<0xB1>(s);
-      s = sd::dpp_add<0x4E>(s);
-      if constexpr (FOLD >= 2) s = sd::dpp_add<0x141>(s);
-      if constexpr (FOLD >= 4) s = sd::dpp_add<0x140>(s);
-      if (u % (4 * FOLD) == 0) lsum[buf][u / (4 * FOLD)][r] = s;
+    for (int i = 0; i < XI; ++i)
+      to_lds16(x0 + s * (2 * kStage), x_off[i] + min(16u * ((lane & 31) ^ ((2 * i + (lane >> 5)) & 15)), last),
+               l + NT * kTileBytes + 1024 * i);
+    load_stage += W;
+    if (load_stage >= stages) {
+      load_stage = wave;
+      ++load_tile;
     }
   };
+  if (wave < stages) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) load(i);
+  }
+  const int srows = static_cast<int>(min(static_cast<int64_t>(16 * NT) * tiles, a.N - n0));
+  // 16 lanes take 16 neighbouring scales of a row, several such items at once
+  const int parts = (a.groups + 15) / 16, items = srows * parts;
+  auto copy_scales = [&](auto s32) {
+    constexpr bool kS32 = decltype(s32)::value;
+    constexpr int kOnce = 4;
+    for (int i0 = 0; i0 < items; i0 += kOnce * W * 4) {
+      uint32_t v[kOnce];
+      int at[kOnce];
+#pragma unroll
+      for (int o = 0; o < kOnce; ++o) {
+        at[o] = -1;
+        if (o && i0 + o * W * 4 >= items) continue;  // uniform
+        const int i = i0 + o * W * 4 + (tid >> 4), r = parts == 1 ? i : i / parts;
+        const int g = (i - r * parts) * 16 + (tid & 15);
+        const bool in = i < items && g < a.groups;
+        at[o] = in ? r * pitch + g : -1;
+        v[o] = load_scale<kS32>(a, n0 * a.groups + (in ? r * a.groups + g : 0));
+      }
+#pragma unroll
+      for (int o = 0; o < kOnce; ++o)
+        if (at[o] >= 0) lscale[at[o]] = scale_value<kS32>(a, v[o]);
+    }
+  };
+  if (a.scale_f32) copy_scales(std::true_type{});
+  else copy_scales(std::false_type{});
+  __syncthreads();
+
+  const uint32_t base = sd::code_base<T>();
+  const u32x4 m24 = {minus24<T>(), minus24<T>(), minus24<T>(), minus24<T>()};
+  f32x4 acc[MT][NT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) acc[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const uint32_t w_at = lr * 128 + ((lg ^ (lr & 7)) * 16);  // unit lg of row lr; the next block's: ^ 64
+  uint32_t x_row[MT];  // LDS row of this lane's operand row, and what its units are turned by
+  uint32_t x_turn[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    const int m = min(16 * i + lr, 2 * XI - 1);
+    x_row[i] = NT * kTileBytes + m * 512;
+    x_turn[i] = m & 15;
+  }
+  auto compute = [&](const char* st, const float* scale, int k) {
+#pragma unroll
+    for (int c = 0; c < kStage / kBlock; ++c) {
+      const int left = a.K - k - c * kBlock;  // columns of this block and after
+      if (left <= 0) break;                   // uniform
+      u32x4 w[NT];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        w[t] = sd::load16(st + t * kTileBytes + (w_at ^ (64 * c)));
+        // one group a block: any order of the columns will do, as long as the activations' is the same
+        if constexpr (FOLD < 4) w[t] = turn(w[t]);
+      }
+#pragma unroll
+      for (int f = 0; f < NF; ++f) {
+        if (FOLD < 4 && 32 * FOLD * f >= left) break;  // uniform
+        const int g = group_of(a, k + c * kBlock + 32 * FOLD * f);
+        u32x4 x[MT][FOLD];
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int j = 0; j < FOLD; ++j) {
+            const uint32_t u = 16 * c + (FOLD == 4 ? 4 * lg + j : 4 * (f * FOLD + j) + lg);
+            x[i][j] = sd::load16(st + x_row[i] + ((u ^ x_turn[i]) * 16));
+          }
+        f32x4 v[MT][NT];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          f32x4 start = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int j = 0; j < FOLD; ++j) start = sd::Elem<T>::mfma(x[i][j], m24, start);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) v[i][t] = start;
+        }
+#pragma unroll
+        for (int j = 0; j < FOLD; ++j)
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            const u32x4 wf = unpack8_in_order<T>(w[t][f * FOLD + j], base);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) v[i][t] = sd::Elem<T>::mfma(x[i][j], wf, v[i][t]);
+          }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const float sv = scale[t * 16 * pitch + g];
+#pragma unroll
+          for (int i = 0; i < MT; ++i) acc[i][t] += sv * v[i][t];
+        }
+      }
+    }
+  };
+
+  int slot = 0;
+  for (int t = 0; t < tiles; ++t) {
+    // rows past N: scales of rows past the group's, never written (the buffer holds whole groups)
+    const float* scale = lscale + (16 * NT * t + lr) * pitch;
+    for (int s = wave; s < stages; s += W) {
+      // the oldest stage has landed (loads issued after it only make this wait longer)
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((2 * NT + XI) * (kAhead - 1)) : "memory");
+      compute(mine + slot * kBytes, scale, s * kStage);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // its words are read
+      load(slot);
+      slot = slot + 1 == kAhead ? 0 : slot + 1;
+    }
+    // ---- the waves' sums meet in LDS
+    float* mr = red + wave * (NT * R * 16);
+#pragma unroll
+    for (int u = 0; u < NT; ++u)
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          mr[(u * R + 16 * i + 4 * lg + e) * 16 + lr] = acc[i][u][e];
+          acc[i][u][e] = 0.f;
+        }
+    __syncthreads();
+    for (int i = tid; i < 16 * NT * M; i += W * 64) {  // 16 NT neighbouring outputs of a row
+      const int m = i / (16 * NT), u = i / 16 % NT, c = i % 16;
+      const int64_t n = n0 + static_cast<int64_t>(16) * (NT * t + u) + c;
+      if (n >= a.N) continue;
+      const float* r = red + (u * R + m) * 16 + c;
+      float s = 0.f;
+      for (int v = 0; v < W; ++v) s += r[v * (NT * R * 16)];
+      if (a.bias) s += sd::from_bits<T>(a.bias[n]);
+      a.y[m * a.ys + n] = sd::to_bits<T>(s);
+    }
+    if (t + 1 < tiles) __syncthreads();
+  }
+  // the loads that ran ahead land before the workgroup's LDS is another's
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+
+// WM x WN waves of MT x NT tiles of 16 x 16 outputs; S stages of activations in LDS, S - 1 blocks of weights
+// in registers.
+template <typename T, int FOLD, bool S32, int WM, int WN, int MT, int NT, int S>
+__global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(2)))
+void w4a16_gemm(Args a) {
+  constexpr int NW = WM * WN, BM = 16 * MT * WM, BN = 16 * NT * WN, NF = 4 / FOLD;
+  constexpr int kRow = 2 * kBlock;                // bytes of an activation row's step
+  constexpr int CX = BM * kRow / 1024 / NW;       // 1 KB loads (4 rows) of a wave and step
+  static_assert(CX * NW * 1024 == BM * kRow, "whole 1 KB loads");
+  __shared__ __attribute__((aligned(1024))) uint8_t lx[S][BM * kRow];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lr = lane & 15, lg = lane >> 4;
+  const int wm = wave / WN, wn = wave % WN;
+
+  // Workgroup -> (slice, tile): every eighth workgroup shares an XCD (one L2), so each XCD takes a
+  // contiguous run of tiles, all activation tiles of a weight tile before the next.
+  const int items = a.tiles_m * a.tiles_n * a.slices;
+  int id = blockIdx.x;
+  {
+    const int per = items / 8, rem = items % 8, xcd = id % 8;
+    id = xcd * per + min(xcd, rem) + id / 8;
+  }
+  const int m_tile = id % a.tiles_m, rest = id / a.tiles_m;
+  const int slice = rest % a.slices, n_tile = rest / a.slices;
+  const int64_t m0 = static_cast<int64_t>(m_tile) * BM, n0 = static_cast<int64_t>(n_tile) * BN;
+  const int blocks = (a.K + kBlock - 1) / kBlock;
+  const int b0 = static_cast<int>(static_cast<int64_t>(slice) * blocks / a.slices);
+  const int b1 = static_cast<int>(static_cast<int64_t>(slice + 1) * blocks / a.slices);
+
+  // ---- activations: 16-byte unit u of row r stands at unit u ^ (r % 16) of its LDS row, so that the
+  //      16 rows of an operand read hit 16 different units
+  const char* xbase = reinterpret_cast<const char*>(a.x + m0 * a.xs);
+  static_assert(CX % 2 == 0, "a wave's rows start at a multiple of 8");
+  uint32_t xoff[CX];
+#pragma unroll
+  for (int i = 0; i < CX; ++i) {
+    const int r = (wave * CX + i) * 4 + lg;
+    xoff[i] = static_cast<uint32_t>(min(static_cast<int64_t>(r), a.M - 1 - m0) * a.xs * 2);
+  }
+  const uint32_t lx_at = lds_addr(&lx[0][0]);
+  const int blast = max(b1 - 1, b0);  // past the slice: its last block again, so that every step loads as much
+  auto load_x = [&](int blk, int buf) {
+    blk = min(blk, blast);
+    const uint32_t last = 2 * (a.K - blk * kBlock) - 16;  // the last unit of a row, past it again
+    const char* xb = xbase + static_cast<int64_t>(blk) * kRow;
+#pragma unroll
+    for (int i = 0; i < CX; ++i)
+      to_lds16(xb, xoff[i] + min(16u * (lr ^ (((wave * CX + i) * 4 + lg) & 15)), last), lx_at + buf * (BM * kRow) + (wave * CX + i) * 1024);
+  };
   // ---- weights and scales of this wave's rows
-  u32x4 wr[NT];
-  uint32_t sr[NT][NF];
-  int64_t nrow[NT];
+  u32x4 wr[S - 1][NT];
+  uint32_t sr[S - 1][NT][NF];
+  const uint8_t* const wbase = a.w + n0 * a.ws;
+  const int64_t sbase = n0 * a.groups;
+  uint32_t wrow[NT], srow[NT];  // from the tile's first row
 #pragma unroll
-  for (int t = 0; t < NT; ++t) nrow[t] = min(n0 + (wave * NT + t) * 16 + lr, a.N - 1);
-  auto load_w = [&](int blk) {
-    const int kb = blk * kBlock;
+  for (int t = 0; t < NT; ++t) {
+    const uint32_t n = static_cast<uint32_t>(min(n0 + (wn * NT + t) * 16 + lr, a.N - 1) - n0);
+    wrow[t] = n * static_cast<uint32_t>(a.ws);
+    srow[t] = n * static_cast<uint32_t>(a.groups);
+  }
+  auto load_w = [&](int blk, int r) {
+    const int kb = min(blk, blast) * kBlock;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      wr[t] = sd::load16(a.w + nrow[t] * a.ws + min(kb + 32 * lg, a.K - 32) / 2);
+    for (int t = 0; t < NT; ++t)
+      wr[r][t] = sd::load16(wbase + (wrow[t] + static_cast<uint32_t>(min(kb + 32 * lg, a.K - 32) / 2)));
 #pragma unroll
-      for (int f = 0; f < NF; ++f)
-        sr[t][f] = load_scale(a, nrow[t] * a.groups + min(kb + 32 * FOLD * f, a.K - 32) / a.group);
+    for (int f = 0; f < NF; ++f) {
+      const int g = group_of(a, min(kb + 32 * FOLD * f, a.K - 32));
+#pragma unroll
+      for (int t = 0; t < NT; ++t) sr[r][t][f] = load_scale<S32>(a, sbase + (srow[t] + static_cast<uint32_t>(g)));
     }
   };
 
   const uint32_t base = sd::code_base<T>();
+  const u32x4 m24 = {minus24<T>(), minus24<T>(), minus24<T>(), minus24<T>()};
   f32x4 acc[MT][NT];
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
     for (int t = 0; t < NT; ++t) acc[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  load_x(0);
-  load_w(0);
-  put_x(0, 0);
-  __syncthreads();
-  for (int blk = 0; blk < blocks; ++blk) {
-    const int buf = blk & 1;
+  uint32_t x_at[4];  // operand reads: unit 4 j + lg of row lr of a tile
+#pragma unroll
+  for (int j = 0; j < 4; ++j) x_at[j] = (wm * MT * 16 + lr) * kRow + (((4 * j + lg) ^ lr) * 16);
+
+  constexpr int kLoads = CX + NT + NT * NF;  // vector memory instructions of a step
+#pragma unroll
+  for (int i = 0; i < S - 1; ++i) {
+    load_x(b0 + i, i);
+    load_w(b0 + i, i);
+  }
+  auto step = [&](int blk, int r) {  // r: blk's slot of the weights (a constant)
+    const int buf = (blk - b0) % S;
+    // this step's activations have landed in every wave's view, the last step's are read
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((S - 2) * kLoads) : "memory");
     u32x4 wf[NT][4];
     float sv[NT][NF];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const u32x4 w = turn(wr[t]);
+      const u32x4 w = turn(wr[r][t]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) wf[t][i] = sd::unpack8<T>(w[i], base);
+      for (int i = 0; i < 4; ++i) wf[t][i] = unpack8_in_order<T>(w[i], base);
 #pragma unroll
-      for (int f = 0; f < NF; ++f) sv[t][f] = scale_value(a, sr[t][f]);
+      for (int f = 0; f < NF; ++f) sv[t][f] = scale_value<S32>(a, sr[r][t][f]);
     }
-    const int next = min(blk + 1, blocks - 1);
-    load_x(next);
-    load_w(next);
+    load_x(blk + S - 1, (buf + S - 1) % S);
+    load_w(blk + S - 1, r);
+    const int valid = min(4, (a.K - blk * kBlock) / 32);  // 32-column parts of this block
+    u32x4 xs[2][4];  // operands of a tile and of the next
+#pragma unroll
+    for (int j = 0; j < 4; ++j) xs[0][j] = sd::load16(&lx[buf][x_at[j]]);
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-      u32x4 xf[4];
+      u32x4(&xf)[4] = xs[i & 1];
+      if (i + 1 < MT) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) xf[j] = lx[buf][(16 * i + lr) * 16 + ((4 * j + lg) ^ lr)];
+        for (int j = 0; j < 4; ++j) xs[(i + 1) & 1][j] = sd::load16(&lx[buf][x_at[j] + (i + 1) * 16 * kRow]);
+      }
+      if (valid < 4) {
+#pragma unroll
+        for (int j = 1; j < 4; ++j)
+          if (j >= valid) xf[j] = u32x4{0u, 0u, 0u, 0u};
+      }
 #pragma unroll
       for (int f = 0; f < NF; ++f) {
-        const f32x4 start = __builtin_bit_cast(f32x4, sd::load16(&lsum[buf][f][16 * i + 4 * lg]));
+        f32x4 start = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          f32x4 d = start;
+        for (int j = 0; j < FOLD; ++j) start = sd::Elem<T>::mfma(xf[f * FOLD + j], m24, start);
+        f32x4 d[NT];
 #pragma unroll
-          for (int j = 0; j < FOLD; ++j) d = sd::Elem<T>::mfma(xf[f * FOLD + j], wf[t][f * FOLD + j], d);
-          acc[i][t] += sv[t][f] * d;
-        }
+        for (int t = 0; t < NT; ++t) d[t] = start;
+#pragma unroll
+        for (int j = 0; j < FOLD; ++j)
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+            d[t] = sd::Elem<T>::mfma(xf[f * FOLD + j], wf[t][f * FOLD + j], d[t]);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[i][t] += sv[t][f] * d[t];
       }
+      // one tile after another: with all tiles' operands hoisted the accumulators spill
+      __builtin_amdgcn_sched_barrier(0);
     }
-    if (blk + 1 < blocks) put_x(blk + 1, buf ^ 1);
-    __syncthreads();
+  };
+  for (int blk = b0; blk < b1; blk += S - 1) {
+#pragma unroll
+    for (int r = 0; r < S - 1; ++r)
+      if (blk + r < b1) step(blk + r, r);
   }
+  // the loads that ran ahead land before the workgroup's LDS is another's
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
-    const int64_t n = n0 + (wave * NT + t) * 16 + lr;
+    const int64_t n = n0 + (wn * NT + t) * 16 + lr;
     if (n >= a.N) continue;
-    const float b = a.bias ? sd::from_bits<T>(a.bias[n]) : 0.f;
+    const float b = a.bias && a.slices == 1 ? sd::from_bits<T>(a.bias[n]) : 0.f;
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int64_t m = m0 + 16 * i + 4 * lg + e;
-        if (m < a.M) a.y[m * a.ys + n] = sd::to_bits<T>(acc[i][t][e] + b);
+        const int64_t m = m0 + (wm * MT + i) * 16 + 4 * lg + e;
+        if (m >= a.M) continue;
+        if (a.slices > 1) a.part[(slice * a.M + m) * a.N + n] = acc[i][t][e];
+        else a.y[m * a.ys + n] = sd::to_bits<T>(acc[i][t][e] + b);
       }
   }
 }
 
-template <typename T, int FOLD> int launch(const Args& a, hipStream_t st) {
-  if (a.M <= 16) {
-    const dim3 grid(static_cast<unsigned>((a.N + 15) / 16));
-    hipLaunchKernelGGL((w4a16_gemv<T, FOLD, 4>), grid, dim3(256), 0, st, a);
-  } else {
-    auto grid = [&](int bm, int bn) {
-      return dim3(static_cast<unsigned>((a.M + bm - 1) / bm), static_cast<unsigned>((a.N + bn - 1) / bn));
-    };
-    if (a.M <= 32) hipLaunchKernelGGL((w4a16_gemm<T, FOLD, 2, 1>), grid(32, 64), dim3(256), 0, st, a);
-    else if (a.M <= 256) hipLaunchKernelGGL((w4a16_gemm<T, FOLD, 4, 2>), grid(64, 128), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((w4a16_gemm<T, FOLD, 8, 4>), grid(128, 256), dim3(256), 0, st, a);
+// Sum of the K slices, in slice order, bias, rounding.
+template <typename T> __global__ __launch_bounds__(256) void w4a16_reduce(Args a) {
+  const int64_t all = a.M * a.N;
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < all; i += gridDim.x * 256ll) {
+    const int64_t m = i / a.N, n = i - m * a.N;
+    float s = 0.f;
+    for (int v = 0; v < a.slices; ++v) s += a.part[v * all + i];
+    if (a.bias) s += sd::from_bits<T>(a.bias[n]);
+    a.y[m * a.ys + n] = sd::to_bits<T>(s);
   }
+}
+
+// What runs a shape: up to 32 rows w4a16_rows<XI, NT> of W waves and its groups a workgroup; above (and
+// where a row has so many groups that a tile's scales leave LDS no room) tiles of bm x bn and K slices.
+struct Plan {
+  int XI, NT, W, tiles;  // XI == 0: w4a16_gemm
+  size_t lds;
+  int bm, bn, slices;
+};
+Plan make_plan(int64_t M, int64_t N, int64_t K, int64_t group) {
+  Plan pl{};
+  const int64_t cus = sd::device_cus(), blocks = (K + kBlock - 1) / kBlock;
+  const int fold = group % 128 == 0 ? 4 : group % 64 == 0 ? 2 : 1;
+  const int64_t all = (N + 15) / 16, stages = (K + kStage - 1) / kStage;  // weight tiles, their stages
+  pl.XI = M <= 2 ? 1 : M <= 8 ? 4 : M <= 16 ? 8 : 16;
+  // Every wave reads its own share of x: past 8 rows that is more than the weights. Tiles of w4a16_gemm
+  // share it: 16 x 151936 x 1024 33 us there and XXX here; past 16 rows (32 x 19456 x 2560 XXX and 30 us)
+  // only layers of few tiles and stages stay (32 x 4096 x 1024 5.2 us here and XXX).
+  if (M <= 8 || (M <= 16 && all < 16 * cus) || (M <= 32 && all <= cus && stages <= 8)) {
+    // tiles that share what a wave reads of x: as many as leave every compute unit a workgroup
+    pl.NT = all < 4 * cus || pl.XI == 16 ? 1 : pl.XI == 8 ? 4 : 2;
+    const int64_t groups = (all + pl.NT - 1) / pl.NT;
+    auto bytes = [&](int64_t tiles, int W) {
+      return static_cast<size_t>(W) * (rows_ahead(pl.XI, pl.NT) * stage_bytes(pl.XI, pl.NT) +
+                                       pl.NT * ((pl.XI + 7) / 8) * 1024) +
+             static_cast<size_t>(tiles) * pl.NT * 16 * ((K / group) | 1) * 4;
+    };
+    constexpr size_t kMost = 150 << 10;
+    // waves: no more than there are stages, more where the tiles are too few for the device
+    // (1 x 2560 x 9728: 9.0 us with 4, 7.2 with 8; 1 x 4096 x 1024 3.4 with 4, 3.6 with 8)
+    pl.W = 4;
+    while (pl.W < (pl.XI == 16 ? 8 : 16) && groups * pl.W < 4 * cus && pl.W < stages && bytes(1, 2 * pl.W) <= kMost)
+      pl.W *= 2;
+    while (pl.W > 1 && bytes(1, pl.W) > kMost) pl.W /= 2;
+    // groups a workgroup: one up to four workgroups a compute unit (1 x 19456 x 2560, 608 groups: 8.8 us,
+    // 12.0 with two), then their share (1 x 151936 x 1024, 4748 groups: 23.8 us with four, 25.6 with one)
+    pl.tiles = static_cast<int>(groups / (4 * cus));
+    if (pl.tiles < 1) pl.tiles = 1;
+    while (pl.tiles > 1 && bytes(pl.tiles, pl.W) > bytes(1, pl.W) + (8 << 10)) --pl.tiles;
+    pl.lds = bytes(pl.tiles, pl.W);
+    if (pl.lds <= (160 << 10)) return pl;
+  }
+  pl.XI = 0;
+  pl.bm = M <= 32 ? 32 : M <= 64 ? 64 : 128;
+  if (M > 64) pl.bn = fold < 4 ? 64 : 128;  // (a scale for every one or two MFMAs: too many registers for 128)
+  else pl.bn = (N + 127) / 128 * 4 < 2 * cus ? 64 : 128;
+  const int64_t tiles = ((M + pl.bm - 1) / pl.bm) * ((N + pl.bn - 1) / pl.bn);
+  // two workgroups a compute unit, slices of two steps or more
+  int64_t s = tiles >= cus ? 1 : (2 * cus) / tiles;
+  if (s > blocks / 2) s = blocks / 2;
+  pl.slices = s < 1 ? 1 : s > 16 ? 16 : static_cast<int>(s);
+  return pl;
+}
+
+template <typename T, int FOLD, int XI> void launch_rows(const Args& a, const Plan& pl, hipStream_t st) {
+  const dim3 grid(static_cast<unsigned>((a.tiles_n + pl.tiles - 1) / pl.tiles)), block(pl.W * 64);
+  if (pl.NT == 1) hipLaunchKernelGGL((w4a16_rows<T, FOLD, XI, 1>), grid, block, pl.lds, st, a);
+  else if (pl.NT == 2) hipLaunchKernelGGL((w4a16_rows<T, FOLD, XI, 2>), grid, block, pl.lds, st, a);
+  else if constexpr (XI == 4 || XI == 8) hipLaunchKernelGGL((w4a16_rows<T, FOLD, XI, 4>), grid, block, pl.lds, st, a);
+}
+
+template <typename T, int FOLD, bool S32> void launch_gemm(const Args& a, const Plan& pl, dim3 grid, hipStream_t st) {
+  const dim3 block(256);
+  if (pl.bm == 128)
+    hipLaunchKernelGGL((w4a16_gemm<T, FOLD, S32, 2, 2, 4, FOLD < 4 ? 2 : 4, 2>), grid, block, 0, st, a);
+  else if (pl.bm == 64 && pl.bn == 128)
+    hipLaunchKernelGGL((w4a16_gemm<T, FOLD, S32, 1, 4, 4, 2, 4>), grid, block, 0, st, a);
+  else if (pl.bm == 64)
+    hipLaunchKernelGGL((w4a16_gemm<T, FOLD, S32, 1, 4, 4, 1, 4>), grid, block, 0, st, a);
+  else if (pl.bn == 128)
+    hipLaunchKernelGGL((w4a16_gemm<T, FOLD, S32, 1, 4, 2, 2, 4>), grid, block, 0, st, a);
+  else
+    hipLaunchKernelGGL((w4a16_gemm<T, FOLD, S32, 1, 4, 2, 1, 4>), grid, block, 0, st, a);
+}
+
+template <typename T, int FOLD> int launch(Args a, int64_t group, hipStream_t st) {
+  const Plan pl = make_plan(a.M, a.N, a.K, group);
+  if (pl.XI) {
+    a.tiles = pl.tiles;
+    a.tiles_n = static_cast<int32_t>((a.N + 16 * pl.NT - 1) / (16 * pl.NT));
+    if (pl.XI == 1) launch_rows<T, FOLD, 1>(a, pl, st);
+    else if (pl.XI == 4) launch_rows<T, FOLD, 4>(a, pl, st);
+    else if (pl.XI == 8) launch_rows<T, FOLD, 8>(a, pl, st);
+    else launch_rows<T, FOLD, 16>(a, pl, st);
+    return sd::check_launch("w4a16_linear");
+  }
+  a.slices = a.part ? pl.slices : 1;  // without its workspace: one slice
+  a.tiles_m = static_cast<int32_t>((a.M + pl.bm - 1) / pl.bm);
+  a.tiles_n = static_cast<int32_t>((a.N + pl.bn - 1) / pl.bn);
+  const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.tiles_m) * a.tiles_n * a.slices));
+  if (a.scale_f32) launch_gemm<T, FOLD, true>(a, pl, grid, st);
+  else launch_gemm<T, FOLD, false>(a, pl, grid, st);
+  const int rc = sd::check_launch("w4a16_linear");
+  if (rc != SD_OK || a.slices == 1) return rc;
+  int64_t wgs = (a.M * a.N + 255) / 256;
+  if (wgs > 2048) wgs = 2048;
+  hipLaunchKernelGGL((w4a16_reduce<T>), dim3(static_cast<unsigned>(wgs)), dim3(256), 0, st, a);
   return sd::check_launch("w4a16_linear");
+}
+
+template <typename T> int launch(const Args& a, int group, hipStream_t st) {
+  if (group % 128 == 0) return launch<T, 4>(a, group, st);
+  if (group % 64 == 0) return launch<T, 2>(a, group, st);
+  return launch<T, 1>(a, group, st);
+}
+
+// (a launch takes fewer than 2^32 threads: tiles of 128 x 64 and 256 threads, 16 slices while tiles are few)
+bool sizes_ok(int64_t M, int64_t N, int64_t K) {
+  return M <= (1ll << 24) && N <= (1ll << 21) && K <= (1ll << 20) &&
+         ((M + 127) / 128) * ((N + 63) / 64) < (1ll << 24);
 }
 
 }  // namespace
 
+extern "C" size_t sd_w4a16_workspace_size(int64_t M, int64_t N, int64_t K, int32_t group_size) {
+  if (M <= 0 || N <= 0 || K <= 0 || group_size <= 0 || !sizes_ok(M, N, K)) return 0;
+  const Plan pl = make_plan(M, N, K, group_size);
+  return pl.slices > 1 ? static_cast<size_t>(pl.slices) * M * N * sizeof(float) : 0;
+}
+
 extern "C" int sd_w4a16_linear(const void* x, int64_t x_stride_m, const uint8_t* w, int64_t w_stride_n,
                                const void* scale, int32_t scale_dtype, int32_t group_size,
                                const void* bias, void* y, int64_t y_stride_m, int64_t M, int64_t N,
-                               int64_t K, int32_t dtype, void* stream) {
+                               int64_t K, int32_t dtype, void* workspace, size_t workspace_bytes,
+                               void* stream) {
   sd::clear_error();
   const char* what = "w4a16_linear";
   if (M < 0 || N <= 0 || K <= 0 || group_size <= 0) {
@@ -304,8 +641,9 @@ extern "C" int sd_w4a16_linear(const void* x, int64_t x_stride_m, const uint8_t*
     sd::set_error("%s: dtype must be bf16 or f16, the scales' bf16, f16 or f32", what);
     return SD_ERR_UNSUPPORTED;
   }
-  if (M > (1ll << 24) || N > (1ll << 21) || K > (1ll << 24)) {
-    sd::set_error("%s: M=%lld N=%lld K=%lld too large", what, (long long)M, (long long)N, (long long)K);
+  if (!sizes_ok(M, N, K) || x_stride_m > (1ll << 24) || w_stride_n > (1ll << 24)) {
+    sd::set_error("%s: M=%lld N=%lld K=%lld (strides %lld, %lld) too large", what, (long long)M, (long long)N,
+                  (long long)K, (long long)x_stride_m, (long long)w_stride_n);
     return SD_ERR_UNSUPPORTED;
   }
   if (M == 0) return SD_OK;
@@ -333,18 +671,20 @@ extern "C" int sd_w4a16_linear(const void* x, int64_t x_stride_m, const uint8_t*
   a.w = w;
   a.ws = w_stride_n;
   a.scale = scale;
-  a.scale_dtype = scale_dtype;
+  a.scale_f16 = scale_dtype == SD_F16;
+  a.scale_f32 = scale_dtype == SD_F32;
   a.groups = static_cast<int32_t>(K / group_size);
-  a.group = group_size;
+  const uint64_t parts = static_cast<uint64_t>(group_size) / 32;
+  a.inv32 = ((1ull << 32) + parts - 1) / parts;
   a.bias = static_cast<const uint16_t*>(bias);
   a.y = static_cast<uint16_t*>(y);
   a.ys = y_stride_m;
   a.M = M;
   a.N = N;
   a.K = static_cast<int32_t>(K);
+  const size_t need = sd_w4a16_workspace_size(M, N, K, group_size);
+  a.part = need && workspace && workspace_bytes >= need ? static_cast<float*>(workspace) : nullptr;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const bool bf = dtype == SD_BF16;
-  if (group_size % 128 == 0) return bf ? launch<__bf16, 4>(a, st) : launch<_Float16, 4>(a, st);
-  if (group_size % 64 == 0) return bf ? launch<__bf16, 2>(a, st) : launch<_Float16, 2>(a, st);
-  return bf ? launch<__bf16, 1>(a, st) : launch<_Float16, 1>(a, st);
+  if (dtype == SD_BF16) return launch<__bf16>(a, group_size, st);
+  return launch<_Float16>(a, group_size, st);
 }

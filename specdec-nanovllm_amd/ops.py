@@ -773,11 +773,15 @@ def w4a16_linear(x: torch.Tensor, qweight: torch.Tensor, scale: torch.Tensor,
         y = out.view(M, N)
         assert y.dtype == x.dtype and (N == 1 or y.stride(1) == 1)
     if M:
+        lib = _lib.load()
         with _lib.on_device(dev):
-            rc = _lib.load().sd_w4a16_linear(
+            # the plan (and so the workspace) depends on the device's compute units; none up to 16 rows
+            ws_bytes = lib.sd_w4a16_workspace_size(M, N, K, K // groups) if M > 16 else 0
+            ws = _workspace(ws_bytes, dev)
+            rc = lib.sd_w4a16_linear(
                 x2.data_ptr(), x2.stride(0), qw.data_ptr(), qw.stride(0), sc.data_ptr(),
                 _lib.dtype_code(sc.dtype), K // groups, _ptr(b), y.data_ptr(), y.stride(0), M, N, K,
-                _lib.dtype_code(x.dtype), _lib.stream_ptr(dev))
+                _lib.dtype_code(x.dtype), _ptr(ws), ws_bytes, _lib.stream_ptr(dev))
         _lib.check(rc)
     return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
 

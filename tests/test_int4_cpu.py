@@ -20,10 +20,10 @@ CALLS = {  # valid calls with one plausible thing left out (dtype 7), so that no
     "sd_load_kvcache_int4": [*CACHE, A[2], 16, 8, 128, 256, 64, 7, A[3], A[4], None],
     "sd_paged_attention_int4": [A[2], 4096, 128, *CACHE, 64, 256, A[3], 16, 16, A[4], None, None, 1, 16, 16, 32, 8,
                                 128, 0.1, BF16, A[5], 4096, 128, None, 0, 0, None],
-    "sd_w4a16_linear": [A[2], 1024, A[3], 512, A[4], BF16, 128, None, A[5], 4096, 4, 4096, 1024, 7, None],
+    "sd_w4a16_linear": [A[2], 1024, A[3], 512, A[4], BF16, 128, None, A[5], 4096, 4, 4096, 1024, 7, None, 0, None],
 }
 DTYPE_AT = {"sd_store_kvcache_int4": -2, "sd_qk_norm_rope_store_int4": -2, "sd_load_kvcache_int4": -4,
-            "sd_w4a16_linear": -2}
+            "sd_w4a16_linear": -4}
 no_gpu = pytest.mark.skipif(torch.cuda.device_count() > 0,
                             reason="fake device addresses: only where no GPU can be reached")
 
@@ -94,6 +94,13 @@ def test_workspace_queries():
     assert f(4, 1, 32, 8, 512, 0) == 0  # few keys a pair: one launch, no workspace
     assert f(4, 1, 32, 8, 4096, 5) == 2 * 4 * 8 * 5 * 4 * 132 * 4
     assert f(4, 9, 32, 8, 4096, 0) == f(1 << 30, 1, 32, 8, 4096, 0) == f(1, 1, 32, 8, 1 << 31, 0) == 2**64 - 1
+
+
+def test_w4a16_workspace():
+    f = _lib.load().sd_w4a16_workspace_size
+    assert f(16, 4096, 4096, 64) == f(0, 64, 64, 64) == f(640, 1 << 30, 64, 64) == f(1000, 19456, 2560, 128) == 0
+    # few tiles, a long K: a whole number of slices
+    assert f(65, 256, 8192, 128) % (65 * 256 * 4) == 0 and f(65, 256, 8192, 128) > 65 * 256 * 4
 
 
 def test_ops_refuse_wrong_tensors():

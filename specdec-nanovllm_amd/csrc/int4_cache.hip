@@ -58,7 +58,6 @@ struct AppendParams {
   int64_t tokens;
   int32_t hq, hkv;
   int32_t units;  // 16-lane items per token
-  int32_t rows;   // rows per item
 };
 
 struct LoadParams {
@@ -100,42 +99,77 @@ template <int LANES, typename F> __device__ __forceinline__ float over(float v, 
   return v;
 }
 
-// Scale and zero of a group from its minimum, maximum and sum of 0 * x (NaN if any is not finite)
-template <typename T>
-__device__ __forceinline__ uint32_t group_params(float lo, float hi, float bad, float& s, float& z) {
-  z = static_cast<float>(sd::round16<T>(lo));
-  s = static_cast<float>(sd::round16<T>(fmaxf(hi - z, 0.f) / 15.f));
-  if (!(bad + s * 0.f + z * 0.f == 0.f)) s = z = __builtin_nanf("");
-  return sd::pack2<T>(s, z);
+// Larger of two, NaN if either is (v_maximum3_f32).
+__device__ __forceinline__ float max_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
+// What turns a group's values into codes: (x - z) f * inv = (x - z) / s.
+struct Grid {
+  float s, z, f, inv;
+};
+// From the minimum and the maximum (NaN if any value is): the grid, and its scale and zero as stored.
+template <typename T> __device__ __forceinline__ Grid group_grid(float lo, float hi, uint32_t& sz) {
+  Grid g;
+  g.z = static_cast<float>(sd::round16<T>(lo));
+  // (a NaN maximum: fmaxf would drop it)
+  g.s = static_cast<float>(sd::round16<T>(max_nan(hi - g.z, 0.f) / 15.f));
+  if (!(g.s * 0.f + g.z * 0.f == 0.f)) g.s = g.z = __builtin_nanf("");
+  sz = sd::pack2<T>(g.s, g.z);
+  // the reciprocal of a bf16 scale below 2^-126 would overflow: both sides times 2^64
+  g.f = g.s < 0x1p-64f ? 0x1p64f : 1.f;
+  g.inv = g.s > 0.f ? 1.f / (g.s * g.f) : 0.f;
+  g.s *= g.f;
+  return g;
 }
 
-// IEEE division: a product with the reciprocal would move values that lie exactly between two
-// codes, which scales of 8 bits make common.
-__device__ __forceinline__ uint32_t code_of(float x, float s, float z) {
-  const float c = rintf((x - z) / s);
-  return s > 0.f ? static_cast<uint32_t>(fminf(fmaxf(c, 0.f), 15.f)) : 0u;
+// Code of a value. The quotient is the correctly rounded one (a product with the correctly rounded
+// reciprocal and one correction from the exact remainder: P. Markstein, 1990): values exactly between two
+// codes, which scales of 8 bits make common, stay exactly between them and go to the even one.
+__device__ __forceinline__ uint32_t code_of(float x, const Grid& g) {
+  const float t = (x - g.z) * g.f, q = t * g.inv;
+  const float c = rintf(fmaf(fmaf(-q, g.s, t), g.inv, q));
+  return static_cast<uint32_t>(__builtin_amdgcn_fmed3f(c, 0.f, 15.f));
 }
 
-template <typename T> __device__ __forceinline__ void load8(const uint16_t* p, float v[8]) {
-  const u32x4 a = sd::load16(p);
-  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+template <typename T> __device__ __forceinline__ void widen(u32x4 a, float v[8]) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = sd::from_bits<T>(static_cast<uint16_t>(w[e / 2] >> (16 * (e & 1))));
+  for (int e = 0; e < 8; ++e) v[e] = sd::from_bits<T>(static_cast<uint16_t>(a[e / 2] >> (16 * (e & 1))));
 }
 template <typename T> __device__ __forceinline__ void store8(uint16_t* p, const float v[8]) {
   sd::store16(p, u32x4{sd::pack2<T>(v[0], v[1]), sd::pack2<T>(v[2], v[3]),
                        sd::pack2<T>(v[4], v[5]), sd::pack2<T>(v[6], v[7])});
 }
 
-// Norm (w != NULL) and rotation of a row: lane c holds dims 8 c .. 8 c + 7; dim d's partner
-// d ^ 64 is the same element of lane c ^ 8.
+// Norm (weights w, if any) and rotation of a row: lane c holds dims 8 c .. 8 c + 7; dim d's partner d ^ 64
+// is the same element of lane c ^ 8, and sinv carries the sign of its term.
 template <typename T>
-__device__ __forceinline__ void norm_rotate(float x[8], const uint16_t* w, float eps, int c,
-                                            const float cosv[8], const float sinv[8], bool turn) {
+__device__ __forceinline__ void norm_rotate_query(u32x4 raw, float x[8], bool norm, const float w[8],
+                                                  float eps, const float cosv[8], const float sinv[8],
+                                                  bool turn) {
+  widen<T>(raw, x);
+  if (norm) {
+    float ss = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) ss = sd::dot2<T>(raw[e], raw[e], ss);
+    ss = over<16>(ss, [](float a, float b) { return a + b; });
+    const float r = rsqrtf(ss / 128.f + eps);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = x[e] * (r * w[e]);
+  }
+  if (turn) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = fmaf(dpp_move<kRor8>(x[e]), sinv[e], x[e] * cosv[e]);
+  }
+}
+// The same for a key, whose codes follow from values that may lie next to a border: the squares are
+// summed in 64 bits and every product is rounded by itself, so that the norm adds no more than its
+// formula's own roundings. (Queries in this form took append's 4001 tokens from XXX to 25 us.)
+template <typename T>
+__device__ __forceinline__ void norm_rotate_key(u32x4 raw, float x[8], bool norm, const float w[8],
+                                                float eps, const float cosv[8], const float sinv[8],
+                                                bool turn) {
 #pragma clang fp contract(off)
-  if (w) {
-    // The squares are summed in 64 bits (8 a lane, then 16 lanes: nothing beside the row's bytes), so
-    // that the norm adds no rounding of its own to a key that may lie next to a code's border.
+  widen<T>(raw, x);
+  if (norm) {
     double sq = 0.0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) sq += static_cast<double>(x[e]) * x[e];
@@ -144,16 +178,12 @@ __device__ __forceinline__ void norm_rotate(float x[8], const uint16_t* w, float
     sq += dpp_move64<kHalfMirror>(sq);
     sq += dpp_move64<kMirror>(sq);
     const float r = rsqrtf(static_cast<float>(sq) / 128.f + eps);
-    float wv[8];
-    load8<T>(w + 8 * c, wv);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = x[e] * r * wv[e];
+    for (int e = 0; e < 8; ++e) x[e] = x[e] * r * w[e];
   }
+  if (turn) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float other = dpp_move<kRor8>(x[e]);
-    const float y = c < 8 ? x[e] * cosv[e] - other * sinv[e] : x[e] * cosv[e] + other * sinv[e];
-    x[e] = turn ? y : x[e];
+    for (int e = 0; e < 8; ++e) x[e] = x[e] * cosv[e] + dpp_move<kRor8>(x[e]) * sinv[e];
   }
 }
 
@@ -161,21 +191,18 @@ __device__ __forceinline__ void norm_rotate(float x[8], const uint16_t* w, float
 template <typename T, int NG>
 __device__ __forceinline__ void write_key(const float x[8], uint8_t* codes, uint16_t* scales, int c) {
   constexpr int kLanes = 16 / NG;
-  float lo = x[0], hi = x[0], bad = 0.f;
+  float lo = x[0], hi = x[0];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
+  for (int e = 1; e < 8; ++e) {
     lo = fminf(lo, x[e]);
-    hi = fmaxf(hi, x[e]);
-    bad += x[e] * 0.f;
+    hi = max_nan(hi, x[e]);
   }
   lo = over<kLanes>(lo, [](float a, float b) { return fminf(a, b); });
-  hi = over<kLanes>(hi, [](float a, float b) { return fmaxf(a, b); });
-  bad = over<kLanes>(bad, [](float a, float b) { return a + b; });
-  float s, z;
-  const uint32_t sz = group_params<T>(lo, hi, bad, s, z);
-  uint32_t word = 0;
+  hi = over<kLanes>(hi, max_nan);
+  uint32_t sz, word = 0;
+  const Grid g = group_grid<T>(lo, hi, sz);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) word |= code_of(x[e], s, z) << (4 * (e / 2) + 16 * (e & 1));
+  for (int e = 0; e < 8; ++e) word |= code_of(x[e], g) << (4 * (e / 2) + 16 * (e & 1));
   reinterpret_cast<uint32_t*>(codes)[4 * (c & 3) + (c >> 2)] = word;
   if (c % kLanes == 0) reinterpret_cast<uint32_t*>(scales)[c / kLanes] = sz;
 }
@@ -190,40 +217,45 @@ __device__ __forceinline__ void write_value(const uint16_t* v, uint8_t* codes, u
   uint32_t word = 0, mine = 0;
 #pragma unroll
   for (int g = 0; g < NG; ++g) {
-    float lo = x[g * kPer], hi = lo, bad = 0.f;
+    float lo = x[g * kPer], hi = lo;
 #pragma unroll
-    for (int t = g * kPer; t < (g + 1) * kPer; ++t) {
+    for (int t = g * kPer + 1; t < (g + 1) * kPer; ++t) {
       lo = fminf(lo, x[t]);
-      hi = fmaxf(hi, x[t]);
-      bad += x[t] * 0.f;
+      hi = max_nan(hi, x[t]);
     }
     lo = over<16>(lo, [](float a, float b) { return fminf(a, b); });
-    hi = over<16>(hi, [](float a, float b) { return fmaxf(a, b); });
-    bad = over<16>(bad, [](float a, float b) { return a + b; });
-    float s, z;
-    const uint32_t sz = group_params<T>(lo, hi, bad, s, z);
+    hi = over<16>(hi, max_nan);
+    uint32_t sz;
+    const Grid grid = group_grid<T>(lo, hi, sz);
     mine = r == g ? sz : mine;
 #pragma unroll
-    for (int t = g * kPer; t < (g + 1) * kPer; ++t) word |= code_of(x[t], s, z) << (4 * t);
+    for (int t = g * kPer; t < (g + 1) * kPer; ++t) word |= code_of(x[t], grid) << (4 * t);
   }
   reinterpret_cast<uint32_t*>(codes + 64)[r] = word;
   if (r < NG) reinterpret_cast<uint32_t*>(scales)[NG + r] = mine;
 }
 
-// ROTATE: rows 0 .. hq - 1 of a token are its query heads (norm, rotation, copy out), the others
-// its kv heads; without, only kv heads. An item takes `rows` rows, every units-th one, and loads
-// its token's cos and sin once.
-template <typename T, int NG, bool ROTATE>
+// ROTATE: a token's query heads in items of QR (norm, rotation, copy out), then its kv heads, one an item;
+// without, only the kv heads. An item's rows are loaded before the first is used, its token's cos and
+// sin once.
+template <typename T, int NG, bool ROTATE, int QR>
 __global__ __launch_bounds__(kThreads) void append_kernel(AppendParams p) {
   const int c = threadIdx.x & 15;
   const int64_t item = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) >> 4;
   const int64_t t = item / p.units;
   if (t >= p.tokens) return;
   const int u = static_cast<int>(item - t * p.units);
-  const int hq = ROTATE ? p.hq : 0;
-  const int32_t slot = p.slots[t];
-  float cosv[8], sinv[8];
+  const int q_items = p.units - p.hkv;
+  float cosv[8], sinv[8], w[8];
   bool turn = false;
+  u32x4 raw[QR];
+  if (u < q_items) {
+#pragma unroll
+    for (int i = 0; i < QR; ++i)
+      raw[i] = sd::load16(p.q + t * p.q_stok + min(QR * u + i, p.hq - 1) * p.q_shead + 8 * c);
+  } else {
+    raw[0] = sd::load16(p.k + t * p.k_stok + (u - q_items) * p.k_shead + 8 * c);
+  }
   if constexpr (ROTATE) {
     const int64_t ps = p.pos[t];
     turn = ps >= 0 && ps < p.max_pos;
@@ -231,28 +263,34 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendParams p) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       cosv[e] = row[e];
-      sinv[e] = row[64 + e];
+      sinv[e] = c < 8 ? -row[64 + e] : row[64 + e];
     }
+    if (p.qw) widen<T>(sd::load16((u < q_items ? p.qw : p.kw) + 8 * c), w);
   }
-  for (int i = 0, r = u; i < p.rows && r < hq + p.hkv; ++i, r += p.units) {
-    float x[8];
-    if (r < hq) {
-      load8<T>(p.q + t * p.q_stok + r * p.q_shead + 8 * c, x);
-      norm_rotate<T>(x, p.qw, p.eps, c, cosv, sinv, turn);
-      store8<T>(p.qo + (t * p.hq + r) * kD + 8 * c, x);
-      continue;
-    }
-    const int h = r - hq;
-    load8<T>(p.k + t * p.k_stok + h * p.k_shead + 8 * c, x);
+  float x[8];
+  if (u < q_items) {
     if constexpr (ROTATE) {
-      norm_rotate<T>(x, p.kw, p.eps, c, cosv, sinv, turn);
-      if (p.ko) store8<T>(p.ko + (t * p.hkv + h) * kD + 8 * c, x);
+#pragma unroll
+      for (int i = 0; i < QR; ++i) {
+        const int r = QR * u + i;
+        if (r >= p.hq) break;
+        norm_rotate_query<T>(raw[i], x, p.qw, w, p.eps, cosv, sinv, turn);
+        store8<T>(p.qo + (t * p.hq + r) * kD + 8 * c, x);
+      }
     }
-    int64_t code, scale;
-    if (!slot_rows(p.c, slot, h, code, scale)) continue;
-    write_key<T, NG>(x, p.c.codes + code, p.c.scales + scale, c);
-    write_value<T, NG>(p.v + t * p.v_stok + h * p.v_shead, p.c.codes + code, p.c.scales + scale, c);
+    return;
   }
+  const int h = u - q_items;
+  const int32_t slot = p.slots[t];
+  if constexpr (!ROTATE) widen<T>(raw[0], x);
+  if constexpr (ROTATE) {
+    norm_rotate_key<T>(raw[0], x, p.kw, w, p.eps, cosv, sinv, turn);
+    if (p.ko) store8<T>(p.ko + (t * p.hkv + h) * kD + 8 * c, x);
+  }
+  int64_t code, scale;
+  if (!slot_rows(p.c, slot, h, code, scale)) return;
+  write_value<T, NG>(p.v + t * p.v_stok + h * p.v_shead, p.c.codes + code, p.c.scales + scale, c);
+  write_key<T, NG>(x, p.c.codes + code, p.c.scales + scale, c);
 }
 
 // Lane c of a row writes dims 8 c .. 8 c + 7 of its key and value.
@@ -334,22 +372,23 @@ int set_cache(const char* what, Cache& c, void* codes, int64_t c_sblk, int64_t c
   return SD_OK;
 }
 
-template <typename T, bool ROTATE> void launch_append(const AppendParams& p, int group, hipStream_t st) {
+template <typename T, bool ROTATE, int QR> void launch_append(AppendParams& p, int group, hipStream_t st) {
+  p.units = p.hkv + (ROTATE ? (p.hq + QR - 1) / QR : 0);
   const int64_t items = p.tokens * p.units;
   const dim3 grid(static_cast<unsigned>((items + kThreads / 16 - 1) / (kThreads / 16)));
   if (group == 32)
-    hipLaunchKernelGGL((append_kernel<T, 4, ROTATE>), grid, dim3(kThreads), 0, st, p);
+    hipLaunchKernelGGL((append_kernel<T, 4, ROTATE, QR>), grid, dim3(kThreads), 0, st, p);
   else if (group == 64)
-    hipLaunchKernelGGL((append_kernel<T, 2, ROTATE>), grid, dim3(kThreads), 0, st, p);
+    hipLaunchKernelGGL((append_kernel<T, 2, ROTATE, QR>), grid, dim3(kThreads), 0, st, p);
   else
-    hipLaunchKernelGGL((append_kernel<T, 1, ROTATE>), grid, dim3(kThreads), 0, st, p);
+    hipLaunchKernelGGL((append_kernel<T, 1, ROTATE, QR>), grid, dim3(kThreads), 0, st, p);
 }
 
-// Rows of a token per 16-lane item: one while few tokens leave the device idle, then four, so that
-// a token's cos and sin are loaded for four rows at a time.
-void plan_items(AppendParams& p, int rows) {
-  p.rows = p.tokens * rows > 16384 ? 4 : 1;
-  p.units = (rows + p.rows - 1) / p.rows;
+// Query heads per 16-lane item: one while few tokens leave the device idle, then four, so that a token's
+// cos and sin are loaded for four rows at a time.
+template <typename T> void launch_rotate(AppendParams& p, int group, hipStream_t st) {
+  if (p.tokens * (p.hq + p.hkv) > 16384) launch_append<T, true, 4>(p, group, st);
+  else launch_append<T, true, 1>(p, group, st);
 }
 
 template <typename T> void launch_load(const LoadParams& p, int group, hipStream_t st) {
@@ -418,11 +457,9 @@ extern "C" int sd_store_kvcache_int4(const void* key, int64_t key_stride_tok, in
   p.slots = slot_mapping;
   p.tokens = num_tokens;
   p.hkv = num_kv_heads;
-  p.rows = 1;
-  p.units = num_kv_heads;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (dtype == SD_BF16) launch_append<__bf16, false>(p, group_size, st);
-  else launch_append<_Float16, false>(p, group_size, st);
+  if (dtype == SD_BF16) launch_append<__bf16, false, 1>(p, group_size, st);
+  else launch_append<_Float16, false, 1>(p, group_size, st);
   return sd::check_launch(what);
 }
 
@@ -494,10 +531,9 @@ extern "C" int sd_qk_norm_rope_store_int4(
   p.tokens = num_tokens;
   p.hq = num_q_heads;
   p.hkv = num_kv_heads;
-  plan_items(p, num_q_heads + num_kv_heads);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (dtype == SD_BF16) launch_append<__bf16, true>(p, group_size, st);
-  else launch_append<_Float16, true>(p, group_size, st);
+  if (dtype == SD_BF16) launch_rotate<__bf16>(p, group_size, st);
+  else launch_rotate<_Float16>(p, group_size, st);
   return sd::check_launch(what);
 }
 

@@ -581,37 +581,54 @@ def int4_kvcache(num_blocks: int, block_size: int, num_kv_heads: int, group_size
     return codes.transpose(1, 2), scales.transpose(1, 2)
 
 
+# (The checks below are written for their cost: a small call is bound by the host, where a tensor's
+# ``reshape`` or ``to`` takes 1 us even if it changes nothing, a launch 4.)
 def _cache4(kv_codes: torch.Tensor, kv_scales: torch.Tensor, dtype: torch.dtype) -> tuple:
-    """The C ABI's arguments of a 4-bit cache (codes, strides, scales, strides, group size)."""
+    """(num_blocks, block_size, num_kv_heads) of a 4-bit cache and the C ABI's arguments of it
+    (codes, strides, scales, strides, group size)."""
     assert kv_codes.dim() == 4 and kv_codes.dtype == torch.uint8 and kv_codes.shape[3] == 128, \
         "kv_codes must be (num_blocks, block_size, num_kv_heads, 128) uint8"
-    assert kv_scales.dim() == 4 and kv_scales.shape[:3] == kv_codes.shape[:3] and \
-        kv_scales.shape[3] in (4, 8, 16), "kv_scales must be kv_codes' blocks, 512 / group_size each"
-    assert kv_scales.dtype == dtype, f"kv_scales must be {dtype}, as the activations"
-    cs, ss = kv_codes.stride(), kv_scales.stride()
-    assert cs[3] == 1 and ss[3] == 1
-    return (kv_codes.data_ptr(), cs[0], cs[1], cs[2], kv_scales.data_ptr(), ss[0], ss[1], ss[2],
-            512 // kv_scales.shape[3])
+    assert kv_scales.dim() == 4 and kv_scales.dtype == dtype, \
+        f"kv_scales must be 4-D and {dtype}, as the activations"
+    nb, bs, heads, _ = kv_codes.shape
+    nb2, bs2, heads2, n = kv_scales.shape
+    assert nb == nb2 and bs == bs2 and heads == heads2 and n in (4, 8, 16), \
+        "kv_scales must be kv_codes' blocks, 512 / group_size each"
+    c0, c1, c2, c3 = kv_codes.stride()
+    s0, s1, s2, s3 = kv_scales.stride()
+    assert c3 == 1 and s3 == 1
+    return nb, bs, heads, (kv_codes.data_ptr(), c0, c1, c2, kv_scales.data_ptr(), s0, s1, s2, 512 // n)
+
+
+def _flat(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """1-D contiguous ``t`` of ``dtype``."""
+    if t.dim() != 1:
+        t = t.reshape(-1)
+    if t.dtype != dtype:
+        t = t.to(dtype)
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def store_kvcache_int4(key: torch.Tensor, value: torch.Tensor, kv_codes: torch.Tensor,
                        kv_scales: torch.Tensor, slot_mapping: torch.Tensor) -> None:
     """``store_kvcache`` into a 4-bit cache (``int4_kvcache``): key / value (N, num_kv_heads,
     128) quantized to ``slot_mapping`` (slots of one call differ; -1 skips the row)."""
-    assert key.dim() == 3 and key.shape == value.shape and key.dtype == value.dtype
+    dt = key.dtype
+    assert key.dim() == 3 and key.shape == value.shape and dt == value.dtype
     N, Hkv, D = key.shape
-    cache = _cache4(kv_codes, kv_scales, key.dtype)
-    assert kv_codes.shape[2] == Hkv and slot_mapping.numel() == N
-    assert key.stride(2) == 1 and value.stride(2) == 1
-    slots = _i32(slot_mapping.reshape(-1))
+    nb, bs, heads, cache = _cache4(kv_codes, kv_scales, dt)
+    slots = _flat(slot_mapping, torch.int32)
+    assert heads == Hkv and slots.numel() == N
+    k0, k1, k2 = key.stride()
+    v0, v1, v2 = value.stride()
+    assert k2 == 1 and v2 == 1
     dev = _lib.require_device(key, value, kv_codes, kv_scales, slots)
     if N == 0:
         return
     with _lib.on_device(dev):
         rc = _lib.load().sd_store_kvcache_int4(
-            key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(), value.stride(0),
-            value.stride(1), *cache, slots.data_ptr(), N, Hkv, D, kv_codes.shape[1],
-            kv_codes.shape[0], _lib.dtype_code(key.dtype), _lib.stream_ptr(dev))
+            key.data_ptr(), k0, k1, value.data_ptr(), v0, v1, *cache, slots.data_ptr(), N, Hkv, D,
+            bs, nb, _lib.dtype_code(dt), _lib.stream_ptr(dev))
     _lib.check(rc)
 
 
@@ -628,39 +645,40 @@ def qk_norm_rope_store_int4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     left as they are; returns (q, k) as new contiguous tensors (k None with ``key_out=False``,
     for decode, where attention reads the cache). fp32 throughout, each output rounded once
     (``qk_norm_rope`` keeps the module's own roundings); the key is quantized unrounded."""
-    assert q.dim() == 3 and k.dim() == 3 and q.shape[0] == k.shape[0] and v.shape == k.shape
-    assert q.stride(2) == 1 and k.stride(2) == 1 and v.stride(2) == 1
-    assert q.dtype == k.dtype == v.dtype and q.shape[2] == k.shape[2]
-    assert (q_weight is None) == (k_weight is None)
+    dt = q.dtype
+    assert q.dim() == 3 and k.dim() == 3 and v.shape == k.shape and dt == k.dtype == v.dtype
     T, Hq, D = q.shape
-    Hkv = k.shape[1]
-    cache = _cache4(kv_codes, kv_scales, k.dtype)
-    assert kv_codes.shape[2] == Hkv
+    T2, Hkv, D2 = k.shape
+    assert T == T2 and D == D2
+    assert (q_weight is None) == (k_weight is None)
+    q0, q1, q2 = q.stride()
+    k0, k1, k2 = k.stride()
+    v0, v1, v2 = v.stride()
+    assert q2 == 1 and k2 == 1 and v2 == 1
+    nb, bs, heads, cache = _cache4(kv_codes, kv_scales, dt)
+    assert heads == Hkv
     cs = cos_sin_cache if cos_sin_cache.dim() == 2 else \
         cos_sin_cache.reshape(cos_sin_cache.shape[0], -1)
-    assert cs.dtype == torch.float32 and cs.shape[1] >= 128 and cs.stride(1) == 1
-    pos = positions.reshape(-1)
-    if pos.dtype != torch.int64:
-        pos = pos.to(torch.int64)
-    pos = pos.contiguous()
-    slots = _i32(slot_mapping.reshape(-1))
+    positions_max, width = cs.shape
+    cs0, cs1 = cs.stride()
+    assert cs.dtype == torch.float32 and width >= 128 and cs1 == 1
+    pos, slots = _flat(positions, torch.int64), _flat(slot_mapping, torch.int32)
     assert pos.numel() == T and slots.numel() == T
     qw = kw = None
     if q_weight is not None:
-        assert q_weight.shape == (D,) and k_weight.shape == (D,)
-        qw, kw = q_weight.to(q.dtype).contiguous(), k_weight.to(q.dtype).contiguous()
+        qw, kw = _flat(q_weight, dt), _flat(k_weight, dt)
+        assert qw.numel() == D and kw.numel() == D
     dev = _lib.require_device(q, k, v, pos, cs, kv_codes, kv_scales, slots, qw, kw)
-    q_out = torch.empty((T, Hq, D), dtype=q.dtype, device=dev)
-    k_out = torch.empty((T, Hkv, D), dtype=q.dtype, device=dev) if key_out else None
+    q_out = torch.empty((T, Hq, D), dtype=dt, device=dev)
+    k_out = torch.empty((T, Hkv, D), dtype=dt, device=dev) if key_out else None
     if T == 0:
         return q_out, k_out
     with _lib.on_device(dev):
         rc = _lib.load().sd_qk_norm_rope_store_int4(
-            q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
-            v.data_ptr(), v.stride(0), v.stride(1), T, Hq, Hkv, D, _ptr(qw), _ptr(kw), float(eps),
-            pos.data_ptr(), cs.data_ptr(), cs.stride(0), cs.shape[0], q_out.data_ptr(), _ptr(k_out),
-            *cache, kv_codes.shape[0], kv_codes.shape[1], slots.data_ptr(),
-            _lib.dtype_code(q.dtype), _lib.stream_ptr(dev))
+            q.data_ptr(), q0, q1, k.data_ptr(), k0, k1, v.data_ptr(), v0, v1, T, Hq, Hkv, D,
+            _ptr(qw), _ptr(kw), eps, pos.data_ptr(), cs.data_ptr(), cs0, positions_max,
+            q_out.data_ptr(), _ptr(k_out), *cache, nb, bs, slots.data_ptr(), _lib.dtype_code(dt),
+            _lib.stream_ptr(dev))
     _lib.check(rc)
     return q_out, k_out
 
@@ -670,18 +688,19 @@ def load_kvcache_int4(kv_codes: torch.Tensor, kv_scales: torch.Tensor,
     """The rows of a 4-bit cache at ``slot_mapping`` (N,) in the activations' type: (key, value),
     each (N, num_kv_heads, 128); rows of slot -1 are zero. Prefill over a cached prefix reads its
     pages this way."""
-    cache = _cache4(kv_codes, kv_scales, kv_scales.dtype)
-    slots = _i32(slot_mapping.reshape(-1))
+    dt = kv_scales.dtype
+    nb, bs, Hkv, cache = _cache4(kv_codes, kv_scales, dt)
+    slots = _flat(slot_mapping, torch.int32)
     dev = _lib.require_device(kv_codes, kv_scales, slots)
-    N, Hkv = slots.numel(), kv_codes.shape[2]
-    k = torch.empty((N, Hkv, 128), dtype=kv_scales.dtype, device=dev)
-    v = torch.empty((N, Hkv, 128), dtype=kv_scales.dtype, device=dev)
+    N = slots.numel()
+    k = torch.empty((N, Hkv, 128), dtype=dt, device=dev)
+    v = torch.empty((N, Hkv, 128), dtype=dt, device=dev)
     if N == 0:
         return k, v
     with _lib.on_device(dev):
         rc = _lib.load().sd_load_kvcache_int4(
-            *cache, slots.data_ptr(), N, Hkv, 128, kv_codes.shape[1], kv_codes.shape[0],
-            _lib.dtype_code(kv_scales.dtype), k.data_ptr(), v.data_ptr(), _lib.stream_ptr(dev))
+            *cache, slots.data_ptr(), N, Hkv, 128, bs, nb, _lib.dtype_code(dt), k.data_ptr(),
+            v.data_ptr(), _lib.stream_ptr(dev))
     _lib.check(rc)
     return k, v
 
@@ -698,10 +717,8 @@ def paged_attention_int4(q: torch.Tensor, kv_codes: torch.Tensor, kv_scales: tor
     if q.dim() != 3:
         raise ValueError(f"q must be (tokens, heads, head_dim), got {tuple(q.shape)}")
     total_q, Hq, D = q.shape
-    cache = _cache4(kv_codes, kv_scales, q.dtype)
-    num_blocks, block_size, Hkv = kv_codes.shape[:3]
+    num_blocks, block_size, Hkv, cache = _cache4(kv_codes, kv_scales, q.dtype)
     assert Hq % Hkv == 0, f"GQA needs num_q_heads divisible by num_kv_heads: {Hq} vs {Hkv}"
-    assert q.stride(2) == 1
     assert block_table.dim() == 2, "block_table must be (num_seqs, max_blocks)"
     if (context_lens is None) == (cu_seqlens_k is None):
         raise ValueError("give exactly one of context_lens / cu_seqlens_k")
@@ -720,11 +737,12 @@ def paged_attention_int4(q: torch.Tensor, kv_codes: torch.Tensor, kv_scales: tor
     if out is None:
         out = torch.empty_like(q)
     else:
-        assert out.shape == q.shape and out.dtype == q.dtype and out.stride(2) == 1
+        assert out.shape == q.shape and out.dtype == q.dtype
     if total_q == 0 or num_seqs == 0:
         return out
     lib = _lib.load()
     qs, os = q.stride(), out.stride()
+    assert qs[2] == 1 and os[2] == 1
     max_seqlen_q = int(max_seqlen_q)
     with _lib.on_device(dev):
         # the plan (and so the workspace) depends on the device's compute units
@@ -758,14 +776,15 @@ def w4a16_linear(x: torch.Tensor, qweight: torch.Tensor, scale: torch.Tensor,
     assert x2.shape[1] == K, f"K mismatch: x {tuple(x2.shape)} vs w {tuple(qweight.shape)}"
     groups = scale.shape[1]
     assert scale.shape[0] == N and groups and K % groups == 0, "scale must be (N, K // group)"
-    if x2.stride(1) != 1 or x2.data_ptr() % 16 or (M > 1 and x2.stride(0) % 8):
-        x2 = x2.contiguous()
+    x0, x1 = x2.stride()
+    if x1 != 1 or x2.data_ptr() % 16 or (M > 1 and x0 % 8):
+        x2, x0 = x2.contiguous(), K
     qw = qweight if qweight.is_contiguous() else qweight.contiguous()
     sc = scale if scale.is_contiguous() else scale.contiguous()
     b = None
     if bias is not None:
         assert bias.shape == (N,), "bias must be (N,)"
-        b = bias.to(x.dtype).contiguous()
+        b = _flat(bias, x.dtype)
     dev = _lib.require_device(x2, qw, sc, b, out)
     if out is None:
         y = torch.empty((M, N), device=dev, dtype=x.dtype)
@@ -779,9 +798,8 @@ def w4a16_linear(x: torch.Tensor, qweight: torch.Tensor, scale: torch.Tensor,
             ws_bytes = lib.sd_w4a16_workspace_size(M, N, K, K // groups) if M > 16 else 0
             ws = _workspace(ws_bytes, dev)
             rc = lib.sd_w4a16_linear(
-                x2.data_ptr(), x2.stride(0), qw.data_ptr(), qw.stride(0), sc.data_ptr(),
-                _lib.dtype_code(sc.dtype), K // groups, _ptr(b), y.data_ptr(), y.stride(0), M, N, K,
-                _lib.dtype_code(x.dtype), _ptr(ws), ws_bytes, _lib.stream_ptr(dev))
+                x2.data_ptr(), x0, qw.data_ptr(), K // 2, sc.data_ptr(), _lib.dtype_code(sc.dtype),
+                K // groups, _ptr(b), y.data_ptr(), y.stride(0), M, N, K, _lib.dtype_code(x.dtype), _ptr(ws), ws_bytes, _lib.stream_ptr(dev))
         _lib.check(rc)
     return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
 

@@ -41,11 +41,12 @@ using sd::f32x4;
 using sd::u32x4;
 
 constexpr int kD = 128;
-constexpr int kWaves = 4;
 constexpr int kStep = 32;               // keys of a wave's step
 constexpr int kPitch = kD + 4;          // floats of a row's state: acc, then m and l
 constexpr int kMergeRows = 8;           // rows of a tile the waves merge at a time
-constexpr int kWholeKeys = 512;         // tables of up to this many keys: no splitting of pairs
+// Tables of up to this many keys: no splitting of pairs, and past kShortKeys twice the waves. One launch
+// of 8 steps' length at most against two (16 heads, 1 x 1000 keys: XXX against 10.0 us in a graph).
+constexpr int kShortKeys = 512, kWholeKeys = 1024;
 
 struct Params {
   const uint16_t* q;
@@ -177,7 +178,7 @@ template <int NG> constexpr int ahead() { return NG == 4 ? 2 : 3; }
 template <int NG> constexpr int slot_bytes() { return kStep * (kD + 8 * NG); }
 template <int NG> constexpr int wave_bytes() { return ahead<NG>() * slot_bytes<NG>() + kStep * 16 * NG; }
 
-template <typename T, int NG, int TS, bool R4, Pages PAGES>
+template <typename T, int NG, int TS, bool R4, Pages PAGES, int kWaves>
 __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2)))
 void int4_attn_main(Params p) {
   static_assert(!R4 || TS == 1, "four rows fit one tile");
@@ -586,10 +587,9 @@ void int4_attn_main(Params p) {
         }
       }
       __syncthreads();
-      const int r = tid >> 5, c = tid & 31;
-      static_assert(kMergeRows * 32 == kWaves * 64, "a thread takes 4 dims of a row of each tile");
-#pragma unroll
-      for (int t = 0; t < TS; ++t) {
+      // a thread takes 4 dims of a row of each tile (8 waves: of one tile; there may be only one)
+      const int r = (tid >> 5) % kMergeRows, c = tid & 31;
+      for (int t = kWaves == 4 ? 0 : tid / (kMergeRows * 32); t < TS; t += kWaves == 4 ? 1 : 2) {
         const int row = 16 * t + kMergeRows * r8 + r;
         if (row >= rows) continue;
         float M = -INFINITY, sum = 0.f;
@@ -729,8 +729,8 @@ template <typename T> __global__ __launch_bounds__(256) void int4_attn_combine(P
   }
 }
 
-// Keys of a chunk: fewer where two waves share them
-int64_t chunk_keys(int64_t rows) { return kStep * kWaves / (rows <= 16 ? 1 : 2); }
+// Keys of a chunk of 4 or 8 waves: fewer where two waves share them
+int64_t chunk_keys(int64_t rows, int waves) { return kStep * waves / (rows <= 16 ? 1 : 2); }
 
 struct Plan {
   int64_t runs;
@@ -747,7 +747,7 @@ Plan make_plan(int num_seqs, int max_qlen, int hq, int hkv, int64_t max_ctx, int
     pl.runs = pairs;
   } else {
     // one resident set of workgroups of 4 waves, two a compute unit
-    const int64_t chunk = chunk_keys(pl.rmax), most = pairs * ((max_ctx + chunk - 1) / chunk);
+    const int64_t chunk = chunk_keys(pl.rmax, 4), most = pairs * ((max_ctx + chunk - 1) / chunk);
     pl.runs = num_splits > 0 ? pairs * num_splits : 2ll * sd::device_cus();
     if (pl.runs > most) pl.runs = most;
   }
@@ -755,7 +755,7 @@ Plan make_plan(int num_seqs, int max_qlen, int hq, int hkv, int64_t max_ctx, int
 }
 
 bool plan_fits(int num_seqs, int hkv, int64_t max_ctx, int num_splits) {
-  const int64_t pairs = static_cast<int64_t>(num_seqs) * hkv, chunk = kStep * kWaves / 2;
+  const int64_t pairs = static_cast<int64_t>(num_seqs) * hkv, chunk = kStep * 2;
   return max_ctx <= (1ll << 30) && pairs <= (1ll << 23) && num_splits <= (1 << 16) &&
          pairs * ((max_ctx + chunk - 1) / chunk) <= (1ll << 30) &&
          (num_splits == 0 || pairs * num_splits <= (1ll << 22));
@@ -765,14 +765,17 @@ size_t ws_bytes(const Plan& pl) {
   return pl.whole ? 0 : static_cast<size_t>(2 * pl.runs) * pl.rmax * kPitch * sizeof(float);
 }
 
-template <typename T, int NG, int TS, bool R4> void launch_main(const Params& p, hipStream_t st) {
-  const dim3 grid(p.runs), block(kWaves * 64);
-  if (p.block_size % kStep == 0)
-    hipLaunchKernelGGL((int4_attn_main<T, NG, TS, R4, kOnePage>), grid, block, 0, st, p);
-  else if (p.block_size % (kStep / 2) == 0)
-    hipLaunchKernelGGL((int4_attn_main<T, NG, TS, R4, kHalfPages>), grid, block, 0, st, p);
+template <typename T, int NG, int TS, bool R4, Pages PAGES> void launch_waves(const Params& p, hipStream_t st) {
+  if (p.whole && p.max_ctx > kShortKeys)
+    hipLaunchKernelGGL((int4_attn_main<T, NG, TS, R4, PAGES, 8>), dim3(p.runs), dim3(512), 0, st, p);
   else
-    hipLaunchKernelGGL((int4_attn_main<T, NG, TS, R4, kAnyPages>), grid, block, 0, st, p);
+    hipLaunchKernelGGL((int4_attn_main<T, NG, TS, R4, PAGES, 4>), dim3(p.runs), dim3(256), 0, st, p);
+}
+
+template <typename T, int NG, int TS, bool R4> void launch_main(const Params& p, hipStream_t st) {
+  if (p.block_size % kStep == 0) launch_waves<T, NG, TS, R4, kOnePage>(p, st);
+  else if (p.block_size % (kStep / 2) == 0) launch_waves<T, NG, TS, R4, kHalfPages>(p, st);
+  else launch_waves<T, NG, TS, R4, kAnyPages>(p, st);
 }
 
 template <typename T, int NG> void launch_rows(const Params& p, hipStream_t st) {
@@ -929,7 +932,7 @@ extern "C" int sd_paged_attention_int4(
   p.runs = static_cast<int32_t>(pl.runs);
   p.whole = pl.whole;
   p.rmax = pl.rmax;
-  p.chunk_shift = __builtin_ctzll(chunk_keys(pl.rmax));
+  p.chunk_shift = __builtin_ctzll(chunk_keys(pl.rmax, pl.whole && max_ctx > kShortKeys ? 8 : 4));
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == SD_BF16) return launch<__bf16>(p, pl, group_size, st);
   return launch<_Float16>(p, pl, group_size, st);

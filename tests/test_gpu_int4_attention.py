@@ -95,8 +95,9 @@ ODD = [1, 0, 31, 32, 33, 127, 128, 129, 300, 1000]
 @pytest.mark.parametrize("kind", ["bf16", "fp16"])
 @pytest.mark.parametrize("group", [32, 64, 128])
 @pytest.mark.parametrize("page,interleaved", [(16, False), (48, True), (64, True), (256, False)])
-def test_decode(kind, group, page, interleaved):
-    c = make(ODD, page, 16, 4, group, kind, interleaved=interleaved)
+@pytest.mark.parametrize("keys", [1024, 4000])  # a workgroup a pair, and split
+def test_decode(kind, group, page, interleaved, keys):
+    c = make(ODD, page, 16, 4, group, kind, interleaved=interleaved, width=keys // page)
     out = ops.paged_attention_int4(c["q"], c["codes"], c["scales"], c["table"], SCALE,
                                    context_lens=torch.tensor(ODD, dtype=torch.int32, device=DEV))
     check(c, out, kind)
@@ -112,7 +113,7 @@ def test_head_layouts(hq, hkv):
 
 
 @pytest.mark.parametrize("group", [32, 128])
-@pytest.mark.parametrize("width", [1, 2, 8, 300])
+@pytest.mark.parametrize("width", [1, 2, 3, 4, 8, 300])
 def test_short_and_wide_tables(width, group):
     # few keys a table: one workgroup a pair; a wide table with short sequences: split
     lens = [min(256 * width, n) for n in (200, 0, 256, 511, 77)]
@@ -124,9 +125,11 @@ def test_short_and_wide_tables(width, group):
 
 @pytest.mark.parametrize("kind", ["bf16", "fp16"])
 @pytest.mark.parametrize("group", [32, 64, 128])
-def test_verify_rows(kind, group):
+@pytest.mark.parametrize("keys", [960, 3000])
+@pytest.mark.parametrize("page", [64, 16, 40])
+def test_verify_rows(kind, group, keys, page):
     lens, nq = [900, 3, 40, 0, 129, 8], [7, 7, 1, 2, 0, 8]  # rows 0 .. 3 of the second see no key
-    c = make(lens, 64, 16, 4, group, kind, nq=nq, seed=3)
+    c = make(lens, page, 16, 4, group, kind, nq=nq, seed=3, width=keys // page)
     out = ops.paged_attention_int4(c["q"], c["codes"], c["scales"], c["table"], SCALE,
                                    context_lens=torch.tensor(lens, dtype=torch.int32, device=DEV),
                                    cu_seqlens_q=cu(nq), max_seqlen_q=8)

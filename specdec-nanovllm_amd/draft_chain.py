@@ -31,6 +31,11 @@ launch on the qkv output (the attention reads q through strides), SiLU*mul in
 the gate_up projection's epilogue (one or two rows; the SiLU launch beyond),
 the sampler's argmax; the embedding lookup stays a torch index.
 
+``weight_bits=4`` holds every linear in 4 bits (groups of 128 columns), ``kv_bits=4``
+the KV cache in 4 bits (groups of 64 dims); either takes the step of
+``_step_4bit``: the library's RMSNorm, linear, append (q/k norm + RoPE + quantize +
+slot write in one launch), attention and SiLU*mul, one launch each.
+
 ``chain()`` runs ``k`` steps back to back, each feeding its tokens to the next,
 on static buffers, so the whole chain can be captured in one HIP graph.
 """
@@ -41,7 +46,7 @@ import math
 import torch
 
 from . import ops
-from .layers.quant import quantize_weight
+from .layers.quant import quantize_weight, quantize_weight_int4
 
 QWEN3_06B = dict(layers=28, hidden=1024, heads=16, kv_heads=8, head_dim=128, inter=3072,
                  vocab=151936, theta=1e6, eps=1e-6)
@@ -55,7 +60,11 @@ class DraftChain:
                  inter: int = 3072, vocab: int = 151936, theta: float = 1e6, eps: float = 1e-6,
                  block_size: int = 256, seed: int = 0, device="cuda",
                  dtype: torch.dtype = torch.bfloat16, fused: bool = False,
-                 context: str = "prefill"):
+                 context: str = "prefill", weight_bits: int = 8, kv_bits: int = 16):
+        if weight_bits not in (4, 8) or kv_bits not in (4, 16):
+            raise ValueError(f"weights in 4 or 8 bits, cache in 4 or 16: got {weight_bits}, {kv_bits}")
+        self.weight_bits, self.kv_bits = weight_bits, kv_bits
+        self._linear = ops.w4a16_linear if weight_bits == 4 else ops.w8a16_linear
         self.B, self.ctx_len, self.k = batch, ctx_len, k
         self.fused = fused
         self.L, self.H, self.Hq, self.Hkv, self.D = layers, hidden, heads, kv_heads, head_dim
@@ -69,8 +78,8 @@ class DraftChain:
             return (torch.randn(shape, generator=g, device=self.dev) * std).to(dtype)
 
         def qlinear(n_out, n_in):
-            q, s = quantize_weight(randn(n_out, n_in))
-            return q, s
+            w = randn(n_out, n_in)
+            return quantize_weight_int4(w, 128) if weight_bits == 4 else quantize_weight(w)
 
         self.embed = randn(vocab, hidden)
         self.layers = []
@@ -96,14 +105,23 @@ class DraftChain:
         # context of ctx_len rows per sequence; pages are a seeded shuffle
         self.pages_per_seq = math.ceil((ctx_len + k) / block_size)
         nblk = batch * self.pages_per_seq
-        if context == "randn":
+        if context not in ("randn", "prefill"):
+            raise ValueError(f"unknown context: {context}")
+        if kv_bits == 4:
+            self.kv4 = [ops.int4_kvcache(nblk, block_size, kv_heads, 64, dtype, self.dev)
+                        for _ in range(layers)]
+            if context == "randn":
+                every = torch.arange(nblk * block_size, dtype=torch.int32, device=self.dev)
+                for cache in self.kv4:
+                    rows = torch.randn((2, nblk * block_size, kv_heads, head_dim), generator=g,
+                                       device=self.dev).to(dtype)
+                    ops.store_kvcache_int4(rows[0], rows[1], *cache, every)
+        elif context == "randn":
             self.kv = torch.randn((2, layers, nblk, block_size, kv_heads, head_dim),
                                   generator=g, device=self.dev).to(dtype)
-        elif context == "prefill":
+        else:
             self.kv = torch.zeros((2, layers, nblk, block_size, kv_heads, head_dim),
                                   device=self.dev, dtype=dtype)
-        else:
-            raise ValueError(f"unknown context: {context}")
         cg = torch.Generator().manual_seed(seed + 1)
         perm = torch.randperm(nblk, generator=cg).to(torch.int32)
         self.block_table = perm.view(batch, self.pages_per_seq).to(self.dev)
@@ -139,10 +157,12 @@ class DraftChain:
         B, C, Hq, Hkv, D = self.B, self.ctx_len, self.Hq, self.Hkv, self.D
         if C == 0:
             return
-        from .layers.quant import dequantize_weight
+        from .layers.quant import dequantize_weight, dequantize_weight_int4
+
+        dequantize = dequantize_weight_int4 if self.weight_bits == 4 else dequantize_weight
 
         def lin(x, qw):
-            return x @ dequantize_weight(*qw).to(self.dtype).T.contiguous()
+            return x @ dequantize(*qw).to(self.dtype).T.contiguous()
 
         pos = torch.arange(C, device=self.dev).repeat(B)
         cos, sin = self.cos[pos], self.sin[pos]
@@ -162,8 +182,11 @@ class DraftChain:
             q = self._rope(self._rms(q.reshape(-1, Hq, D), lw["q_norm"]), cos, sin)
             kk = self._rope(self._rms(kk.reshape(-1, Hkv, D), lw["k_norm"]), cos, sin)
             v = v.reshape(-1, Hkv, D).contiguous()
-            self.kv[0, li].view(-1, Hkv, D)[slots] = kk
-            self.kv[1, li].view(-1, Hkv, D)[slots] = v
+            if self.kv_bits == 4:
+                ops.store_kvcache_int4(kk.contiguous(), v, *self.kv4[li], slots)
+            else:
+                self.kv[0, li].view(-1, Hkv, D)[slots] = kk
+                self.kv[1, li].view(-1, Hkv, D)[slots] = v
             o = ops.prefill_attention(q.contiguous(), kk.contiguous(), v, cu, cu, C, self.scale)
             h = lin(o.reshape(-1, Hq * D), lw["o"])
             x, residual = self._add_rms(h, residual, lw["post_norm"])
@@ -191,6 +214,8 @@ class DraftChain:
     # ----------------------------------------------------------------------- step
     def step(self, s: int) -> torch.Tensor:
         """Draft step s: reads tokens[s], writes tokens[s + 1], returns the logits."""
+        if self.weight_bits == 4 or self.kv_bits == 4:
+            return self._step_4bit(s)
         if self.fused:
             return self._step_fused(s)
         B, Hq, Hkv, D = self.B, self.Hq, self.Hkv, self.D
@@ -264,6 +289,36 @@ class DraftChain:
         ops.sample(logits, out=self.tokens[s + 1])
         return logits
 
+    def _step_4bit(self, s: int) -> torch.Tensor:
+        B, Hq, Hkv, D, eps, lin = self.B, self.Hq, self.Hkv, self.D, self.eps, self._linear
+        pos, slots, ctx = self.positions[s], self.slots[s], self.ctx[s]
+        h, residual = self.embed[self.tokens[s]], None
+        for li, lw in enumerate(self.layers):
+            if residual is None:
+                residual, x = h, ops.rmsnorm(h, lw["in_norm"], eps)
+            else:
+                x, residual = ops.rmsnorm(h, lw["in_norm"], eps, residual)
+            qkv = lin(x, *lw["qkv"])
+            q = qkv[:, :Hq * D].view(B, Hq, D)
+            kk = qkv[:, Hq * D:(Hq + Hkv) * D].view(B, Hkv, D)
+            v = qkv[:, (Hq + Hkv) * D:].view(B, Hkv, D)
+            if self.kv_bits == 4:
+                q, _ = ops.qk_norm_rope_store_int4(q, kk, v, pos, self.cos_sin, *self.kv4[li], slots,
+                                                   lw["q_norm"], lw["k_norm"], eps, key_out=False)
+                o = ops.paged_attention_int4(q, *self.kv4[li], self.block_table, self.scale,
+                                             context_lens=ctx)
+            else:
+                ops.qk_norm_rope(q, kk, pos, self.cos_sin, lw["q_norm"], lw["k_norm"], eps, v=v,
+                                 k_cache=self.kv[0, li], v_cache=self.kv[1, li], slot_mapping=slots)
+                o = ops.paged_attention(q, self.kv[0, li], self.kv[1, li], self.block_table,
+                                        self.scale, context_lens=ctx)
+            x, residual = ops.rmsnorm(lin(o.reshape(B, Hq * D), *lw["o"]), lw["post_norm"], eps, residual)
+            h = lin(ops.silu_mul(lin(x, *lw["gate_up"])), *lw["down"])
+        x, _ = ops.rmsnorm(h, self.final_norm, eps, residual)
+        logits = lin(x, *self.lm_head)
+        ops.sample(logits, out=self.tokens[s + 1])
+        return logits
+
     def chain(self) -> None:
         for s in range(self.k):
             self.step(s)
@@ -282,13 +337,18 @@ class DraftChain:
         q, kk, v = self._qkv_static
         for s in range(self.k):
             for li in range(self.L):
+                if self.kv_bits == 4:
+                    ops.store_kvcache_int4(kk, v, *self.kv4[li], self.slots[s])
+                    ops.paged_attention_int4(q, *self.kv4[li], self.block_table, self.scale,
+                                             context_lens=self.ctx[s])
+                    continue
                 kc, vc = self.kv[0, li], self.kv[1, li]
                 ops.paged_attention(q, kc, vc, self.block_table, self.scale,
                                     context_lens=self.ctx[s], key=kk, value=v,
                                     slot_mapping=self.slots[s])
 
     def gemv_chain(self) -> None:
-        """Only the W8A16 linears of every step (4 per layer + lm_head), on static
+        """Only the quantized linears of every step (4 per layer + lm_head), on static
         activations of the step's shape."""
         if not hasattr(self, "_act_static"):
             g = torch.Generator(device=self.dev)
@@ -300,15 +360,15 @@ class DraftChain:
         xh, xo, xi = self._act_static
         for _ in range(self.k):
             for lw in self.layers:
-                ops.w8a16_linear(xh, *lw["qkv"])
-                ops.w8a16_linear(xo, *lw["o"])
-                ops.w8a16_linear(xh, *lw["gate_up"])
-                ops.w8a16_linear(xi, *lw["down"])
-            ops.w8a16_linear(xh, *self.lm_head)
+                self._linear(xh, *lw["qkv"])
+                self._linear(xo, *lw["o"])
+                self._linear(xh, *lw["gate_up"])
+                self._linear(xi, *lw["down"])
+            self._linear(xh, *self.lm_head)
 
     # ----------------------------------------------------------------- accounting
     def step_bytes(self) -> int:
-        """Algorithmic HBM bytes of one draft step: every int8 weight and scale
+        """Algorithmic HBM bytes of one draft step: every quantized weight and scale
         once, the visible K/V rows of every layer, the embedding rows read."""
         w = 0
         for lw in self.layers:
@@ -317,5 +377,6 @@ class DraftChain:
                 w += q.numel() + sc.numel() * sc.element_size()
         q, sc = self.lm_head
         w += q.numel() + sc.numel() * sc.element_size()
-        kv = self.L * self.B * (self.ctx_len + 1) * self.Hkv * self.D * 2 * 2
+        row = self.D * 2 * 2 if self.kv_bits == 16 else self.D + 8 * 2  # 4 bits: codes, 2 + 2 groups
+        kv = self.L * self.B * (self.ctx_len + 1) * self.Hkv * row
         return w + kv + self.B * self.H * 2

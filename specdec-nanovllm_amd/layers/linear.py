@@ -2,8 +2,8 @@
 
 ``LinearBase._apply(x, bias)`` is the one call site of the W8A16 path in the
 reference (linear.py:40-45): an int8 ``weight`` goes to ``int8_linear`` with
-the module's ``weight_scale``/``quant_granularity``/``quant_group_size``,
-anything else to ``F.linear``. Tensor-parallel sharding and its all-reduce are
+the module's ``weight_scale``/``quant_granularity``/``quant_group_size``, a
+packed 4-bit ``weight`` (uint8) to ``int4_linear``, anything else to ``F.linear``. Tensor-parallel sharding and its all-reduce are
 not part of this single-GPU library (tp_size is 1).
 
 ``nn.Module`` already uses the name ``_apply(fn)`` for ``.to()``/``.cuda()``;
@@ -17,7 +17,7 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
-from .quant import int8_linear
+from .quant import int4_linear, int8_linear
 
 
 class LinearBase(nn.Module):
@@ -42,6 +42,8 @@ class LinearBase(nn.Module):
         if self.weight.dtype == torch.int8:
             return int8_linear(x, self.weight, self.weight_scale, bias,
                                self.quant_granularity, self.quant_group_size)
+        if self.weight.dtype == torch.uint8:
+            return int4_linear(x, self.weight, self.weight_scale, bias)
         return F.linear(x, self.weight, bias)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:

@@ -13,6 +13,9 @@
   (quant.py:31-63).
 * ``apply_int8_quant`` — in-place swap of named linear layers to int8
   (quant.py:66-117).
+* ``quantize_weight_int4`` / ``dequantize_weight_int4`` / ``int4_linear`` /
+  ``apply_int4_quant`` — the same with 4-bit weights and group scales (W4A16; the
+  reference has no 4-bit weights).
 """
 from __future__ import annotations
 
@@ -24,6 +27,7 @@ import torch.nn as nn
 from .. import ops
 
 QMAX = 127
+QMAX4 = 7
 
 
 def quantize_weight(w: torch.Tensor, granularity: str = "per_channel", group_size: int = 128):
@@ -108,6 +112,42 @@ def int8_linear(x: torch.Tensor, qweight: torch.Tensor, scale: torch.Tensor,
     return ops.w8a16_linear(x, qweight, scale, bias, gs)
 
 
+def quantize_weight_int4(w: torch.Tensor, group_size: int = 128):
+    """Symmetric 4-bit quantization of a 2-D weight ``[N, K]`` in groups of ``group_size`` columns (a
+    multiple of 32 that divides K), on the weight's device.
+
+    scale = max(|w| over the group) / 7, floored at 1e-8, and q = clamp(round_half_even(w / scale), -7, 7),
+    in fp32. Returns ``(uint8 [N, K // 2], scale bf16 [N, K // group_size])``: byte j holds q + 8 of columns
+    2j (low half) and 2j + 1, and the scale is rounded to bf16 after q, as ``quantize_weight``'s.
+    """
+    assert w.dim() == 2, f"expects a 2-D weight, got {tuple(w.shape)}"
+    N, K = w.shape
+    assert group_size > 0 and group_size % 32 == 0 and K % group_size == 0, \
+        f"groups must be a multiple of 32 columns and divide K, got {group_size} of {K}"
+    packed = torch.empty((N, K // 2), dtype=torch.uint8, device=w.device)
+    scales = torch.empty((N, K // group_size), dtype=torch.bfloat16, device=w.device)
+    rows = max(1, (1 << 26) // K)  # a slice of the weight at a time in fp32
+    for n in range(0, N, rows):
+        f = w[n:n + rows].float().view(-1, K // group_size, group_size)
+        scale = (f.abs().amax(-1, keepdim=True) / QMAX4).clamp_min(1e-8)
+        q = ((f / scale).round().clamp(-QMAX4, QMAX4) + 8).to(torch.uint8).view(-1, K)
+        packed[n:n + rows] = q[:, 0::2] | (q[:, 1::2] << 4)
+        scales[n:n + rows] = scale.squeeze(-1)
+    return packed, scales
+
+
+def dequantize_weight_int4(qweight: torch.Tensor, scale: torch.Tensor):
+    """fp32 weight ``[N, K]`` of a 4-bit weight; for checking only."""
+    q = torch.stack((qweight & 15, qweight >> 4), dim=-1).flatten(-2).float() - 8
+    return (q.view(*scale.shape, -1) * scale.float()[..., None]).flatten(-2)
+
+
+def int4_linear(x: torch.Tensor, qweight: torch.Tensor, scale: torch.Tensor,
+                bias: torch.Tensor | None = None):
+    """y = x @ dequant(qweight).T + bias, the 4-bit counterpart of ``int8_linear``."""
+    return ops.w4a16_linear(x, qweight, scale, bias)
+
+
 def _error_sample(w: torch.Tensor, q: torch.Tensor, s: torch.Tensor, granularity: str,
                   group_size: int) -> float:
     """Relative Frobenius error of the dequantized weight on its first 256
@@ -136,6 +176,49 @@ def _swap_to_int8(name: str, mod: nn.Module, granularity: str, group_size: int) 
                 bytes_before=2 * w.numel(), bytes_after=q.numel() + 2 * s.numel())
 
 
+def _swap_to_int4(name: str, mod: nn.Module, group_size: int) -> dict:
+    """Replace ``mod.weight`` (bf16) by its 4-bit form, as ``_swap_to_int8`` does by int8."""
+    w = mod.weight.data
+    q, s = quantize_weight_int4(w, group_size)
+    n = min(w.shape[0], 256)
+    ref = w[:n].float()
+    err = ((ref - dequantize_weight_int4(q[:n], s[:n])).norm() / ref.norm()).item()
+    mod.weight = nn.Parameter(q, requires_grad=False)
+    mod.weight_scale = nn.Parameter(s, requires_grad=False)
+    mod.quant_granularity, mod.quant_group_size = "per_group", group_size
+    return dict(name=name, shape=list(w.shape), rel_err=err, bytes_before=2 * w.numel(),
+                bytes_after=q.numel() + 2 * s.numel())
+
+
+def _chosen_modules(model: nn.Module, module_names) -> list:
+    """The named ``LinearBase`` submodules with bf16 weights; every name is checked first."""
+    from .linear import LinearBase
+
+    wanted = set(module_names)
+    chosen = [(n, m) for n, m in model.named_modules() if n in wanted]
+    absent = wanted.difference(n for n, _ in chosen)
+    if absent:
+        raise KeyError(f"modules not found in the model: {sorted(absent)}")
+    for name, mod in chosen:
+        if not isinstance(mod, LinearBase):
+            raise TypeError(f"{name} is a {type(mod).__name__}, not a LinearBase")
+        assert mod.weight.dtype == torch.bfloat16, \
+            f"{name}: weight dtype {mod.weight.dtype} is not bf16"
+    return chosen
+
+
+def apply_int4_quant(model: nn.Module, module_names, group_size: int = 128):
+    """``apply_int8_quant`` with 4-bit weights: the named ``LinearBase`` submodules' bf16 weights become
+    packed uint8 ones with a ``weight_scale`` per group, which ``LinearBase._apply`` dispatches to
+    ``int4_linear``. Same report (without the scale statistics), errors and all-or-nothing checks."""
+    chosen = _chosen_modules(model, module_names)
+    for name, mod in chosen:
+        if mod.weight.shape[1] % group_size or group_size % 32:
+            raise ValueError(f"{name}: groups must be a multiple of 32 columns and divide "
+                             f"{mod.weight.shape[1]}, got {group_size}")
+    return [_swap_to_int4(name, mod, group_size) for name, mod in chosen]
+
+
 def apply_int8_quant(model: nn.Module, module_names, granularity: str = "per_channel",
                      group_size: int = 128, verbose: bool = False):
     """Quantize the named ``LinearBase`` submodules of ``model`` in place
@@ -151,18 +234,7 @@ def apply_int8_quant(model: nn.Module, module_names, granularity: str = "per_cha
     ``AssertionError`` for a weight that is not bf16. Every module is checked
     before any is changed, so a refused call leaves the model as it was.
     """
-    from .linear import LinearBase
-
-    wanted = set(module_names)
-    chosen = [(n, m) for n, m in model.named_modules() if n in wanted]
-    absent = wanted.difference(n for n, _ in chosen)
-    if absent:
-        raise KeyError(f"modules not found in the model: {sorted(absent)}")
-    for name, mod in chosen:
-        if not isinstance(mod, LinearBase):
-            raise TypeError(f"{name} is a {type(mod).__name__}, not a LinearBase")
-        assert mod.weight.dtype == torch.bfloat16, \
-            f"{name}: weight dtype {mod.weight.dtype} is not bf16"
+    chosen = _chosen_modules(model, module_names)
     report = [_swap_to_int8(name, mod, granularity, group_size) for name, mod in chosen]
     if verbose:
         for r in report:

@@ -138,6 +138,46 @@ def test_ops_refuse_wrong_tensors():
         ops.w4a16_linear(x, w.to(torch.int8), torch.ones((8, 2)))
 
 
+@pytest.mark.parametrize("n,k,group", [(3, 64, 32), (70, 256, 128), (1, 96, 96)])
+def test_quantize_weight_int4(n, k, group):
+    from specdec_nanovllm_amd.layers.quant import dequantize_weight_int4, quantize_weight_int4
+
+    w = torch.randn((n, k), generator=torch.Generator().manual_seed(n)).to(torch.bfloat16)
+    w[0, :group] = 0
+    q, s = quantize_weight_int4(w, group)
+    assert q.shape == (n, k // 2) and s.shape == (n, k // group) and s.dtype == torch.bfloat16
+    x = w.double().numpy().reshape(n, -1, group)
+    exact = np.maximum(np.abs(x).max(-1) / 7, 1e-8)
+    assert (np.abs(s.double().numpy() - exact) <= 2**-8 * exact * 1.001).all()  # rounded to bf16 once
+    code = np.empty((n, k), dtype=np.int64)
+    code[:, 0::2], code[:, 1::2] = q.numpy() & 15, q.numpy() >> 4
+    assert code.min() >= 1 and code.max() <= 15
+    # the nearest level of the unrounded scale; 2^-20: its fp32 quotient
+    assert (np.abs(code.reshape(x.shape) - 8 - x / exact[..., None]) <= 0.5 + 2**-20).all()
+    assert np.array_equal(dequantize_weight_int4(q, s).double().numpy(), o4.weights(q.numpy(), s.double().numpy()))
+    for bad in (48, 0, 2 * k):
+        with pytest.raises(AssertionError, match="groups"):
+            quantize_weight_int4(w, bad)
+
+
+def test_apply_int4_quant_checks_before_it_changes():
+    from specdec_nanovllm_amd.layers.linear import ReplicatedLinear
+    from specdec_nanovllm_amd.layers.quant import apply_int4_quant
+
+    m = torch.nn.ModuleDict(dict(a=ReplicatedLinear(64, 8), b=ReplicatedLinear(96, 8), c=torch.nn.Linear(64, 8)))
+    for p in m.parameters():
+        p.data = torch.randn(p.shape, generator=torch.Generator().manual_seed(0)).to(torch.bfloat16)
+    for names, group, error in ((["a", "x"], 32, KeyError), (["a", "c"], 32, TypeError), (["a", "b"], 64, ValueError)):
+        with pytest.raises(error):
+            apply_int4_quant(m, names, group)
+        assert m["a"].weight.dtype == torch.bfloat16
+    report = apply_int4_quant(m, ["a", "b"], 32)
+    assert [r["name"] for r in report] == ["a", "b"] and all(0 < r["rel_err"] < 0.15 for r in report)
+    assert m["a"].weight.dtype == torch.uint8 and m["b"].weight_scale.shape == (8, 3)
+    with pytest.raises(RuntimeError, match="ROCm GPU"):  # dispatched to the 4-bit linear, which has no CPU form
+        m["a"](torch.zeros((1, 64), dtype=torch.bfloat16))
+
+
 def test_oracle_orders_are_permutations_and_rounding_is_to_even():
     for f in (o4.key_dim, o4.value_dim):
         assert sorted(f(i) for i in range(128)) == list(range(128))

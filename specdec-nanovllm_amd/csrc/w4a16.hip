@@ -80,12 +80,6 @@ __device__ __forceinline__ u32x4 turn(u32x4 d) {
   return u32x4{a, b, c, e};
 }
 
-// 8 activations in the order 0, 4, 1, 5, 2, 6, 3, 7.
-__device__ __forceinline__ u32x4 reorder(u32x4 v) {
-  return u32x4{__builtin_amdgcn_perm(v.z, v.x, 0x05040100u), __builtin_amdgcn_perm(v.z, v.x, 0x07060302u),
-               __builtin_amdgcn_perm(v.w, v.y, 0x05040100u), __builtin_amdgcn_perm(v.w, v.y, 0x07060302u)};
-}
-
 template <typename T> __device__ __forceinline__ uint32_t minus24() {  // two T of -24
   return __is_same(T, __bf16) ? 0xC1C0C1C0u : 0xCE00CE00u;
 }
@@ -101,25 +95,17 @@ __device__ __forceinline__ uint32_t lds_addr(const void* l) {
       reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) void*)l)));
 }
 
-// The 8 codes of a dword as 8 T of 16 + u in their own order (10 instructions where unpack8 takes 8,
-// for activations that cannot be reordered on their way to LDS).
+// The 8 codes of a dword as 8 T of 16 + u in their own order, which unpack8's order costs activations
+// that go straight to LDS. A byte's two codes reach their halves' mantissas by one product: at bit
+// p of each half the byte moved by p and by 16 + p - 4, which do not meet.
 template <typename T> __device__ __forceinline__ u32x4 unpack8_in_order(uint32_t w, uint32_t base) {
-  // low (high) half bytes at the mantissa bits of a byte each; fp16: within a half, after the perm
-  if constexpr (__is_same(T, __bf16)) {
-    const uint32_t lo = w << 3, hi = w >> 1;
-    u32x4 r;
+  constexpr uint32_t kShift = __is_same(T, __bf16) ? 3 : 6;
+  constexpr uint32_t kBoth = (1u << kShift) | (1u << (kShift + 12));
+  u32x4 r;
 #pragma unroll
-    for (int b = 0; b < 4; ++b)
-      r[b] = (__builtin_amdgcn_perm(hi, lo, 0x0c040c00u + 0x00010001u * b) & sd::Magic<T>::kMask) | base;
-    return r;
-  } else {
-    const uint32_t hi = w >> 4;
-    u32x4 r;
-#pragma unroll
-    for (int b = 0; b < 4; ++b)
-      r[b] = sd::code_pair<T, 0>(__builtin_amdgcn_perm(hi, w, 0x0c040c00u + 0x00010001u * b), base);
-    return r;
-  }
+  for (int b = 0; b < 4; ++b)
+    r[b] = ((((w >> (8 * b)) & 0xffu) * kBoth) & sd::Magic<T>::kMask) | base;
+  return r;
 }
 
 // Up to 2 XI rows. FOLD: MFMAs (32 columns each) between two scalings, 4, 2 or 1. A workgroup takes
@@ -131,6 +117,7 @@ constexpr int kStage = 256;                   // columns of a stage
 constexpr int kTileBytes = 16 * kStage / 2;   // of a tile's weights in a stage
 constexpr int stage_bytes(int xi, int nt) { return nt * kTileBytes + xi * 1024; }
 constexpr int rows_ahead(int xi, int nt) { return xi == 1 && nt == 1 ? 3 : 2; }
+constexpr int wide_tiles(int xi) { return xi == 8 ? 4 : 2; }  // where there are tiles enough, else 1
 
 template <typename T, int FOLD, int XI, int NT>
 __global__ __launch_bounds__(XI == 16 ? 512 : 1024) void w4a16_rows(Args a) {
@@ -359,6 +346,7 @@ void w4a16_gemm(Args a) {
   for (int i = 0; i < CX; ++i) {
     const int r = (wave * CX + i) * 4 + lg;
     xoff[i] = static_cast<uint32_t>(min(static_cast<int64_t>(r), a.M - 1 - m0) * a.xs * 2);
+    if constexpr (FOLD == 4) xoff[i] += 16 * (lr ^ (r & 15));  // whole blocks: no unit past K
   }
   const uint32_t lx_at = lds_addr(&lx[0][0]);
   const int blast = max(b1 - 1, b0);  // past the slice: its last block again, so that every step loads as much
@@ -367,8 +355,11 @@ void w4a16_gemm(Args a) {
     const uint32_t last = 2 * (a.K - blk * kBlock) - 16;  // the last unit of a row, past it again
     const char* xb = xbase + static_cast<int64_t>(blk) * kRow;
 #pragma unroll
-    for (int i = 0; i < CX; ++i)
-      to_lds16(xb, xoff[i] + min(16u * (lr ^ (((wave * CX + i) * 4 + lg) & 15)), last), lx_at + buf * (BM * kRow) + (wave * CX + i) * 1024);
+    for (int i = 0; i < CX; ++i) {
+      uint32_t at = xoff[i];
+      if constexpr (FOLD < 4) at += min(16u * (lr ^ (((wave * CX + i) * 4 + lg) & 15)), last);
+      to_lds16(xb, at, lx_at + buf * (BM * kRow) + (wave * CX + i) * 1024);
+    }
   };
   // ---- weights and scales of this wave's rows
   u32x4 wr[S - 1][NT];
@@ -379,14 +370,15 @@ void w4a16_gemm(Args a) {
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     const uint32_t n = static_cast<uint32_t>(min(n0 + (wn * NT + t) * 16 + lr, a.N - 1) - n0);
-    wrow[t] = n * static_cast<uint32_t>(a.ws);
+    wrow[t] = n * static_cast<uint32_t>(a.ws) + (FOLD == 4 ? 16 * lg : 0);
     srow[t] = n * static_cast<uint32_t>(a.groups);
   }
   auto load_w = [&](int blk, int r) {
     const int kb = min(blk, blast) * kBlock;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
-      wr[r][t] = sd::load16(wbase + (wrow[t] + static_cast<uint32_t>(min(kb + 32 * lg, a.K - 32) / 2)));
+      wr[r][t] = sd::load16(FOLD == 4 ? wbase + kb / 2 + wrow[t]
+                                      : wbase + (wrow[t] + static_cast<uint32_t>(min(kb + 32 * lg, a.K - 32) / 2)));
 #pragma unroll
     for (int f = 0; f < NF; ++f) {
       const int g = group_of(a, min(kb + 32 * FOLD * f, a.K - 32));
@@ -425,11 +417,14 @@ void w4a16_gemm(Args a) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) wf[t][i] = unpack8_in_order<T>(w[i], base);
 #pragma unroll
-      for (int f = 0; f < NF; ++f) sv[t][f] = scale_value<S32>(a, sr[r][t][f]);
+      for (int f = 0; f < NF; ++f) {
+        sv[t][f] = scale_value<S32>(a, sr[r][t][f]);
+        // past K the last columns again (never with whole blocks): they count nothing
+        if (f && blk * kBlock + 32 * FOLD * f >= a.K) sv[t][f] = 0.f;
+      }
     }
     load_x(blk + S - 1, (buf + S - 1) % S);
     load_w(blk + S - 1, r);
-    const int valid = min(4, (a.K - blk * kBlock) / 32);  // 32-column parts of this block
     u32x4 xs[2][4];  // operands of a tile and of the next
 #pragma unroll
     for (int j = 0; j < 4; ++j) xs[0][j] = sd::load16(&lx[buf][x_at[j]]);
@@ -439,11 +434,6 @@ void w4a16_gemm(Args a) {
       if (i + 1 < MT) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) xs[(i + 1) & 1][j] = sd::load16(&lx[buf][x_at[j] + (i + 1) * 16 * kRow]);
-      }
-      if (valid < 4) {
-#pragma unroll
-        for (int j = 1; j < 4; ++j)
-          if (j >= valid) xf[j] = u32x4{0u, 0u, 0u, 0u};
       }
 #pragma unroll
       for (int f = 0; f < NF; ++f) {
@@ -519,7 +509,7 @@ Plan make_plan(int64_t M, int64_t N, int64_t K, int64_t group) {
   // only layers of few tiles and stages stay (32 x 4096 x 1024 5.2 us here and XXX).
   if (M <= 8 || (M <= 16 && all < 16 * cus) || (M <= 32 && all <= cus && stages <= 8)) {
     // tiles that share what a wave reads of x: as many as leave every compute unit a workgroup
-    pl.NT = all < 4 * cus || pl.XI == 16 ? 1 : pl.XI == 8 ? 4 : 2;
+    pl.NT = all < 4 * cus || pl.XI == 16 ? 1 : wide_tiles(pl.XI);
     const int64_t groups = (all + pl.NT - 1) / pl.NT;
     auto bytes = [&](int64_t tiles, int W) {
       return static_cast<size_t>(W) * (rows_ahead(pl.XI, pl.NT) * stage_bytes(pl.XI, pl.NT) +
@@ -556,8 +546,7 @@ Plan make_plan(int64_t M, int64_t N, int64_t K, int64_t group) {
 template <typename T, int FOLD, int XI> void launch_rows(const Args& a, const Plan& pl, hipStream_t st) {
   const dim3 grid(static_cast<unsigned>((a.tiles_n + pl.tiles - 1) / pl.tiles)), block(pl.W * 64);
   if (pl.NT == 1) hipLaunchKernelGGL((w4a16_rows<T, FOLD, XI, 1>), grid, block, pl.lds, st, a);
-  else if (pl.NT == 2) hipLaunchKernelGGL((w4a16_rows<T, FOLD, XI, 2>), grid, block, pl.lds, st, a);
-  else if constexpr (XI == 4 || XI == 8) hipLaunchKernelGGL((w4a16_rows<T, FOLD, XI, 4>), grid, block, pl.lds, st, a);
+  else if constexpr (XI < 16) hipLaunchKernelGGL((w4a16_rows<T, FOLD, XI, wide_tiles(XI)>), grid, block, pl.lds, st, a);
 }
 
 template <typename T, int FOLD, bool S32> void launch_gemm(const Args& a, const Plan& pl, dim3 grid, hipStream_t st) {

@@ -13,10 +13,12 @@
 // Up to 32 rows (w4a16_rows): bound by the weights' bytes, N K / 2. A workgroup takes tiles of 16 weight
 // rows, its waves the columns in turn; their sums meet in LDS and are added in wave order.
 // Activations read by every wave from the caches instead of from LDS kept the address units busy: 75 us
-// at 1 x 151936 x 1024 against XXX.
-// Above (w4a16_gemm): a tile of activation rows goes straight to LDS for the workgroup's waves
-// (global_load_lds, one step of 128 columns ahead), weights to registers; K is split over workgroups
-// where the tiles alone leave compute units idle, and w4a16_reduce adds the slices in order.
+// at 1 x 151936 x 1024 against 22 (78 MB of weights: 3.5 TB/s).
+// Above (w4a16_gemm): activations, weights and scales go straight to LDS for the workgroup's waves
+// (global_load_lds, steps of 128 columns, two or three ahead); K is split over workgroups where the tiles
+// alone leave compute units idle, and w4a16_reduce adds the slices in order. Bound by instruction issue:
+// a step of 128 x 256 outputs takes 2.0 us, of which its MFMAs, a fifth of them for the -24 sum x, are 1.1
+// (4096 x 19456 x 2560: 449 us, 910 TFLOP/s; 777 rows 114 us).
 #include <type_traits>
 
 #include "int4.h"
@@ -43,6 +45,7 @@ struct Args {
   int32_t tiles;  // w4a16_rows: groups of weight tiles a workgroup
   float* part;    // K slices: [slices][M][N] sums
   int32_t tiles_m, tiles_n, slices;
+  int32_t wide_y;  // 16-byte stores of y are aligned
 };
 
 // Group of column k: k / 32 is below 2^15 and a group below 2^20 columns, where the product with the
@@ -54,6 +57,10 @@ __device__ __forceinline__ int group_of(const Args& a, int k) {
 template <bool S32> __device__ __forceinline__ uint32_t load_scale(const Args& a, int64_t at) {
   if constexpr (S32) return static_cast<const uint32_t*>(a.scale)[at];
   else return static_cast<const uint16_t*>(a.scale)[at];
+}
+template <typename ST> __device__ __forceinline__ float scale_of(uint32_t bits) {
+  if constexpr (sizeof(ST) == 4) return __uint_as_float(bits);
+  else return sd::from_bits<ST>(static_cast<uint16_t>(bits));
 }
 template <bool S32> __device__ __forceinline__ float scale_value(const Args& a, uint32_t bits) {
   if constexpr (S32) return __uint_as_float(bits);
@@ -90,6 +97,15 @@ __device__ __forceinline__ void to_lds16(const void* base, uint32_t off, uint32_
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                ::"s"(l), "v"(off), "s"(base) : "memory", "m0");
 }
+// 32 bits a lane: a 16-bit word lands zero-extended.
+template <bool S32> __device__ __forceinline__ void scale_to_lds(const void* base, uint32_t off, uint32_t l) {
+  if constexpr (S32)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2"
+                 ::"s"(l), "v"(off), "s"(base) : "memory", "m0");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ushort %1, %2"
+                 ::"s"(l), "v"(off), "s"(base) : "memory", "m0");
+}
 __device__ __forceinline__ uint32_t lds_addr(const void* l) {
   return __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(
       reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) void*)l)));
@@ -117,7 +133,6 @@ constexpr int kStage = 256;                   // columns of a stage
 constexpr int kTileBytes = 16 * kStage / 2;   // of a tile's weights in a stage
 constexpr int stage_bytes(int xi, int nt) { return nt * kTileBytes + xi * 1024; }
 constexpr int rows_ahead(int xi, int nt) { return xi == 1 && nt == 1 ? 3 : 2; }
-constexpr int wide_tiles(int xi) { return xi == 8 ? 4 : 2; }  // where there are tiles enough, else 1
 
 template <typename T, int FOLD, int XI, int NT>
 __global__ __launch_bounds__(XI == 16 ? 512 : 1024) void w4a16_rows(Args a) {
@@ -307,84 +322,94 @@ __global__ __launch_bounds__(XI == 16 ? 512 : 1024) void w4a16_rows(Args a) {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
-// WM x WN waves of MT x NT tiles of 16 x 16 outputs; S stages of activations in LDS, S - 1 blocks of weights
-// in registers.
-template <typename T, int FOLD, bool S32, int WM, int WN, int MT, int NT, int S>
+// WM x WN waves of MT x NT tiles of 16 x 16 outputs; S stages of activations, weights and scales in LDS,
+// all of them loaded S - 1 steps ahead straight from memory. (Weights and scales loaded to registers
+// instead: the compiler's waits for them were waits for the activations behind them as well, 559 us.)
+// The MFMAs take the weights as their rows: a lane then holds neighbouring outputs of one row, and the
+// tile leaves through LDS in whole lines (2-byte stores of the other order: 487 us; 8-byte ones 661).
+// Where there are 8 waves, two share a SIMD: they take turns, one unpacks while the other multiplies
+// (503 us without; these three at 4096 x 19456 x 2560, between the first form's 559 and 449 now).
+template <typename T, typename ST, int FOLD, int WM, int WN, int MT, int NT, int S>
 __global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(2)))
 void w4a16_gemm(Args a) {
   constexpr int NW = WM * WN, BM = 16 * MT * WM, BN = 16 * NT * WN, NF = 4 / FOLD;
   constexpr int kRow = 2 * kBlock;                // bytes of an activation row's step
   constexpr int CX = BM * kRow / 1024 / NW;       // 1 KB loads (4 rows) of a wave and step
-  static_assert(CX * NW * 1024 == BM * kRow, "whole 1 KB loads");
-  __shared__ __attribute__((aligned(1024))) uint8_t lx[S][BM * kRow];
+  constexpr int CW = (WN * NT + NW - 1) / NW;     // 1 KB loads (a tile's 16 rows) of a wave and step
+  constexpr int kX = BM * kRow, kW = CW * NW * 1024, kS = NF * 256, kBytes = kX + kW + NW * kS;
+  static_assert(CX * NW * 1024 == kX, "whole 1 KB loads");
+  static_assert(S * kBytes <= (160 << 10), "a compute unit's LDS");
+  __shared__ __attribute__((aligned(1024))) uint8_t sm[S * kBytes];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 15, lg = lane >> 4;
   const int wm = wave / WN, wn = wave % WN;
 
   // Workgroup -> (slice, tile): every eighth workgroup shares an XCD (one L2), so each XCD takes a
-  // contiguous run of tiles, all activation tiles of a weight tile before the next.
+  // contiguous run: 8 activation tiles by all weight tiles, then the next 8.
   const int items = a.tiles_m * a.tiles_n * a.slices;
   int id = blockIdx.x;
   {
     const int per = items / 8, rem = items % 8, xcd = id % 8;
     id = xcd * per + min(xcd, rem) + id / 8;
   }
-  const int m_tile = id % a.tiles_m, rest = id / a.tiles_m;
+  const int band = 8 * a.tiles_n * a.slices, band_i = id / band, in_band = id - band_i * band;
+  const int rows = min(8, a.tiles_m - 8 * band_i);
+  const int m_tile = 8 * band_i + in_band % rows, rest = in_band / rows;
   const int slice = rest % a.slices, n_tile = rest / a.slices;
   const int64_t m0 = static_cast<int64_t>(m_tile) * BM, n0 = static_cast<int64_t>(n_tile) * BN;
   const int blocks = (a.K + kBlock - 1) / kBlock;
   const int b0 = static_cast<int>(static_cast<int64_t>(slice) * blocks / a.slices);
   const int b1 = static_cast<int>(static_cast<int64_t>(slice + 1) * blocks / a.slices);
 
-  // ---- activations: 16-byte unit u of row r stands at unit u ^ (r % 16) of its LDS row, so that the
-  //      16 rows of an operand read hit 16 different units
+  // ---- loads. Activations: 16-byte unit u of row r stands at unit u ^ (r % 16) of its LDS row, so that
+  //      the 16 rows of an operand read hit 16 different units. Weights: a lane's unit as it reads it.
+  //      With groups of whole blocks (FOLD == 4) no unit lies past K.
   const char* xbase = reinterpret_cast<const char*>(a.x + m0 * a.xs);
-  static_assert(CX % 2 == 0, "a wave's rows start at a multiple of 8");
-  uint32_t xoff[CX];
+  uint32_t xoff[CX], woff[CW];
 #pragma unroll
   for (int i = 0; i < CX; ++i) {
     const int r = (wave * CX + i) * 4 + lg;
     xoff[i] = static_cast<uint32_t>(min(static_cast<int64_t>(r), a.M - 1 - m0) * a.xs * 2);
-    if constexpr (FOLD == 4) xoff[i] += 16 * (lr ^ (r & 15));  // whole blocks: no unit past K
+    if constexpr (FOLD == 4) xoff[i] += 16 * (lr ^ (r & 15));
   }
-  const uint32_t lx_at = lds_addr(&lx[0][0]);
+  const uint8_t* const wbase = a.w + n0 * a.ws;
+  const int64_t last_n = a.N - 1 - n0;
+#pragma unroll
+  for (int i = 0; i < CW; ++i) {
+    const int q = wave * CW + i, t = q % NT;
+    const int r = min(q / NT * (16 * NT) + 4 * NT * (lr >> 2) + 4 * t + (lr & 3), BN - 1);
+    woff[i] = static_cast<uint32_t>(min(static_cast<int64_t>(r), last_n)) * static_cast<uint32_t>(a.ws);
+    if constexpr (FOLD == 4) woff[i] += 16 * lg;
+  }
+  constexpr int kScale = sizeof(ST);
+  const char* const sbase = static_cast<const char*>(a.scale) + n0 * a.groups * kScale;
+  const uint32_t soff =
+      static_cast<uint32_t>(min(static_cast<int64_t>(wn * NT * 16 + min(lane, NT * 16 - 1)), last_n)) * a.groups * kScale;
+  const uint32_t sm_at = lds_addr(sm);
   const int blast = max(b1 - 1, b0);  // past the slice: its last block again, so that every step loads as much
-  auto load_x = [&](int blk, int buf) {
+  auto load = [&](int blk, int buf) {
     blk = min(blk, blast);
-    const uint32_t last = 2 * (a.K - blk * kBlock) - 16;  // the last unit of a row, past it again
+    const uint32_t at = sm_at + buf * kBytes;
     const char* xb = xbase + static_cast<int64_t>(blk) * kRow;
+    const uint32_t last = 2 * (a.K - blk * kBlock) - 16;  // the last unit of a row, past it again
 #pragma unroll
     for (int i = 0; i < CX; ++i) {
-      uint32_t at = xoff[i];
-      if constexpr (FOLD < 4) at += min(16u * (lr ^ (((wave * CX + i) * 4 + lg) & 15)), last);
-      to_lds16(xb, at, lx_at + buf * (BM * kRow) + (wave * CX + i) * 1024);
+      uint32_t off = xoff[i];
+      if constexpr (FOLD < 4) off += min(16u * (lr ^ (((wave * CX + i) * 4 + lg) & 15)), last);
+      to_lds16(xb, off, at + (wave * CX + i) * 1024);
     }
-  };
-  // ---- weights and scales of this wave's rows
-  u32x4 wr[S - 1][NT];
-  uint32_t sr[S - 1][NT][NF];
-  const uint8_t* const wbase = a.w + n0 * a.ws;
-  const int64_t sbase = n0 * a.groups;
-  uint32_t wrow[NT], srow[NT];  // from the tile's first row
+    const uint8_t* wb = wbase + blk * (kBlock / 2);
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const uint32_t n = static_cast<uint32_t>(min(n0 + (wn * NT + t) * 16 + lr, a.N - 1) - n0);
-    wrow[t] = n * static_cast<uint32_t>(a.ws) + (FOLD == 4 ? 16 * lg : 0);
-    srow[t] = n * static_cast<uint32_t>(a.groups);
-  }
-  auto load_w = [&](int blk, int r) {
-    const int kb = min(blk, blast) * kBlock;
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-      wr[r][t] = sd::load16(FOLD == 4 ? wbase + kb / 2 + wrow[t]
-                                      : wbase + (wrow[t] + static_cast<uint32_t>(min(kb + 32 * lg, a.K - 32) / 2)));
-#pragma unroll
-    for (int f = 0; f < NF; ++f) {
-      const int g = group_of(a, min(kb + 32 * FOLD * f, a.K - 32));
-#pragma unroll
-      for (int t = 0; t < NT; ++t) sr[r][t][f] = load_scale<S32>(a, sbase + (srow[t] + static_cast<uint32_t>(g)));
+    for (int i = 0; i < CW; ++i) {
+      uint32_t off = woff[i];
+      if constexpr (FOLD < 4) off += min(16u * lg, static_cast<uint32_t>(a.K / 2 - 16 - blk * (kBlock / 2)));
+      to_lds16(wb, off, at + kX + (wave * CW + i) * 1024);
     }
+#pragma unroll
+    for (int f = 0; f < NF; ++f)
+      scale_to_lds<kScale == 4>(sbase + group_of(a, min(blk * kBlock + 32 * FOLD * f, a.K - 32)) * kScale, soff,
+                        at + kX + kW + wave * kS + f * 256);
   };
 
   const uint32_t base = sd::code_base<T>();
@@ -399,47 +424,67 @@ void w4a16_gemm(Args a) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) x_at[j] = (wm * MT * 16 + lr) * kRow + (((4 * j + lg) ^ lr) * 16);
 
-  constexpr int kLoads = CX + NT + NT * NF;  // vector memory instructions of a step
+  constexpr int kLoads = CX + CW + NF;  // vector memory instructions of a step
 #pragma unroll
-  for (int i = 0; i < S - 1; ++i) {
-    load_x(b0 + i, i);
-    load_w(b0 + i, i);
-  }
-  auto step = [&](int blk, int r) {  // r: blk's slot of the weights (a constant)
-    const int buf = (blk - b0) % S;
-    // this step's activations have landed in every wave's view, the last step's are read
+  for (int i = 0; i < S - 1; ++i) load(b0 + i, i);
+  int buf = 0;
+  constexpr bool kTurns = NW == 8;  // waves w and w + 4 are on one SIMD
+  const bool second = kTurns && wave >= 4;
+  // All but the newest S - 2 steps' loads have landed in every wave's view, and every LDS read so far is
+  // done: the slot of the step before is free. The second waves run half a step behind: while they
+  // multiply step b the first unpack b + 1, so the first load b + S - 1 only after their middle meeting.
+  auto meet = [&]() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((S - 2) * kLoads) : "memory");
+  };
+  if (second) meet();
+  for (int blk = b0; blk < b1; ++blk) {
+    meet();
+    const uint8_t* const lx = sm + buf * kBytes;
+    if (!kTurns || second) load(blk + S - 1, buf == 0 ? S - 1 : buf - 1);
     u32x4 wf[NT][4];
-    float sv[NT][NF];
+    f32x4 sv[NT][NF];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const u32x4 w = turn(wr[r][t]);
+      const u32x4 w = turn(sd::load16(lx + kX + (wn * NT + t) * 1024 + lane * 16));
 #pragma unroll
       for (int i = 0; i < 4; ++i) wf[t][i] = unpack8_in_order<T>(w[i], base);
 #pragma unroll
       for (int f = 0; f < NF; ++f) {
-        sv[t][f] = scale_value<S32>(a, sr[r][t][f]);
+        const u32x4 bits = sd::load16(lx + kX + kW + wave * kS + f * 256 + (4 * NT * lg + 4 * t) * 4);
         // past K the last columns again (never with whole blocks): they count nothing
-        if (f && blk * kBlock + 32 * FOLD * f >= a.K) sv[t][f] = 0.f;
+        const bool none = f && blk * kBlock + 32 * FOLD * f >= a.K;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sv[t][f][e] = none ? 0.f : scale_of<ST>(bits[e]);
       }
     }
-    load_x(blk + S - 1, (buf + S - 1) % S);
-    load_w(blk + S - 1, r);
+    if constexpr (kTurns) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(wf[t][i]));
+#pragma unroll
+        for (int f = 0; f < NF; ++f) asm volatile("" : "+v"(sv[t][f]));
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      meet();
+      if (!second) load(blk + S - 1, buf == 0 ? S - 1 : buf - 1);
+      __builtin_amdgcn_s_setprio(1);
+    }
     u32x4 xs[2][4];  // operands of a tile and of the next
 #pragma unroll
-    for (int j = 0; j < 4; ++j) xs[0][j] = sd::load16(&lx[buf][x_at[j]]);
+    for (int j = 0; j < 4; ++j) xs[0][j] = sd::load16(lx + x_at[j]);
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
       u32x4(&xf)[4] = xs[i & 1];
       if (i + 1 < MT) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) xs[(i + 1) & 1][j] = sd::load16(&lx[buf][x_at[j] + (i + 1) * 16 * kRow]);
+        for (int j = 0; j < 4; ++j) xs[(i + 1) & 1][j] = sd::load16(lx + x_at[j] + (i + 1) * 16 * kRow);
       }
 #pragma unroll
       for (int f = 0; f < NF; ++f) {
         f32x4 start = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int j = 0; j < FOLD; ++j) start = sd::Elem<T>::mfma(xf[f * FOLD + j], m24, start);
+        for (int j = 0; j < FOLD; ++j) start = sd::Elem<T>::mfma(m24, xf[f * FOLD + j], start);
         f32x4 d[NT];
 #pragma unroll
         for (int t = 0; t < NT; ++t) d[t] = start;
@@ -447,36 +492,65 @@ void w4a16_gemm(Args a) {
         for (int j = 0; j < FOLD; ++j)
 #pragma unroll
           for (int t = 0; t < NT; ++t)
-            d[t] = sd::Elem<T>::mfma(xf[f * FOLD + j], wf[t][f * FOLD + j], d[t]);
+            d[t] = sd::Elem<T>::mfma(wf[t][f * FOLD + j], xf[f * FOLD + j], d[t]);
 #pragma unroll
         for (int t = 0; t < NT; ++t) acc[i][t] += sv[t][f] * d[t];
       }
       // one tile after another: with all tiles' operands hoisted the accumulators spill
       __builtin_amdgcn_sched_barrier(0);
     }
-  };
-  for (int blk = b0; blk < b1; blk += S - 1) {
-#pragma unroll
-    for (int r = 0; r < S - 1; ++r)
-      if (blk + r < b1) step(blk + r, r);
+    __builtin_amdgcn_s_setprio(0);
+    buf = buf + 1 == S ? 0 : buf + 1;
   }
+  if (kTurns && !second) meet();
   // the loads that ran ahead land before the workgroup's LDS is another's
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  // ---- a lane's 4 NT neighbouring outputs of a row of every activation tile, through LDS to whole lines
+  auto out = [&](auto one, auto* to, int64_t stride, bool wide) {
+    using O = decltype(one);
+    constexpr int kPitch = BN * sizeof(O) + 16, kUnit = 16 / sizeof(O), kUnits = BN / kUnit;
+    static_assert(BM * kPitch <= S * kBytes, "the tile fits where the stages were");
+    const int64_t n = n0 + wn * (16 * NT) + 4 * NT * lg;
+    __syncthreads();
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const int64_t n = n0 + (wn * NT + t) * 16 + lr;
-    if (n >= a.N) continue;
-    const float b = a.bias && a.slices == 1 ? sd::from_bits<T>(a.bias[n]) : 0.f;
+    for (int t = 0; t < NT; ++t) {
+      f32x4 bias = {0.f, 0.f, 0.f, 0.f};
+      if (a.bias && a.slices == 1) {
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int64_t m = m0 + (wm * MT + i) * 16 + 4 * lg + e;
-        if (m >= a.M) continue;
-        if (a.slices > 1) a.part[(slice * a.M + m) * a.N + n] = acc[i][t][e];
-        else a.y[m * a.ys + n] = sd::to_bits<T>(acc[i][t][e] + b);
+        for (int e = 0; e < 4; ++e)
+          bias[e] = sd::from_bits<T>(a.bias[min(n + 4 * t + e, a.N - 1)]);
       }
-  }
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        O* p = reinterpret_cast<O*>(sm + ((wm * MT + i) * 16 + lr) * kPitch) + wn * (16 * NT) + 4 * NT * lg + 4 * t;
+        const f32x4 v = acc[i][t] + bias;
+        if constexpr (sizeof(O) == 4) *reinterpret_cast<f32x4*>(p) = v;
+        else {
+          union { uint16_t h[4]; uint2 u; } o;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o.h[e] = sd::to_bits<T>(v[e]);
+          *reinterpret_cast<uint2*>(p) = o.u;
+        }
+      }
+    }
+    __syncthreads();
+    const int rows = static_cast<int>(min(static_cast<int64_t>(BM), a.M - m0));
+    const int cols = static_cast<int>(min(static_cast<int64_t>(BN), a.N - n0));
+    O* const y0 = to + m0 * stride + n0;
+    if (wide && cols % kUnit == 0) {
+      for (int i = tid; i < rows * kUnits; i += NW * 64) {
+        const int r = i / kUnits, u = i % kUnits;
+        if (u * kUnit < cols) *reinterpret_cast<u32x4*>(y0 + r * stride + u * kUnit) = sd::load16(sm + r * kPitch + u * 16);
+      }
+    } else {
+      for (int i = tid; i < rows * BN; i += NW * 64) {
+        const int r = i / BN, c = i % BN;
+        if (c < cols) y0[r * stride + c] = *reinterpret_cast<const O*>(sm + r * kPitch + c * sizeof(O));
+      }
+    }
+  };
+  if (a.slices > 1) out(0.f, a.part + slice * a.M * a.N, a.N, a.N % 4 == 0);
+  else out(uint16_t{}, a.y, a.ys, a.wide_y != 0);
 }
 
 // Sum of the K slices, in slice order, bias, rounding.
@@ -505,11 +579,11 @@ Plan make_plan(int64_t M, int64_t N, int64_t K, int64_t group) {
   const int64_t all = (N + 15) / 16, stages = (K + kStage - 1) / kStage;  // weight tiles, their stages
   pl.XI = M <= 2 ? 1 : M <= 8 ? 4 : M <= 16 ? 8 : 16;
   // Every wave reads its own share of x: past 8 rows that is more than the weights. Tiles of w4a16_gemm
-  // share it: 16 x 151936 x 1024 33 us there and XXX here; past 16 rows (32 x 19456 x 2560 XXX and 30 us)
-  // only layers of few tiles and stages stay (32 x 4096 x 1024 5.2 us here and XXX).
-  if (M <= 8 || (M <= 16 && all < 16 * cus) || (M <= 32 && all <= cus && stages <= 8)) {
-    // tiles that share what a wave reads of x: as many as leave every compute unit a workgroup
-    pl.NT = all < 4 * cus || pl.XI == 16 ? 1 : wide_tiles(pl.XI);
+  // share it: 16 x 19456 x 2560 16 us there and 19 here, 16 x 2560 x 9728 34 and 10; past 16 rows (32 x
+  // 2560 x 9728 14 and 20) only layers of few tiles and stages stay (32 x 4096 x 1024 7.5 and 5.5).
+  if (M <= 8 || (M <= 16 && all < 4 * cus) || (M <= 32 && all <= cus && stages <= 8)) {
+    // two tiles share what a wave reads of x where there are workgroups enough
+    pl.NT = all < 4 * cus ? 1 : 2;
     const int64_t groups = (all + pl.NT - 1) / pl.NT;
     auto bytes = [&](int64_t tiles, int W) {
       return static_cast<size_t>(W) * (rows_ahead(pl.XI, pl.NT) * stage_bytes(pl.XI, pl.NT) +
@@ -532,35 +606,61 @@ Plan make_plan(int64_t M, int64_t N, int64_t K, int64_t group) {
     if (pl.lds <= (160 << 10)) return pl;
   }
   pl.XI = 0;
-  pl.bm = M <= 32 ? 32 : M <= 64 ? 64 : 128;
-  if (M > 64) pl.bn = fold < 4 ? 64 : 128;  // (a scale for every one or two MFMAs: too many registers for 128)
-  else pl.bn = (N + 127) / 128 * 4 < 2 * cus ? 64 : 128;
-  const int64_t tiles = ((M + pl.bm - 1) / pl.bm) * ((N + pl.bn - 1) / pl.bn);
-  // two workgroups a compute unit, slices of two steps or more
-  int64_t s = tiles >= cus ? 1 : (2 * cus) / tiles;
-  if (s > blocks / 2) s = blocks / 2;
-  pl.slices = s < 1 ? 1 : s > 16 ? 16 : static_cast<int>(s);
+  auto tiles_of = [&](int bn) { return ((M + pl.bm - 1) / pl.bm) * ((N + bn - 1) / bn); };
+  if (M <= 64) {
+    pl.bm = M <= 32 ? 32 : 64;
+    pl.bn = (N + 127) / 128 * 4 < 2 * cus ? 64 : 128;
+    // two workgroups a compute unit, slices of two steps or more
+    const int64_t tiles = tiles_of(pl.bn);
+    int64_t s = tiles >= cus ? 1 : (2 * cus) / tiles;
+    if (s > blocks / 2) s = blocks / 2;
+    pl.slices = s < 1 ? 1 : s > 16 ? 16 : static_cast<int>(s);
+    return pl;
+  }
+  // One workgroup a compute unit: the columns and slices of the least time, by ns that were measured at
+  // 4096 rows: a step 1380 with 128 columns, 2200 with 256; slices cost a launch and their sums' way to
+  // memory and back. (777 x 19456 x 2560: 128 143 us, 192 114, 256 132; 777 x 2560 x 9728: 104, 81, 71;
+  // 777 x 4096 x 1024: 16, 20, 22.)
+  pl.bm = 128;
+  int64_t least = INT64_MAX;
+  for (int bn = 128; bn <= (fold == 1 ? 128 : 256); bn += 64) {
+    const int64_t t = tiles_of(bn), most = t >= cus ? 1 : blocks / 2 < 16 ? blocks / 2 : 16;
+    for (int64_t s = 1; s == 1 || (s <= most && t * s <= cus); ++s) {
+      const int64_t cost = (t * s + cus - 1) / cus * ((blocks + s - 1) / s) * (560 + 32 * bn / 5) +
+                           (s > 1 ? 3000 + s * M * N / 500 : 0);
+      if (cost < least) {
+        least = cost;
+        pl.bn = bn;
+        pl.slices = static_cast<int>(s);
+      }
+    }
+  }
   return pl;
 }
 
 template <typename T, int FOLD, int XI> void launch_rows(const Args& a, const Plan& pl, hipStream_t st) {
   const dim3 grid(static_cast<unsigned>((a.tiles_n + pl.tiles - 1) / pl.tiles)), block(pl.W * 64);
   if (pl.NT == 1) hipLaunchKernelGGL((w4a16_rows<T, FOLD, XI, 1>), grid, block, pl.lds, st, a);
-  else if constexpr (XI < 16) hipLaunchKernelGGL((w4a16_rows<T, FOLD, XI, wide_tiles(XI)>), grid, block, pl.lds, st, a);
+  else if constexpr (XI < 8) hipLaunchKernelGGL((w4a16_rows<T, FOLD, XI, 2>), grid, block, pl.lds, st, a);
 }
 
-template <typename T, int FOLD, bool S32> void launch_gemm(const Args& a, const Plan& pl, dim3 grid, hipStream_t st) {
+template <typename T, typename ST, int FOLD> void launch_gemm(const Args& a, const Plan& pl, dim3 grid, hipStream_t st) {
   const dim3 block(256);
-  if (pl.bm == 128)
-    hipLaunchKernelGGL((w4a16_gemm<T, FOLD, S32, 2, 2, 4, FOLD < 4 ? 2 : 4, 2>), grid, block, 0, st, a);
-  else if (pl.bm == 64 && pl.bn == 128)
-    hipLaunchKernelGGL((w4a16_gemm<T, FOLD, S32, 1, 4, 4, 2, 4>), grid, block, 0, st, a);
+  if (pl.bm == 128 && pl.bn == 128)
+    hipLaunchKernelGGL((w4a16_gemm<T, ST, FOLD, 2, 4, 4, 2, 3>), grid, dim3(512), 0, st, a);
+  else if (pl.bm == 128) {
+    if constexpr (FOLD > 1) {
+      if (pl.bn == 256) hipLaunchKernelGGL((w4a16_gemm<T, ST, FOLD, 2, 4, 4, 4, 3>), grid, dim3(512), 0, st, a);
+      else hipLaunchKernelGGL((w4a16_gemm<T, ST, FOLD, 2, 4, 4, 3, 3>), grid, dim3(512), 0, st, a);
+    }
+  } else if (pl.bm == 64 && pl.bn == 128)
+    hipLaunchKernelGGL((w4a16_gemm<T, ST, FOLD, 1, 4, 4, 2, 3>), grid, block, 0, st, a);
   else if (pl.bm == 64)
-    hipLaunchKernelGGL((w4a16_gemm<T, FOLD, S32, 1, 4, 4, 1, 4>), grid, block, 0, st, a);
+    hipLaunchKernelGGL((w4a16_gemm<T, ST, FOLD, 1, 4, 4, 1, 3>), grid, block, 0, st, a);
   else if (pl.bn == 128)
-    hipLaunchKernelGGL((w4a16_gemm<T, FOLD, S32, 1, 4, 2, 2, 4>), grid, block, 0, st, a);
+    hipLaunchKernelGGL((w4a16_gemm<T, ST, FOLD, 1, 4, 2, 2, 4>), grid, block, 0, st, a);
   else
-    hipLaunchKernelGGL((w4a16_gemm<T, FOLD, S32, 1, 4, 2, 1, 4>), grid, block, 0, st, a);
+    hipLaunchKernelGGL((w4a16_gemm<T, ST, FOLD, 1, 4, 2, 1, 4>), grid, block, 0, st, a);
 }
 
 template <typename T, int FOLD> int launch(Args a, int64_t group, hipStream_t st) {
@@ -578,8 +678,9 @@ template <typename T, int FOLD> int launch(Args a, int64_t group, hipStream_t st
   a.tiles_m = static_cast<int32_t>((a.M + pl.bm - 1) / pl.bm);
   a.tiles_n = static_cast<int32_t>((a.N + pl.bn - 1) / pl.bn);
   const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.tiles_m) * a.tiles_n * a.slices));
-  if (a.scale_f32) launch_gemm<T, FOLD, true>(a, pl, grid, st);
-  else launch_gemm<T, FOLD, false>(a, pl, grid, st);
+  if (a.scale_f32) launch_gemm<T, float, FOLD>(a, pl, grid, st);
+  else if (a.scale_f16) launch_gemm<T, _Float16, FOLD>(a, pl, grid, st);
+  else launch_gemm<T, __bf16, FOLD>(a, pl, grid, st);
   const int rc = sd::check_launch("w4a16_linear");
   if (rc != SD_OK || a.slices == 1) return rc;
   int64_t wgs = (a.M * a.N + 255) / 256;
@@ -668,6 +769,7 @@ extern "C" int sd_w4a16_linear(const void* x, int64_t x_stride_m, const uint8_t*
   a.bias = static_cast<const uint16_t*>(bias);
   a.y = static_cast<uint16_t*>(y);
   a.ys = y_stride_m;
+  a.wide_y = sd::aligned16(y) && y_stride_m % 8 == 0;
   a.M = M;
   a.N = N;
   a.K = static_cast<int32_t>(K);

@@ -670,7 +670,9 @@ int sd_load_kvcache_int4(const void* codes, int64_t codes_stride_block, int64_t 
  * clamps and limits as sd_paged_attention ((num_q_heads / num_kv_heads) *
  * max_qlen <= 32; rows without a visible key are zero; rows at or beyond
  * total_q are neither read nor written). Sums and softmax in fp32, one
- * rounding at the end. Keys that a row does not see may hold anything.
+ * rounding at the end. Keys that a row does not see may hold anything. The cache's
+ * strides are not negative: of positions at most 2^25 bytes of codes and 2^24 scales,
+ * of blocks and heads below 2^32 bytes.
  * workspace: >= sd_paged_attention_int4_workspace_size(...) bytes (0: none
  * needed), 16-byte aligned, queried on the same device; num_splits 0 = library
  * default, n > 0 = n workgroups per (sequence, kv head) on average. The result
@@ -701,12 +703,12 @@ int sd_paged_attention_int4(const void* q, int64_t q_stride_tok, int64_t q_strid
  *           byte j holds the codes of columns 2 j (low half) and 2 j + 1
  *   scale : (N, K / group_size) row-major, scale_dtype bf16/f16/f32
  *   bias  : (N,) dtype or NULL
- *   y     : (M, N) dtype, row stride y_stride_m, sharing no byte with x
+ *   y     : (M, N) dtype, row stride y_stride_m (>= N), sharing no byte with x
  * group_size: a multiple of 32 that divides K. fp32 sums, one rounding. A row of
  * x with an infinity, or with values past 2^120, gives NaN where a product with
  * the weight alone would give an infinity (the sums are of code + 16, less 24 sum x).
  * workspace: sd_w4a16_workspace_size bytes on the same device, 16-byte aligned (partial
- * sums of K slices, where more than 32 rows leave compute units idle; 0 elsewhere). Without it
+ * sums of K slices, where more than 8 rows leave compute units idle; 0 elsewhere). Without it
  * (NULL or too small) the call runs in one slice. x_stride_m and w_stride_n <= 2^24, K <= 2^20.
  */
 size_t sd_w4a16_workspace_size(int64_t M, int64_t N, int64_t K, int32_t group_size);

@@ -14,8 +14,9 @@
 // Work: a pair is one (sequence, kv head), a chunk 128 keys of one pair: 32 for each of the 4 waves
 // of a workgroup (64 keys where a pair has two 16-row tiles: two waves then take the same keys, one
 // tile each, and share what they load in the caches; one wave with both tiles has no registers left
-// for a second wave on its SIMD and measured 32 us instead of XXX us for 8 x 7 rows). All chunks, laid end to end, are cut into equal runs, one a workgroup, whatever
-// the length mix (context lengths are read on the device). When a pair or the run ends, the waves
+// for a second wave on its SIMD and measured 32 us instead of 22 us for 8 x 7 rows). All chunks, laid end
+// to end, are cut into equal runs, one a workgroup, whatever the length mix (context lengths are read
+// on the device). When a pair or the run ends, the waves
 // merge their softmax states in LDS; a pair that several runs share leaves partials in the workspace
 // (two slots a run: the pair it starts in, the pair it ends in), which the combine kernel merges.
 // Where the table admits few chunks a pair, a run is one whole pair and there is no second launch.
@@ -45,7 +46,8 @@ constexpr int kStep = 32;               // keys of a wave's step
 constexpr int kPitch = kD + 4;          // floats of a row's state: acc, then m and l
 constexpr int kMergeRows = 8;           // rows of a tile the waves merge at a time
 // Tables of up to this many keys: no splitting of pairs, and past kShortKeys twice the waves. One launch
-// of 8 steps' length at most against two (16 heads, 1 x 1000 keys: XXX against 10.0 us in a graph).
+// of 8 steps' length at most against two (16 heads, 1 x 1000 keys: 10.9 us a call against 14.8; without
+// the host, from a graph, 11.4 against 10.0: a call from the host is what a decode step of one pays).
 constexpr int kShortKeys = 512, kWholeKeys = 1024;
 
 struct Params {

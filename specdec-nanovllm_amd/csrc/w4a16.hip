@@ -751,6 +751,10 @@ extern "C" int sd_w4a16_linear(const void* x, int64_t x_stride_m, const uint8_t*
     sd::set_error("%s: x and weight rows must be 16-byte aligned", what);
     return SD_ERR_UNSUPPORTED;
   }
+  if (M > 1 && y_stride_m < N) {
+    sd::set_error("%s: rows of y overlap (stride %lld, %lld columns)", what, (long long)y_stride_m, (long long)N);
+    return SD_ERR_VALUE;
+  }
   if (sd::span16(x, M, x_stride_m, K).overlaps(sd::span16(y, M, y_stride_m, N))) {
     sd::set_error("%s: y shares memory with x", what);
     return SD_ERR_VALUE;

@@ -789,17 +789,19 @@ def w4a16_linear(x: torch.Tensor, qweight: torch.Tensor, scale: torch.Tensor,
     if out is None:
         y = torch.empty((M, N), device=dev, dtype=x.dtype)
     else:
+        assert out.shape == (*x.shape[:-1], N), f"out must be {(*x.shape[:-1], N)}, got {tuple(out.shape)}"
         y = out.view(M, N)
         assert y.dtype == x.dtype and (N == 1 or y.stride(1) == 1)
     if M:
         lib = _lib.load()
         with _lib.on_device(dev):
-            # the plan (and so the workspace) depends on the device's compute units; none up to 16 rows
-            ws_bytes = lib.sd_w4a16_workspace_size(M, N, K, K // groups) if M > 16 else 0
+            # the plan (and so the workspace) depends on the device's compute units; none up to 8 rows
+            ws_bytes = lib.sd_w4a16_workspace_size(M, N, K, K // groups) if M > 8 else 0
             ws = _workspace(ws_bytes, dev)
             rc = lib.sd_w4a16_linear(
                 x2.data_ptr(), x0, qw.data_ptr(), K // 2, sc.data_ptr(), _lib.dtype_code(sc.dtype),
-                K // groups, _ptr(b), y.data_ptr(), y.stride(0), M, N, K, _lib.dtype_code(x.dtype), _ptr(ws), ws_bytes, _lib.stream_ptr(dev))
+                K // groups, _ptr(b), y.data_ptr(), y.stride(0), M, N, K, _lib.dtype_code(x.dtype),
+                _ptr(ws), ws_bytes, _lib.stream_ptr(dev))
         _lib.check(rc)
     return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
 

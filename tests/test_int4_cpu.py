@@ -64,6 +64,7 @@ def call(name, **change):
     ("sd_w4a16_linear", {"a13": BF16, "a8": A[2] + 512}, 1, "shares memory"),
     ("sd_w4a16_linear", {"a13": BF16, "a1": 1020}, 2, "aligned"),
     ("sd_w4a16_linear", {"a13": BF16, "a3": -512}, 1, "strides"),
+    ("sd_w4a16_linear", {"a13": BF16, "a9": 4095}, 1, "overlap"),
     ("sd_w4a16_linear", {"a13": BF16, "a11": 1 << 30}, 2, "too large"),
 ])
 def test_refusals_say_what_is_wrong(name, change, rc, says):
@@ -136,6 +137,13 @@ def test_ops_refuse_wrong_tensors():
         ops.w4a16_linear(x[:, :32], w, torch.ones((8, 2)))
     with pytest.raises(AssertionError, match="uint8"):
         ops.w4a16_linear(x, w.to(torch.int8), torch.ones((8, 2)))
+
+
+def test_w4a16_out_has_the_result_s_shape(monkeypatch):
+    monkeypatch.setattr(_lib, "require_device", lambda *t: torch.device("cpu"))
+    x, w, s = torch.zeros((4, 64), dtype=torch.bfloat16), torch.zeros((8, 32), dtype=torch.uint8), torch.ones((8, 2))
+    with pytest.raises(AssertionError, match="out must be"):
+        ops.w4a16_linear(x, w, s, out=torch.empty((8, 4), dtype=torch.bfloat16))
 
 
 @pytest.mark.parametrize("n,k,group", [(3, 64, 32), (70, 256, 128), (1, 96, 96)])

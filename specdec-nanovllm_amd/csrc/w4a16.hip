@@ -499,7 +499,7 @@ void w4a16_gemm(Args a) {
       // one tile after another: with all tiles' operands hoisted the accumulators spill
       __builtin_amdgcn_sched_barrier(0);
     }
-    __builtin_amdgcn_s_setprio(0);
+    if constexpr (kTurns) __builtin_amdgcn_s_setprio(0);
     buf = buf + 1 == S ? 0 : buf + 1;
   }
   if (kTurns && !second) meet();
@@ -695,10 +695,10 @@ template <typename T> int launch(const Args& a, int group, hipStream_t st) {
   return launch<T, 1>(a, group, st);
 }
 
-// (a launch takes fewer than 2^32 threads: tiles of 128 x 64 and 256 threads, 16 slices while tiles are few)
+// (a launch takes fewer than 2^32 threads: tiles of 128 x 128 or more and 512 threads, 16 slices while tiles are few)
 bool sizes_ok(int64_t M, int64_t N, int64_t K) {
   return M <= (1ll << 24) && N <= (1ll << 21) && K <= (1ll << 20) &&
-         ((M + 127) / 128) * ((N + 63) / 64) < (1ll << 24);
+         ((M + 127) / 128) * ((N + 127) / 128) < (1ll << 23);
 }
 
 }  // namespace

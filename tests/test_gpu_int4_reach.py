@@ -52,6 +52,17 @@ def test_wide_tiles(n, cols, k, group):
     assert bool((out[:, 0] == 7).all()) and bool((out[:, n + 1:] == 7).all())
 
 
+@pytest.mark.parametrize("m", [1, 7, 20])
+@pytest.mark.parametrize("k", [1 << 15, 1 << 17])
+def test_scales_that_fill_the_lds(m, k):
+    """A row of 1024 groups of 32 leaves room for few waves; of 4096, for none."""
+    g = torch.Generator().manual_seed(k)
+    w = torch.randint(0, 256, (37, k // 2), generator=g, dtype=torch.uint8).to(DEV)
+    s = ((torch.rand((37, k // 32), generator=g) + 0.2) * 0.02).to(torch.bfloat16).to(DEV)
+    x = rand((m, k), 8)
+    check_linear(ops.w4a16_linear(x, w, s), x, w, s)
+
+
 @pytest.mark.parametrize("m", [1, 20, 100])
 def test_weights_past_4_gb(m):
     n, k, group = 1 << 21, 4608, 512

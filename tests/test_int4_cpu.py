@@ -66,6 +66,7 @@ def call(name, **change):
     ("sd_w4a16_linear", {"a13": BF16, "a3": -512}, 1, "strides"),
     ("sd_w4a16_linear", {"a13": BF16, "a9": 4095}, 1, "overlap"),
     ("sd_w4a16_linear", {"a13": BF16, "a11": 1 << 30}, 2, "too large"),
+    ("sd_w4a16_linear", {"a13": BF16, "a10": 1 << 24, "a11": 8128, "a9": 8128}, 2, "too large"),
 ])
 def test_refusals_say_what_is_wrong(name, change, rc, says):
     got, message = call(name, **change)

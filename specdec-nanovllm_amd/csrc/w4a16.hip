@@ -613,9 +613,10 @@ Plan make_plan(int64_t M, int64_t N, int64_t K, int64_t group) {
   }
   pl.XI = 0;
   auto tiles_of = [&](int bn) { return ((M + pl.bm - 1) / pl.bm) * ((N + bn - 1) / bn); };
-  if (M <= 64) {
+  const bool wide = (N + 127) / 128 * 4 >= 2 * cus;
+  if (M <= 32 || (M <= 64 && wide)) {
     pl.bm = M <= 32 ? 32 : 64;
-    pl.bn = (N + 127) / 128 * 4 < 2 * cus ? 64 : 128;
+    pl.bn = wide ? 128 : 64;
     // two workgroups a compute unit, slices of two steps or more
     const int64_t tiles = tiles_of(pl.bn);
     int64_t s = tiles >= cus ? 1 : (2 * cus) / tiles;
@@ -623,24 +624,33 @@ Plan make_plan(int64_t M, int64_t N, int64_t K, int64_t group) {
     pl.slices = s < 1 ? 1 : s > 16 ? 16 : static_cast<int>(s);
     return pl;
   }
-  // One workgroup a compute unit: the columns and slices of the least time, by ns that were measured at
-  // 4096 rows: a step 1380 with 128 columns, 2200 with 256; slices cost a launch and their sums' way to
-  // memory and back. (777 x 19456 x 2560: 128 143 us, 192 114, 256 132; 777 x 2560 x 9728: 104, 81, 71;
-  // 777 x 4096 x 1024: 16, 20, 22.)
-  pl.bm = 128;
+  // Tile and slices of the least time, by the ns that a step was measured to take: with 64 x 64 outputs 570,
+  // 900 for two workgroups of a compute unit together; with 128 rows, one workgroup a compute unit, 1380
+  // for 128 columns to 2200 for 256. Slices cost a launch and their sums' way to memory and back.
+  // (128 x 4096 x 1024: 64 x 64 7.5 us, 128 x 128 13.9; 384 x 2560 x 2560: 15, 29, in 4 slices 23;
+  // 128 x 2560 x 2560: 64 x 64 14.5, in 2 slices 12.3; 777 x 19456 x 2560: 128 columns 143, 192 114, 256
+  // 132; 777 x 2560 x 9728: 104, 81, 71 in 1, 2 and 3 slices.)
   int64_t least = INT64_MAX;
-  for (int bn = 128; bn <= (fold == 1 ? 128 : 256); bn += 64) {
-    const int64_t t = tiles_of(bn), most = t >= cus ? 1 : blocks / 2 < 16 ? blocks / 2 : 16;
-    for (int64_t s = 1; s == 1 || (s <= most && t * s <= cus); ++s) {
-      const int64_t cost = (t * s + cus - 1) / cus * ((blocks + s - 1) / s) * (560 + 32 * bn / 5) +
-                           (s > 1 ? 3000 + s * M * N / 500 : 0);
+  auto consider = [&](int bm, int bn) {
+    const int64_t t = ((M + bm - 1) / bm) * ((N + bn - 1) / bn), slots = bm == 64 ? 2 * cus : cus;
+    const int64_t most = t >= cus ? 1 : blocks / 2 < 16 ? blocks / 2 : 16;
+    for (int64_t s = 1; s == 1 || (s <= most && t * s <= slots); ++s) {
+      const int64_t rounds = t * s / slots, rest = t * s % slots;
+      int64_t step;
+      if (bm == 64) step = rounds * 900 + (rest > cus ? 900 : rest > 0 ? 570 : 0);
+      else step = (rounds + (rest > 0 ? 1 : 0)) * (560 + 32 * bn / 5);
+      const int64_t cost = step * ((blocks + s - 1) / s) + (s > 1 ? 2600 + s * M * N / 500 : 0);
       if (cost < least) {
         least = cost;
+        pl.bm = bm;
         pl.bn = bn;
         pl.slices = static_cast<int>(s);
       }
     }
-  }
+  };
+  consider(64, 64);
+  if (M > 64)
+    for (int bn = 128; bn <= (fold == 1 ? 128 : 256); bn += 64) consider(128, bn);
   return pl;
 }
 

@@ -36,7 +36,7 @@ def check_linear(got, x, w, s, eps=2.0**-7):
     assert (np.abs(f64(got) - want) <= tol).all()
 
 
-@pytest.mark.parametrize("n,cols", [(24500, 192), (32760, 256), (33000, 256)])
+@pytest.mark.parametrize("n,cols", [(16300, 128), (24500, 192), (32760, 256), (33000, 256)])
 @pytest.mark.parametrize("k,group", [(128, 128), (192, 64), (96, 32)])
 def test_wide_tiles(n, cols, k, group):
     """Two row tiles whose second has 2 rows; columns past the last whole tile and, at 33000, past one

@@ -334,7 +334,8 @@ void int4_attn_main(Params p) {
     if constexpr (PAGES == kOnePage) {
       const int blk = min(max(pos.blk[0], 0), p.num_blocks - 1), off = in_page(t0);
       const uint8_t* cp = hc + wide(blk, p.c_sblk) + wide(off, p.c_spos);
-      const uint32_t most = static_cast<uint32_t>(last - t0) * p.c_spos + unit;
+      // (the step's keys, then the product: that of all keys left may pass 32 bits)
+      const uint32_t most = static_cast<uint32_t>(min(last - t0, kStep - 1)) * p.c_spos + unit;
 #pragma unroll
       for (int r = 0; r < 4; ++r) to_lds16(cp, min(row_off[r], most), l + 1024 * r);
       s_at = hs + wide(blk, p.s_sblk) + wide(off, p.s_spos) +
@@ -346,7 +347,7 @@ void int4_attn_main(Params p) {
         const int t = min(t0 + 16 * f, last);
         const int blk = min(max(pos.blk[f], 0), p.num_blocks - 1), off = in_page(t);
         const uint8_t* cp = hc + wide(blk, p.c_sblk) + wide(off, p.c_spos);
-        const uint32_t most = static_cast<uint32_t>(last - t) * p.c_spos + unit;
+        const uint32_t most = static_cast<uint32_t>(min(last - t, kStep / 2 - 1)) * p.c_spos + unit;
 #pragma unroll
         for (int r = 0; r < 2; ++r) to_lds16(cp, min(row_off[r], most), l + 2048 * f + 1024 * r);
         sp[f] = hs + wide(blk, p.s_sblk) + wide(off, p.s_spos) +

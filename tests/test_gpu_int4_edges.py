@@ -1,0 +1,45 @@
+"""The 4-bit operators at the edges of what their entries accept: each call is held to the 64-bit
+oracle with the tolerance of the operator's own tests, or bit for bit to the same call on compact
+tensors."""
+import pytest
+import torch
+
+import test_gpu_int4_attention as ta
+from specdec_nanovllm_amd import ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+SCALE = 128 ** -0.5
+
+
+def position_major(t, stride):
+    """A copy of the cache tensor ``t`` whose positions lie ``stride`` elements apart, all pages of a
+    position side by side."""
+    blocks, page, heads, width = t.shape
+    assert blocks * heads * width <= stride
+    room = torch.empty((page - 1) * stride + blocks * heads * width, dtype=t.dtype, device=t.device)
+    return room.as_strided(t.shape, (heads * width, stride, width, 1)).copy_(t)
+
+
+# (keys left in the sequence) x (bytes between positions) passes 2^32 in each
+@pytest.mark.parametrize("page,keys,stride", [
+    (64, 200, 1 << 25),            # the largest stride there is; one page a step
+    (16, 200, 1 << 25),            # a page for each half of a step
+    (64, 1100, 1 << 22),
+    (64, 1100, 36864 * 128),       # a stride that is no power of two wraps between rows
+    (48, 2100, 1 << 21),
+    (40, 1100, 1 << 22)])          # pages anywhere in a step
+@pytest.mark.parametrize("rows,hq,group", [(1, 8, 64), (2, 16, 128), (7, 8, 32)])
+def test_far_apart_positions(page, keys, stride, rows, hq, group):
+    """One, one and two row tiles of two kv heads (4 rows, 16 and 28 of each)."""
+    c = ta.make([keys, 70], page, hq, 2, group, "bf16", nq=[rows, rows], seed=page)
+    lens = torch.tensor(c["lens"], dtype=torch.int32, device=DEV)
+
+    def attend(codes, scales):
+        return ops.paged_attention_int4(c["q"], codes, scales, c["table"], SCALE, context_lens=lens,
+                                        cu_seqlens_q=ta.cu(c["nq"]), max_seqlen_q=rows)
+
+    compact = attend(c["codes"], c["scales"])
+    ta.check(c, compact, "bf16")
+    far = attend(position_major(c["codes"], stride), position_major(c["scales"], stride >> 4))
+    assert torch.equal(far, compact)

@@ -795,8 +795,9 @@ def w4a16_linear(x: torch.Tensor, qweight: torch.Tensor, scale: torch.Tensor,
     if M:
         lib = _lib.load()
         with _lib.on_device(dev):
-            # the plan (and so the workspace) depends on the device's compute units; none up to 8 rows
-            ws_bytes = lib.sd_w4a16_workspace_size(M, N, K, K // groups) if M > 8 else 0
+            # the plan (and so the workspace) depends on the device's compute units; up to 8 rows there is
+            # none unless a row's scales leave LDS no room, which 512 of them never do (the question takes 1 us)
+            ws_bytes = lib.sd_w4a16_workspace_size(M, N, K, K // groups) if M > 8 or groups > 512 else 0
             ws = _workspace(ws_bytes, dev)
             rc = lib.sd_w4a16_linear(
                 x2.data_ptr(), x0, qw.data_ptr(), K // 2, sc.data_ptr(), _lib.dtype_code(sc.dtype),

@@ -5,7 +5,8 @@ import pytest
 import torch
 
 import test_gpu_int4_attention as ta
-from specdec_nanovllm_amd import ops
+import test_gpu_w4a16 as tw
+from specdec_nanovllm_amd import _lib, ops
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -43,3 +44,16 @@ def test_far_apart_positions(page, keys, stride, rows, hq, group):
     ta.check(c, compact, "bf16")
     far = attend(position_major(c["codes"], stride), position_major(c["scales"], stride >> 4))
     assert torch.equal(far, compact)
+
+
+@pytest.mark.parametrize("m", [1, 7])
+def test_few_rows_with_very_many_scales_take_their_slices(monkeypatch, m):
+    """Rows whose scales leave LDS no room run in K slices, whose workspace the call gives."""
+    given = []
+    make = ops._workspace
+    monkeypatch.setattr(ops, "_workspace", lambda n, dev: given.append(n) or make(n, dev))
+    k = 1 << 17
+    x, w, s, b = tw.make(m, 37, k, 32, "bf16", seed=m)
+    y = ops.w4a16_linear(x, w, s, b)
+    tw.check(y, x, w, s, b, "bf16")
+    assert given == [_lib.load().sd_w4a16_workspace_size(m, 37, k, 32)] and given[0] > 0

@@ -57,3 +57,15 @@ def test_few_rows_with_very_many_scales_take_their_slices(monkeypatch, m):
     y = ops.w4a16_linear(x, w, s, b)
     tw.check(y, x, w, s, b, "bf16")
     assert given == [_lib.load().sd_w4a16_workspace_size(m, 37, k, 32)] and given[0] > 0
+
+
+@pytest.mark.parametrize("m", [1, 3, 20, 70])
+def test_activations_that_start_anywhere(m):
+    x, w, s, b = tw.make(m, 96, 256, 64, "bf16", seed=m)
+    room = torch.empty(x.numel() + 1, dtype=x.dtype, device=DEV)
+    moved = room[1:].view(x.shape).copy_(x)
+    assert moved.is_contiguous() and moved.data_ptr() % 16
+    want = ops.w4a16_linear(x, w, s, b)
+    tw.check(want, x, w, s, b, "bf16")
+    assert torch.equal(ops.w4a16_linear(moved, w, s, b), want)
+    assert torch.equal(ops.w4a16_linear(moved.view(m, 1, 256), w, s, b).view(m, 96), want)

@@ -709,7 +709,8 @@ int sd_paged_attention_int4(const void* q, int64_t q_stride_tok, int64_t q_strid
  * the weight alone would give an infinity (the sums are of code + 16, less 24 sum x).
  * workspace: sd_w4a16_workspace_size bytes on the same device, 16-byte aligned (partial
  * sums of K slices; 0 where one slice runs, as for up to 8 rows in at most 512 groups). Without
- * it (NULL or too small) the call runs in one slice. x_stride_m and w_stride_n <= 2^24, K <= 2^20.
+ * it (NULL or too small) the call runs in one slice. K <= 2^20; x_stride_m and w_stride_n <= 2^24
+ * where there is more than one row to step over.
  */
 size_t sd_w4a16_workspace_size(int64_t M, int64_t N, int64_t K, int32_t group_size);
 int sd_w4a16_linear(const void* x, int64_t x_stride_m, const uint8_t* w, int64_t w_stride_n,

@@ -747,7 +747,7 @@ extern "C" int sd_w4a16_linear(const void* x, int64_t x_stride_m, const uint8_t*
     sd::set_error("%s: dtype must be bf16 or f16, the scales' bf16, f16 or f32", what);
     return SD_ERR_UNSUPPORTED;
   }
-  if (!sizes_ok(M, N, K) || x_stride_m > (1ll << 24) || w_stride_n > (1ll << 24)) {
+  if (!sizes_ok(M, N, K) || (M > 1 && x_stride_m > (1ll << 24)) || (N > 1 && w_stride_n > (1ll << 24))) {
     sd::set_error("%s: M=%lld N=%lld K=%lld (strides %lld, %lld) too large", what, (long long)M, (long long)N,
                   (long long)K, (long long)x_stride_m, (long long)w_stride_n);
     return SD_ERR_UNSUPPORTED;

@@ -777,7 +777,7 @@ def w4a16_linear(x: torch.Tensor, qweight: torch.Tensor, scale: torch.Tensor,
     groups = scale.shape[1]
     assert scale.shape[0] == N and groups and K % groups == 0, "scale must be (N, K // group)"
     x0, x1 = x2.stride()
-    if x1 != 1 or x2.data_ptr() % 16 or (M > 1 and x0 % 8):
+    if x1 != 1 or x2.data_ptr() % 16 or (M > 1 and (x0 % 8 or x0 > 1 << 24)):
         # (not contiguous(): a contiguous view may start anywhere, and stays where it is)
         x2, x0 = x2.clone(memory_format=torch.contiguous_format), K
     qw = qweight if qweight.is_contiguous() else qweight.contiguous()

@@ -69,3 +69,15 @@ def test_activations_that_start_anywhere(m):
     tw.check(want, x, w, s, b, "bf16")
     assert torch.equal(ops.w4a16_linear(moved, w, s, b), want)
     assert torch.equal(ops.w4a16_linear(moved.view(m, 1, 256), w, s, b).view(m, 96), want)
+
+
+@pytest.mark.parametrize("m", [1, 2])
+def test_the_last_token_of_a_long_prompt(m):
+    """Rows further apart than the kernels' strides reach."""
+    hidden = torch.empty((m, 8200, 2560), dtype=torch.bfloat16, device=DEV)
+    x, w, s, b = tw.make(m, 100, 2560, 128, "bf16", seed=9)
+    hidden[:, -1] = x
+    last = hidden[:, -1]
+    assert last.stride(0) > 1 << 24
+    y = ops.w4a16_linear(last, w, s, b)
+    tw.check(y, x, w, s, b, "bf16")

@@ -1,5 +1,6 @@
 """What the 4-bit entries accept at the edges of their ranges, as far as the host decides it."""
 import pytest
+import torch
 
 from specdec_nanovllm_amd import _lib
 
@@ -14,3 +15,17 @@ def test_few_rows_need_a_workspace_only_past_512_groups(m, n):
             if group * groups <= 1 << 20:
                 assert f(m, n, group * groups, group) == 0
     assert f(m, 37, 1 << 17, 32) > 0
+
+
+@pytest.mark.skipif(torch.cuda.device_count() > 0, reason="fake device addresses: only where no GPU can be reached")
+@pytest.mark.parametrize("m,n,x_stride,w_stride,says", [
+    (1, 64, 1 << 40, 512, "shares memory"),   # as far as the call gets: the stride is that of no second row
+    (1, 1, 1 << 25, 1 << 40, "shares memory"),
+    (2, 64, (1 << 24) + 8, 512, "too large"),
+    (1, 2, 1024, (1 << 24) + 16, "too large"),
+    (2, 64, 1 << 24, 1 << 24, "shares memory")])
+def test_row_strides_count_where_there_are_rows(m, n, x_stride, w_stride, says):
+    lib, at = _lib.load(), 0x10000000
+    rc = lib.sd_w4a16_linear(at, x_stride, at << 4, w_stride, at << 3, _lib.SD_BF16, 128, None, at + 16, 4096, m, n,
+                             1024, _lib.SD_BF16, None, 0, None)
+    assert rc != 0 and says in lib.sd_last_error().decode()

@@ -34,7 +34,9 @@ def store_kvcache(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor,
 def _aligned(t: torch.Tensor) -> torch.Tensor:
     """``t`` with 16-byte aligned rows (views of a projection's output are)."""
     s = t.stride()
-    return t if s[2] == 1 and not (s[0] % 8 or s[1] % 8 or t.data_ptr() % 16) else t.contiguous()
+    if s[2] == 1 and not (s[0] % 8 or s[1] % 8 or t.data_ptr() % 16):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)  # a contiguous tensor may start anywhere
 
 
 def _pages_in_16_bits(kv_codes: torch.Tensor, kv_scales: torch.Tensor, block_tables: torch.Tensor):

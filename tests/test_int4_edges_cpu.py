@@ -29,3 +29,16 @@ def test_row_strides_count_where_there_are_rows(m, n, x_stride, w_stride, says):
     rc = lib.sd_w4a16_linear(at, x_stride, at << 4, w_stride, at << 3, _lib.SD_BF16, 128, None, at + 16, 4096, m, n,
                              1024, _lib.SD_BF16, None, 0, None)
     assert rc != 0 and says in lib.sd_last_error().decode()
+
+
+def test_the_attention_layer_aligns_rows_that_start_anywhere():
+    from specdec_nanovllm_amd.layers.attention import _aligned
+
+    for t in (torch.empty(3 * 4 * 128 + 1, dtype=torch.bfloat16)[1:].view(3, 4, 128),
+              torch.empty((3, 4, 129), dtype=torch.bfloat16)[..., :128],
+              torch.empty((3, 128, 4), dtype=torch.bfloat16).transpose(1, 2)):
+        t.copy_(torch.arange(t.numel()).view(t.shape) % 251)
+        a = _aligned(t)
+        assert a.data_ptr() % 16 == 0 and a.is_contiguous() and torch.equal(a, t)
+    t = torch.empty((3, 4, 256), dtype=torch.bfloat16)[..., 128:]
+    assert _aligned(t) is t  # a view of aligned rows stays one

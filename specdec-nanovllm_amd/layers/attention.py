@@ -39,10 +39,15 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
     return t.clone(memory_format=torch.contiguous_format)  # a contiguous tensor may start anywhere
 
 
-def _pages_in_16_bits(kv_codes: torch.Tensor, kv_scales: torch.Tensor, block_tables: torch.Tensor):
+def _pages_in_16_bits(kv_codes: torch.Tensor, kv_scales: torch.Tensor, block_tables: torch.Tensor,
+                      max_keys: int = 0):
     """The pages of a block table read back from a 4-bit cache: paged K and V of their own, and
-    the table over them (entry (b, i) is page b * width + i; unused entries are zero pages)."""
+    the table over them (entry (b, i) is page b * width + i; unused entries are zero pages).
+    max_keys: the longest sequence's keys, past which a table (as wide as the longest sequence
+    there may be, say) is not read; 0: all of it."""
     page, heads = kv_codes.shape[1], kv_codes.shape[2]
+    if max_keys > 0:
+        block_tables = block_tables[:, :-(-max_keys // page)]
     B, width = block_tables.shape
     rows = torch.arange(page, dtype=torch.int32, device=block_tables.device)
     slots = torch.where(block_tables[..., None] >= 0, block_tables[..., None] * page + rows, -1)
@@ -118,6 +123,6 @@ class Attention(nn.Module):
                 return ops.paged_attention_int4(q, codes, scales, tables, self.scale,
                                                 cu_seqlens_k=context.cu_seqlens_k,
                                                 cu_seqlens_q=context.cu_seqlens_q, max_seqlen_q=n)
-            k, v, tables = _pages_in_16_bits(codes, scales, tables)
+            k, v, tables = _pages_in_16_bits(codes, scales, tables, int(context.max_seqlen_k))
         return ops.prefill_attention(q, k, v, context.cu_seqlens_q, context.cu_seqlens_k, n,
                                      self.scale, block_table=tables)

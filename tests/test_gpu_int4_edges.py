@@ -81,3 +81,27 @@ def test_the_last_token_of_a_long_prompt(m):
     assert last.stride(0) > 1 << 24
     y = ops.w4a16_linear(last, w, s, b)
     tw.check(y, x, w, s, b, "bf16")
+
+
+def test_a_cached_prefix_under_a_table_of_the_longest_sequence():
+    from specdec_nanovllm_amd.layers.attention import Attention
+    from specdec_nanovllm_amd.utils.context import reset_context, set_context
+
+    heads, page, new, keys = 8, 64, [40, 90], [168, 154]
+    c = ta.make(keys, page, 16, heads, 64, "bf16", seed=11)
+    layer = Attention(16, 128, SCALE, heads)
+    layer.k_cache, layer.v_cache = c["codes"], c["scales"]
+    wide = torch.full((2, 140_000), -1, dtype=torch.int32, device=DEV)  # 9 M positions a sequence
+    wide[:, :c["table"].shape[1]] = c["table"]
+    g = torch.Generator().manual_seed(12)
+    q, k, v = (torch.randn((sum(new), h, 128), generator=g).to(torch.bfloat16).to(DEV) for h in (16, heads, heads))
+    out = []
+    for table in (c["table"], wide):
+        slots = torch.cat([table[b, p // page] * page + p % page for b in (0, 1)
+                           for p in [torch.arange(keys[b] - new[b], keys[b], device=DEV)]]).to(torch.int32)
+        try:
+            set_context(True, ta.cu(new), ta.cu(keys), max(new), max(keys), slots, None, table)
+            out.append(layer(q, k, v))
+        finally:
+            reset_context()
+    assert torch.equal(*out) and bool(out[0].isfinite().all())

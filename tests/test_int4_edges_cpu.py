@@ -42,3 +42,41 @@ def test_the_attention_layer_aligns_rows_that_start_anywhere():
         assert a.data_ptr() % 16 == 0 and a.is_contiguous() and torch.equal(a, t)
     t = torch.empty((3, 4, 256), dtype=torch.bfloat16)[..., 128:]
     assert _aligned(t) is t  # a view of aligned rows stays one
+
+
+def test_a_cached_prefix_is_read_back_as_far_as_there_are_keys(monkeypatch):
+    """A table as wide as the longest sequence that may come is not read to its end."""
+    from specdec_nanovllm_amd import ops
+    from specdec_nanovllm_amd.layers.attention import Attention
+    from specdec_nanovllm_amd.utils.context import reset_context, set_context
+
+    page, heads, asked = 16, 2, {}
+
+    def load(codes, scales, slots):
+        asked["slots"] = slots
+        return torch.zeros((slots.numel(), heads, 128)), torch.zeros((slots.numel(), heads, 128))
+
+    def prefill(q, k, v, cu_q, cu_k, n, scale, block_table):
+        asked["k"], asked["table"] = k, block_table
+        return q
+
+    monkeypatch.setattr(ops, "load_kvcache_int4", load)
+    monkeypatch.setattr(ops, "prefill_attention", prefill)
+    monkeypatch.setattr(ops, "store_kvcache_int4", lambda *a: None)
+    layer = Attention(4, 128, 0.1, heads)
+    layer.k_cache, layer.v_cache = ops.int4_kvcache(9, page, heads, device="cpu")
+    table = torch.full((2, 1000), -1, dtype=torch.int32)
+    table[0, :3], table[1, :2] = torch.tensor([7, 1, 4], dtype=torch.int32), torch.tensor([0, 8], dtype=torch.int32)
+    cu_q, cu_k = torch.tensor([0, 20, 40]), torch.tensor([0, 41, 41 + 24])
+    q, k = torch.zeros((40, 4, 128)), torch.zeros((40, heads, 128))
+    try:
+        set_context(True, cu_q, cu_k, 20, 41, torch.zeros(40, dtype=torch.int32), None, table)
+        layer(q, k, k)
+    finally:
+        reset_context()
+    rows = torch.arange(page)
+    want = torch.stack([torch.cat([b * page + rows if b >= 0 else torch.full((page,), -1) for b in seq])
+                        for seq in ([7, 1, 4], [0, 8, -1])])
+    assert torch.equal(asked["slots"].reshape(2, -1).long(), want)
+    assert asked["k"].shape == (6, page, heads, 128)
+    assert torch.equal(asked["table"], torch.arange(6, dtype=torch.int32).view(2, 3))

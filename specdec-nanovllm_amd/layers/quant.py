@@ -213,7 +213,7 @@ def apply_int4_quant(model: nn.Module, module_names, group_size: int = 128):
     ``int4_linear``. Same report (without the scale statistics), errors and all-or-nothing checks."""
     chosen = _chosen_modules(model, module_names)
     for name, mod in chosen:
-        if mod.weight.shape[1] % group_size or group_size % 32:
+        if group_size <= 0 or mod.weight.shape[1] % group_size or group_size % 32:
             raise ValueError(f"{name}: groups must be a multiple of 32 columns and divide "
                              f"{mod.weight.shape[1]}, got {group_size}")
     return [_swap_to_int4(name, mod, group_size) for name, mod in chosen]

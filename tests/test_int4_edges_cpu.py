@@ -80,3 +80,15 @@ def test_a_cached_prefix_is_read_back_as_far_as_there_are_keys(monkeypatch):
     assert torch.equal(asked["slots"].reshape(2, -1).long(), want)
     assert asked["k"].shape == (6, page, heads, 128)
     assert torch.equal(asked["table"], torch.arange(6, dtype=torch.int32).view(2, 3))
+
+
+@pytest.mark.parametrize("group", [0, -32])
+def test_apply_int4_quant_refuses_groups_of_no_columns(group):
+    from specdec_nanovllm_amd.layers.linear import ReplicatedLinear
+    from specdec_nanovllm_amd.layers.quant import apply_int4_quant
+
+    m = torch.nn.ModuleDict(dict(a=ReplicatedLinear(64, 8)))
+    m["a"].weight.data = torch.zeros((8, 64), dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="multiple of 32"):
+        apply_int4_quant(m, ["a"], group)
+    assert m["a"].weight.dtype == torch.bfloat16

@@ -713,6 +713,13 @@ int sd_paged_attention_int4(const void* q, int64_t q_stride_tok, int64_t q_strid
  * where there is more than one row to step over.
  */
 size_t sd_w4a16_workspace_size(int64_t M, int64_t N, int64_t K, int32_t group_size);
+/*
+ * The route of sd_w4a16_linear for this shape on the current device (host only):
+ *   K slices | tile columns << 8 | tile rows << 20
+ * of the tiled kernel; waves | weight rows of a tile << 8 of the kernel for few rows; 0 for
+ * sizes that sd_w4a16_linear refuses.
+ */
+int64_t sd_w4a16_plan(int64_t M, int64_t N, int64_t K, int32_t group_size);
 int sd_w4a16_linear(const void* x, int64_t x_stride_m, const uint8_t* w, int64_t w_stride_n,
                     const void* scale, int32_t scale_dtype, int32_t group_size, const void* bias,
                     void* y, int64_t y_stride_m, int64_t M, int64_t N, int64_t K, int32_t dtype,

@@ -165,6 +165,7 @@ SIGNATURES.update({
         _f32, _i32, _p, _i64, _i64,      # scale, dtype, out, strides
         _p, _sz, _i32, _p]),             # workspace, bytes, num_splits, stream
     "sd_w4a16_workspace_size": (_sz, [_i64, _i64, _i64, _i32]),
+    "sd_w4a16_plan": (_i64, [_i64, _i64, _i64, _i32]),
     "sd_w4a16_linear": (ctypes.c_int, [
         _p, _i64, _p, _i64,              # x, x_stride, w, w_stride
         _p, _i32, _i32, _p,              # scale, scale_dtype, group_size, bias

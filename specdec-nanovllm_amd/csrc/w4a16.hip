@@ -725,6 +725,14 @@ extern "C" size_t sd_w4a16_workspace_size(int64_t M, int64_t N, int64_t K, int32
   return pl.slices > 1 ? static_cast<size_t>(pl.slices) * M * N * sizeof(float) : 0;
 }
 
+extern "C" int64_t sd_w4a16_plan(int64_t M, int64_t N, int64_t K, int32_t group_size) {
+  if (M <= 0 || N <= 0 || K <= 0 || group_size <= 0 || group_size % 32 != 0 || K % group_size != 0 || !sizes_ok(M, N, K))
+    return 0;
+  const Plan pl = make_plan(M, N, K, group_size);
+  if (pl.XI) return pl.W | 16 * pl.NT << 8;
+  return pl.slices | pl.bn << 8 | static_cast<int64_t>(pl.bm) << 20;
+}
+
 extern "C" int sd_w4a16_linear(const void* x, int64_t x_stride_m, const uint8_t* w, int64_t w_stride_n,
                                const void* scale, int32_t scale_dtype, int32_t group_size,
                                const void* bias, void* y, int64_t y_stride_m, int64_t M, int64_t N,

@@ -92,3 +92,18 @@ def test_apply_int4_quant_refuses_groups_of_no_columns(group):
     with pytest.raises(ValueError, match="multiple of 32"):
         apply_int4_quant(m, ["a"], group)
     assert m["a"].weight.dtype == torch.bfloat16
+
+
+def test_w4a16_plans_agree_with_their_workspaces():
+    lib = _lib.load()
+    for m in (1, 3, 9, 17, 40, 66, 130, 777, 5000):
+        for n, k, group in ((1, 32, 32), (2570, 9728, 64), (4100, 1312, 32), (19456, 2560, 128), (1 << 21, 128, 128)):
+            plan, need = lib.sd_w4a16_plan(m, n, k, group), lib.sd_w4a16_workspace_size(m, n, k, group)
+            rows, columns, parts = plan >> 20, plan >> 8 & 0xfff, plan & 0xff
+            if rows:
+                assert (rows, columns) in ((32, 64), (32, 128), (64, 64), (64, 128), (128, 128), (128, 192), (128, 256))
+                assert 1 <= parts <= 16 and need == (parts * m * n * 4 if parts > 1 else 0)
+            else:
+                assert m <= 32 and columns in (16, 32) and 1 <= parts <= 16 and need == 0
+    for bad in ((0, 64, 64, 32), (4, 64, 64, 48), (4, 64, 96, 64), (4, 1 << 30, 64, 64), (4, 64, 1 << 21, 64)):
+        assert lib.sd_w4a16_plan(*bad) == 0

@@ -34,7 +34,9 @@ the sampler's argmax; the embedding lookup stays a torch index.
 ``weight_bits=4`` holds every linear in 4 bits (groups of 128 columns), ``kv_bits=4``
 the KV cache in 4 bits (groups of 64 dims); either takes the step of
 ``_step_4bit``: the library's RMSNorm, linear, append (q/k norm + RoPE + quantize +
-slot write in one launch), attention and SiLU*mul, one launch each.
+slot write in one launch), attention and SiLU*mul, one launch each. ``fused`` changes
+nothing there: the linears have no 4-bit form with a norm or SiLU*mul in it, and the
+8-bit ones with a 4-bit cache run without.
 
 ``chain()`` runs ``k`` steps back to back, each feeding its tokens to the next,
 on static buffers, so the whole chain can be captured in one HIP graph.

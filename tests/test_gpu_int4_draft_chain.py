@@ -45,3 +45,10 @@ def test_logits_match_the_float32_reference(monkeypatch, weight_bits, kv_bits, b
         allowed = (span / 30 + 2**-7 * (span + own.abs()) if kv_bits == 4 else 0) + 2e-2 * most
         assert bool(((got - own).abs() <= allowed).all()), f"step {s}: off by {(got - own).abs().max().item():.4g}"
         assert torch.equal(ch.tokens[s + 1], logits.argmax(-1))
+
+
+@pytest.mark.parametrize("weight_bits,kv_bits", [(4, 4), (8, 4), (4, 16)])
+def test_fused_changes_nothing_in_4_bits(weight_bits, kv_bits):
+    a, b = (DraftChain(2, weight_bits=weight_bits, kv_bits=kv_bits, context="randn", fused=fused, **td.SMALL)
+            for fused in (False, True))
+    assert torch.equal(a.step(0), b.step(0)) and torch.equal(a.tokens, b.tokens)

@@ -45,7 +45,7 @@ def sources() -> list[str]:
 COMMON_FLAGS = [
     f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC",
     "-I", INCLUDE, "-I", CSRC,
-    # Packed FP32 instructions stay off on this hardware pool (hipcc only).
+    # Packed FP32 instructions stay off: some of their forms have given wrong results (hipcc only).
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     "-Wall", "-Wno-unused-command-line-argument",
 ]

@@ -13,12 +13,13 @@
 // Up to 32 rows (w4a16_rows): bound by the weights' bytes, N K / 2. A workgroup takes tiles of 16 weight
 // rows, its waves the columns in turn; their sums meet in LDS and are added in wave order.
 // Activations read by every wave from the caches instead of from LDS kept the address units busy: 75 us
-// at 1 x 151936 x 1024 against 22 (78 MB of weights: 3.5 TB/s).
+// at 1 x 151936 x 1024 against 23 (78 MB of weights: 3.4 TB/s).
 // Above (w4a16_gemm): activations, weights and scales go straight to LDS for the workgroup's waves
 // (global_load_lds, steps of 128 columns, two or three ahead); K is split over workgroups where the tiles
 // alone leave compute units idle, and w4a16_reduce adds the slices in order. Bound by instruction issue:
 // a step of 128 x 256 outputs takes 2.0 us, of which its MFMAs, a fifth of them for the -24 sum x, are 1.1
-// (4096 x 19456 x 2560: 449 us, 910 TFLOP/s; 777 rows 114 us).
+// (4096 x 19456 x 2560: 445 to 468 us from card to card, 872 to 916 TFLOP/s; 777 rows, in tiles of 192
+// columns, 112 to 118 us).
 #include <type_traits>
 
 #include "int4.h"
@@ -604,7 +605,7 @@ Plan make_plan(int64_t M, int64_t N, int64_t K, int64_t group) {
     if (pl.XI < 16 && groups < cus)
       while (pl.W < 12 && pl.W < stages && bytes(1, pl.W + 1) <= kMost) ++pl.W;
     // groups a workgroup: one up to four workgroups a compute unit (1 x 19456 x 2560, 608 groups: 8.8 us,
-    // 12.0 with two), then their share (1 x 151936 x 1024, 4748 groups: 23.8 us with four, 25.6 with one)
+    // 12.0 with two), then their share (1 x 151936 x 1024, 4748 groups: 22.8 us with four, 26.9 with one)
     pl.tiles = static_cast<int>(groups / (4 * cus));
     if (pl.tiles < 1) pl.tiles = 1;
     while (pl.tiles > 1 && bytes(pl.tiles, pl.W) > bytes(1, pl.W) + (8 << 10)) --pl.tiles;

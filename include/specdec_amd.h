@@ -725,6 +725,82 @@ int sd_w4a16_linear(const void* x, int64_t x_stride_m, const uint8_t* w, int64_t
                     void* y, int64_t y_stride_m, int64_t M, int64_t N, int64_t K, int32_t dtype,
                     void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Linears in 8-bit integers (no counterpart in the reference, whose int8 weights
+ * meet 16-bit activations). A row of activations is held as codes -127 .. 127 and
+ * one fp32 scale:
+ *   scale = max |v| / 127,  code = round_half_even(127 v / max |v|),  value = code * scale
+ * A row with a NaN or an infinity in v has scale NaN and codes 0 (a linear's outputs
+ * of that row are NaN); a row of zeros has scale 0. Rows of codes and of 16-bit
+ * tensors are 16-byte aligned; columns are a multiple of 16.
+ * ------------------------------------------------------------------------- */
+
+/*
+ * codes (rows, columns) and scale (rows,) of the rows of x (rows, columns) dtype
+ * bf16/f16. columns <= 32768, rows < 2^24 (2^22 past 8192 columns).
+ */
+int sd_quantize_rows_int8(const void* x, int64_t x_stride, int8_t* codes, int64_t codes_stride,
+                          float* scale, int64_t rows, int32_t columns, int32_t dtype,
+                          void* stream);
+
+/*
+ * RMSNorm whose result is quantized unrounded: s = x (+ residual) in fp32,
+ *   v = s * rsqrt(mean(s^2) + eps) * weight,  residual_out = dtype(s)
+ * residual and residual_out may both be NULL; residual_out may be x or residual.
+ * Limits as sd_quantize_rows_int8. A row whose squares' sum leaves fp32 gives
+ * zeros, as in sd_rmsnorm.
+ */
+int sd_rmsnorm_int8(const void* x, int64_t x_stride, const void* residual,
+                    int64_t residual_stride, const void* weight, int8_t* codes,
+                    int64_t codes_stride, float* scale, void* residual_out,
+                    int64_t residual_out_stride, int64_t rows, int32_t hidden, float eps,
+                    int32_t dtype, void* stream);
+
+/*
+ * The rows read back: out (rows, columns) = code * scale, rounded to dtype
+ * (bf16/f16/f32). rows * ceil(columns / 2048) < 2^26.
+ */
+int sd_dequantize_rows_int8(const int8_t* codes, int64_t codes_stride, const float* scale,
+                            void* out, int64_t out_stride, int64_t rows, int32_t columns,
+                            int32_t dtype, void* stream);
+
+/*
+ * W8A8 linear: y[m, n] = (sum_k x[m, k] w[n, k]) * scale[n] * x_scale[m] (+ bias[n]).
+ *   x       : (M, K) codes, row stride x_stride_m;  x_scale : (M,) fp32
+ *   w       : (N, K) int8, row stride w_stride_n (the W8A16 linear's per-channel weights)
+ *   scale   : (N,) scale_dtype bf16/f16/f32;  bias : (N,) dtype or NULL
+ *   y       : (M, N) dtype (bf16/f16), row stride y_stride_m (>= N), sharing no byte with
+ *             x, x_scale or w
+ * K is a multiple of 16 below 2^17: the integer sums are exact (any codes, -128 too).
+ * Three fp32 products and one rounding follow; a row's outputs are the same bits
+ * whatever M. x_stride_m and w_stride_n <= 2^23 where there is more than one row.
+ * workspace: sd_w8a8_workspace_size bytes on the same device, 16-byte aligned (sums of
+ * K slices; 0 where one slice runs). Without it (NULL or too small) the call runs in
+ * one slice. `gated`: the query is for sd_w8a8_gate_up_silu.
+ */
+size_t sd_w8a8_workspace_size(int64_t M, int64_t N, int64_t K, int32_t gated);
+/*
+ * The route of a shape on the current device (host only):
+ *   K slices | weight rows of a tile << 8 | activation rows of a tile << 20
+ * of the tiled kernel; waves | weight rows of a tile << 8 of the kernel for few rows; 0
+ * for sizes that the linear refuses.
+ */
+int64_t sd_w8a8_plan(int64_t M, int64_t N, int64_t K, int32_t gated);
+int sd_w8a8_linear(const int8_t* x, int64_t x_stride_m, const float* x_scale, const int8_t* w,
+                   int64_t w_stride_n, const void* scale, int32_t scale_dtype, const void* bias,
+                   void* y, int64_t y_stride_m, int64_t M, int64_t N, int64_t K, int32_t dtype,
+                   void* workspace, size_t workspace_bytes, void* stream);
+/*
+ * The gated projections of an MLP: w (2 N, K) = [gate; up], scale and bias (2 N,),
+ *   y[m, n] = silu(g[m, n]) * u[m, n]
+ * with g and u the linear's outputs before their rounding; otherwise as sd_w8a8_linear.
+ */
+int sd_w8a8_gate_up_silu(const int8_t* x, int64_t x_stride_m, const float* x_scale,
+                         const int8_t* w, int64_t w_stride_n, const void* scale,
+                         int32_t scale_dtype, const void* bias, void* y, int64_t y_stride_m,
+                         int64_t M, int64_t N, int64_t K, int32_t dtype, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

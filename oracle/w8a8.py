@@ -1,0 +1,51 @@
+"""Oracle of the 8-bit activations and the integer linears (numpy).
+
+16-bit inputs arrive as float32 arrays of their exact values. The codes follow from fp32 v and max |v| by one exact
+quotient, so they are compared for equality; scales and outputs in 64 bits, the linear's also by its own three fp32
+products."""
+from __future__ import annotations
+
+import numpy as np
+
+
+def codes(v):
+    """v (rows, K) float32 -> (int64 codes, max |v| float64 (rows,)); rows with a NaN or an infinity: codes 0, NaN."""
+    v = np.asarray(v, dtype=np.float32).astype(np.float64)
+    most = np.abs(v).max(-1)
+    fine = np.isfinite(most)
+    safe = np.where(fine & (most > 0), most, 1.0)
+    # a quotient of two 24-bit numbers is a tie or at least 2^-26 from one: rounding it to 53 bits moves none
+    c = np.rint(127 * np.where(fine[:, None], v, 0) / safe[:, None]).astype(np.int64)
+    return np.where((fine & (most > 0))[:, None], c, 0), np.where(fine, most, np.nan)
+
+
+def norm_products(x, w, residual=None):
+    """s = x (+ residual) and s w, each rounded to fp32 as the operator does."""
+    with np.errstate(over="ignore", invalid="ignore"):
+        s = x.astype(np.float32) if residual is None else x.astype(np.float32) + residual.astype(np.float32)
+        return s, s * w.astype(np.float32)
+
+
+def norm_scale(most, s, eps):
+    """max |v| / 127 times 1 / sqrt(mean(s^2) + eps), 64 bits."""
+    s = s.astype(np.float64)
+    return most / 127 / np.sqrt((s * s).mean(-1) + eps)
+
+
+def linear32(x, x_scale, w, scale, bias=None):
+    """The operator's own arithmetic: exact integer sums, then fp32 products in its order. float32, unrounded."""
+    sums = x.astype(np.int64) @ w.astype(np.int64).T
+    y = sums.astype(np.float32) * scale.astype(np.float32)[None] * x_scale.astype(np.float32)[:, None]
+    return y if bias is None else y + bias.astype(np.float32)[None]
+
+
+def linear64(x, x_scale, w, scale, bias=None):
+    sums = (x.astype(np.int64) @ w.astype(np.int64).T).astype(np.float64)
+    y = sums * scale.astype(np.float64)[None] * x_scale.astype(np.float64)[:, None]
+    return y if bias is None else y + bias.astype(np.float64)[None]
+
+
+def silu_up(y):
+    """silu(gate) * up of y = [gate | up] (64 bits)."""
+    gate, up = np.split(y, 2, axis=-1)
+    return gate / (1 + np.exp(-gate)) * up

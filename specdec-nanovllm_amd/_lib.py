@@ -173,6 +173,28 @@ SIGNATURES.update({
         _i32, _p, _sz, _p]),             # dtype, workspace, bytes, stream
 })
 
+_w8a8 = [
+    _p, _i64, _p, _p, _i64,              # x, x_stride, x_scale, w, w_stride
+    _p, _i32, _p,                        # scale, scale_dtype, bias
+    _p, _i64, _i64, _i64, _i64,          # y, y_stride, M, N, K
+    _i32, _p, _sz, _p]                   # dtype, workspace, bytes, stream
+SIGNATURES.update({
+    "sd_quantize_rows_int8": (ctypes.c_int, [
+        _p, _i64, _p, _i64, _p,          # x, stride, codes, stride, scale
+        _i64, _i32, _i32, _p]),          # rows, columns, dtype, stream
+    "sd_rmsnorm_int8": (ctypes.c_int, [
+        _p, _i64, _p, _i64, _p,          # x, stride, residual, stride, weight
+        _p, _i64, _p, _p, _i64,          # codes, stride, scale, residual_out, stride
+        _i64, _i32, _f32, _i32, _p]),    # rows, hidden, eps, dtype, stream
+    "sd_dequantize_rows_int8": (ctypes.c_int, [
+        _p, _i64, _p, _p, _i64,          # codes, stride, scale, out, stride
+        _i64, _i32, _i32, _p]),          # rows, columns, dtype, stream
+    "sd_w8a8_workspace_size": (_sz, [_i64, _i64, _i64, _i32]),
+    "sd_w8a8_plan": (_i64, [_i64, _i64, _i64, _i32]),
+    "sd_w8a8_linear": (ctypes.c_int, _w8a8),
+    "sd_w8a8_gate_up_silu": (ctypes.c_int, _w8a8),
+})
+
 _lib = None
 
 

@@ -1,0 +1,339 @@
+// act_int8.hip — activations in 8 bits with a scale per row, for gfx950: what the linears of w8a8.hip read.
+//
+//   v = x                                    (quantize)
+//   v = s w, s = x + residual in fp32        (RMSNorm; residual_out = s rounded once)
+//   code = round_half_even(127 v / max |v|), scale = max |v| / 127 (times 1 / sqrt(mean(s^2) + eps))
+//   value = code scale
+//
+// The root mean square cancels out of the codes: the sum of squares and max |v| are one reduction, between
+// which and the codes the row stays in registers. A code is that of the exact quotient of the fp32 v and max |v|;
+// the normalised value itself is never rounded. A row with a NaN or an infinity in v has scale NaN and codes 0,
+// a row of zeros scale 0.
+// Bound by memory: 7 bytes an element with a residual, 3 without either.
+#include <math.h>
+
+#include "sd_common.h"
+
+namespace {
+
+using sd::u32x4;
+
+struct Params {
+  const uint16_t* x;
+  int64_t xs;
+  const uint16_t* res;  // NULL: no residual
+  int64_t rs;
+  const uint16_t* w;
+  int8_t* codes;
+  int64_t cs;
+  float* scale;
+  uint16_t* res_out;
+  int64_t ros;
+  int64_t rows;
+  int32_t K;
+  float eps;
+};
+
+__device__ __forceinline__ uint32_t max_u32(uint32_t a, uint32_t b) { return a > b ? a : b; }
+template <int CTRL> __device__ __forceinline__ uint32_t dpp_max(uint32_t v) {
+  return max_u32(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, 0xF, 0xF, false)));
+}
+// Maximum over the wave, by the moves of sd::xor_sum_down<32>.
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+  const auto a = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  v = max_u32(a[0], a[1]);
+  const auto b = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = max_u32(b[0], b[1]);
+  v = dpp_max<0x128>(v);  // row_ror:8
+  v = dpp_max<0x124>(v);  // row_ror:4
+  v = dpp_max<0x4E>(v);   // quad_perm [2, 3, 0, 1]
+  return dpp_max<0xB1>(v);  // quad_perm [1, 0, 3, 2]
+}
+
+__device__ __forceinline__ float element(const u32x4& v, int i, float (*to)(uint16_t)) {
+  return to(static_cast<uint16_t>(v[i / 2] >> (16 * (i & 1))));
+}
+
+// The codes of 8 values. v inv is off by 2^-16 at most (two roundings of up to 127), so that only a quotient
+// that near to a border needs 127 v - r most, which two exact products give.
+__device__ __forceinline__ uint2 codes8(const float (&v)[8], float most, float inv) {
+#pragma clang fp contract(off)
+  float r[8], near = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float q = v[i] * inv;
+    r[i] = rintf(q);
+    near = fmaxf(near, fabsf(q - r[i]));
+  }
+  if (near > 0.5f - 0x1p-14f) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float p = r[i] * most, p_low = fmaf(r[i], most, -p);
+      const float u = 127.f * v[i], u_low = fmaf(127.f, v[i], -u);
+      const float d = (u - p) + (u_low - p_low), half = 0.5f * most;
+      const bool odd = static_cast<int>(r[i]) & 1;
+      if (d > half || (d == half && odd)) r[i] += 1.f;
+      else if (d < -half || (d == -half && odd)) r[i] -= 1.f;
+    }
+  }
+  uint32_t b[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) b[i / 4] |= (static_cast<uint32_t>(static_cast<int>(r[i])) & 0xffu) << (8 * (i % 4));
+  return uint2{b[0], b[1]};
+}
+
+// TPR threads a row (64: four rows a workgroup, no barrier); thread t holds the 8-element chunks t, t + TPR, ...
+template <typename T, bool NORM, bool RES, int TPR, int C>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rows_int8_kernel(Params p) {
+#pragma clang fp contract(off)
+  constexpr int kRows = TPR < 256 ? 256 / TPR : 1;
+  __shared__ float red_sum[TPR / 64];
+  __shared__ uint32_t red_max[TPR / 64];
+  const int t = static_cast<int>(threadIdx.x) % TPR;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows +
+                      __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / TPR);
+  if (kRows > 1 && row >= p.rows) return;
+  const uint16_t* x = p.x + row * p.xs;
+  const uint16_t* res = RES ? p.res + row * p.rs : nullptr;
+  u32x4 xb[C], rb[C], wb[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    if (c * TPR * 8 >= p.K) break;  // uniform
+    const int e = min((c * TPR + t) * 8, p.K - 8);
+    xb[c] = sd::load16(x + e);
+    if constexpr (RES) rb[c] = sd::load16(res + e);
+    if constexpr (NORM) wb[c] = sd::load16(p.w + e);
+  }
+  float v[C][8], sum = 0.f;
+  uint32_t most_bits = 0;
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    if (c * TPR * 8 >= p.K) break;  // uniform
+    const int e = (c * TPR + t) * 8;
+    const bool in = e < p.K;
+    float s[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      s[i] = element(xb[c], i, sd::from_bits<T>);
+      if constexpr (RES) s[i] = s[i] + element(rb[c], i, sd::from_bits<T>);
+      if (!in) s[i] = 0.f;
+      v[c][i] = s[i];
+      if constexpr (NORM) {
+        sum += s[i] * s[i];
+        v[c][i] = in ? s[i] * element(wb[c], i, sd::from_bits<T>) : 0.f;
+      }
+      most_bits = max_u32(most_bits, __float_as_uint(v[c][i]) & 0x7fffffffu);  // NaN above infinity above all else
+    }
+    if (RES && in)
+      sd::store16(p.res_out + row * p.ros + e, u32x4{sd::pack2<T>(s[0], s[1]), sd::pack2<T>(s[2], s[3]),
+                                                     sd::pack2<T>(s[4], s[5]), sd::pack2<T>(s[6], s[7])});
+  }
+  if constexpr (NORM) sum = sd::xor_sum_down<32>(sum);
+  most_bits = wave_max(most_bits);
+  if constexpr (TPR > 64) {
+    const int wave = t >> 6;
+    if ((t & 63) == 0) {
+      red_sum[wave] = sum;
+      red_max[wave] = most_bits;
+    }
+    __syncthreads();
+    sum = 0.f;
+    most_bits = 0;
+#pragma unroll
+    for (int i = 0; i < TPR / 64; ++i) {
+      sum += red_sum[i];
+      most_bits = max_u32(most_bits, red_max[i]);
+    }
+  }
+  const bool none = most_bits >= 0x7f800000u || most_bits == 0;
+  const float most = __uint_as_float(most_bits);
+  if (t == 0) {
+    float scale = most / 127.f;
+    if constexpr (NORM) scale = scale * (1.f / sqrtf(sum / static_cast<float>(p.K) + p.eps));
+    if (most_bits == 0) scale = 0.f;
+    if (most_bits >= 0x7f800000u) scale = __uint_as_float(0x7fc00000u);
+    p.scale[row] = scale;
+  }
+  // by a power of two into the range where 127 v and the quotient's inverse are finite and normal
+  const float to = most < 0x1p-60f ? 0x1p64f : most > 0x1p60f ? 0x1p-64f : 1.f;
+  const float scaled = most * to, inv = 127.f / scaled;
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const int e = (c * TPR + t) * 8;
+    if (e >= p.K) break;
+    float u[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) u[i] = v[c][i] * to;
+    *reinterpret_cast<uint2*>(p.codes + row * p.cs + e) = none ? uint2{0, 0} : codes8(u, scaled, inv);
+  }
+}
+
+// code scale in T: a wave takes 2048 columns of a row.
+constexpr int kSpan = 2048;
+struct BackParams {
+  const int8_t* codes;
+  int64_t cs;
+  const float* scale;
+  void* out;
+  int64_t os;
+  int64_t items;  // rows * spans
+  int32_t spans;
+  int32_t K;
+};
+template <typename T> __global__ __launch_bounds__(256) void rows_from_int8_kernel(BackParams p) {
+  const int lane = threadIdx.x & 63;
+  const uint32_t item = blockIdx.x * 4u + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (item >= p.items) return;
+  const uint32_t row = item / static_cast<uint32_t>(p.spans);
+  const int first = static_cast<int>(item - row * p.spans) * kSpan + lane * 8;
+  const int8_t* codes = p.codes + row * p.cs;
+  const float scale = p.scale[row];
+  uint2 b[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) b[c] = *reinterpret_cast<const uint2*>(codes + min(first + c * 512, p.K - 8));
+  T* const out = static_cast<T*>(p.out) + row * p.os;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const int e = first + c * 512;
+    if (e >= p.K) break;
+    float f[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t word = i < 4 ? b[c].x : b[c].y;
+      f[i] = static_cast<float>(static_cast<int8_t>(word >> (8 * (i % 4)))) * scale;
+    }
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<sd::f32x4*>(out + e) = sd::f32x4{f[0], f[1], f[2], f[3]};
+      *reinterpret_cast<sd::f32x4*>(out + e + 4) = sd::f32x4{f[4], f[5], f[6], f[7]};
+    } else {
+      sd::store16(out + e, u32x4{sd::pack2<T>(f[0], f[1]), sd::pack2<T>(f[2], f[3]), sd::pack2<T>(f[4], f[5]),
+                                 sd::pack2<T>(f[6], f[7])});
+    }
+  }
+}
+
+template <typename T, bool NORM, bool RES> void launch(const Params& p, hipStream_t st) {
+#define SD_ROWS_INT8(tpr, c)                                                                              \
+  hipLaunchKernelGGL((rows_int8_kernel<T, NORM, RES, tpr, c>),                                            \
+                     dim3(static_cast<unsigned>(tpr < 256 ? (p.rows + 256 / tpr - 1) / (256 / tpr) : p.rows)), \
+                     dim3(tpr < 256 ? 256 : tpr), 0, st, p)
+  if (p.K <= 512) SD_ROWS_INT8(64, 1);
+  else if (p.K <= 1024) SD_ROWS_INT8(64, 2);
+  else if (p.K <= 4096) SD_ROWS_INT8(256, 2);
+  else if (p.K <= 8192) SD_ROWS_INT8(256, 4);
+  else if (p.K <= 16384) SD_ROWS_INT8(1024, 2);
+  else SD_ROWS_INT8(1024, 4);
+#undef SD_ROWS_INT8
+}
+template <typename T> void launch(const Params& p, hipStream_t st) {
+  if (!p.w) launch<T, false, false>(p, st);
+  else if (p.res) launch<T, true, true>(p, st);
+  else launch<T, true, false>(p, st);
+}
+
+constexpr int kMostColumns = 32768;
+// (a launch takes fewer than 2^32 threads)
+constexpr int64_t most_rows(int32_t columns) { return columns > 8192 ? (1 << 22) - 1 : (1 << 24) - 1; }
+
+// What both entries ask of their sizes and outputs; SD_OK or the refusal.
+int check(const char* what, const Params& p, int32_t dtype, bool residual) {
+  if (p.rows < 0 || p.K <= 0) {
+    sd::set_error("%s: invalid sizes (%lld rows of %d columns)", what, (long long)p.rows, p.K);
+    return SD_ERR_VALUE;
+  }
+  if (p.K % 16 != 0 || p.K > kMostColumns || p.rows > most_rows(p.K) || (dtype != SD_BF16 && dtype != SD_F16)) {
+    sd::set_error("%s: columns must be a multiple of 16 up to %d, rows below 2^24 (2^22 past 8192 columns), dtype bf16 "
+                  "or f16 (%lld rows of %d columns, dtype %d)", what, kMostColumns, (long long)p.rows, p.K, dtype);
+    return SD_ERR_UNSUPPORTED;
+  }
+  if (p.rows == 0) return SD_OK;
+  if (!p.x || !p.codes || !p.scale || (residual && !p.res_out)) {
+    sd::set_error("%s: null pointer argument", what);
+    return SD_ERR_VALUE;
+  }
+  if (!sd::strides_ok({p.xs, p.rs, p.cs, p.ros}) || (p.rows > 1 && (p.cs < p.K || (residual && p.ros < p.K)))) {
+    sd::set_error("%s: strides must lie within 2^40, output rows may not overlap", what);
+    return SD_ERR_VALUE;
+  }
+  const bool more = p.rows > 1;
+  if (!sd::aligned16(p.x) || !sd::aligned16(p.codes) || (more && (p.xs % 8 || p.cs % 16)) ||
+      (p.w && !sd::aligned16(p.w)) ||
+      (residual && (!sd::aligned16(p.res) || !sd::aligned16(p.res_out) || (more && (p.rs % 8 || p.ros % 8))))) {
+    sd::set_error("%s: rows must be 16-byte aligned", what);
+    return SD_ERR_UNSUPPORTED;
+  }
+  return SD_OK;
+}
+
+int run(const char* what, const Params& p, int32_t dtype, void* stream) {
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (dtype == SD_BF16) launch<__bf16>(p, st);
+  else launch<_Float16>(p, st);
+  return sd::check_launch(what);
+}
+
+}  // namespace
+
+extern "C" int sd_quantize_rows_int8(const void* x, int64_t x_stride, int8_t* codes, int64_t codes_stride,
+                                     float* scale, int64_t rows, int32_t columns, int32_t dtype, void* stream) {
+  sd::clear_error();
+  const Params p{static_cast<const uint16_t*>(x), x_stride, nullptr, 0, nullptr, codes, codes_stride, scale,
+                 nullptr, 0, rows, columns, 0.f};
+  const int rc = check("quantize_rows_int8", p, dtype, false);
+  return rc != SD_OK || rows == 0 ? rc : run("quantize_rows_int8", p, dtype, stream);
+}
+
+extern "C" int sd_rmsnorm_int8(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
+                               const void* weight, int8_t* codes, int64_t codes_stride, float* scale,
+                               void* residual_out, int64_t residual_out_stride, int64_t rows, int32_t hidden,
+                               float eps, int32_t dtype, void* stream) {
+  sd::clear_error();
+  const Params p{static_cast<const uint16_t*>(x), x_stride, static_cast<const uint16_t*>(residual), residual_stride,
+                 static_cast<const uint16_t*>(weight), codes, codes_stride, scale,
+                 static_cast<uint16_t*>(residual_out), residual_out_stride, rows, hidden, eps};
+  const int rc = check("rmsnorm_int8", p, dtype, residual != nullptr);
+  if (rc != SD_OK || rows == 0) return rc;
+  if (!weight) {
+    sd::set_error("rmsnorm_int8: null pointer argument");
+    return SD_ERR_VALUE;
+  }
+  return run("rmsnorm_int8", p, dtype, stream);
+}
+
+extern "C" int sd_dequantize_rows_int8(const int8_t* codes, int64_t codes_stride, const float* scale, void* out,
+                                       int64_t out_stride, int64_t rows, int32_t columns, int32_t dtype,
+                                       void* stream) {
+  sd::clear_error();
+  const char* what = "dequantize_rows_int8";
+  if (rows < 0 || columns <= 0) {
+    sd::set_error("%s: invalid sizes (%lld rows of %d columns)", what, (long long)rows, columns);
+    return SD_ERR_VALUE;
+  }
+  BackParams p{codes, codes_stride, scale, out, out_stride, 0, (columns - 1) / kSpan + 1, columns};
+  if (columns % 16 != 0 || rows >= (1ll << 26) / p.spans || (dtype != SD_BF16 && dtype != SD_F16 && dtype != SD_F32)) {
+    sd::set_error("%s: columns must be a multiple of 16, rows below 2^26 for each 2048 of them, dtype bf16, f16 or f32 "
+                  "(%lld rows of %d columns, dtype %d)", what, (long long)rows, columns, dtype);
+    return SD_ERR_UNSUPPORTED;
+  }
+  if (rows == 0) return SD_OK;
+  if (!codes || !scale || !out) {
+    sd::set_error("%s: null pointer argument", what);
+    return SD_ERR_VALUE;
+  }
+  if (!sd::strides_ok({codes_stride, out_stride}) || (rows > 1 && out_stride < columns)) {
+    sd::set_error("%s: strides must lie within 2^40, output rows may not overlap", what);
+    return SD_ERR_VALUE;
+  }
+  if (!sd::aligned16(codes) || !sd::aligned16(out) ||
+      (rows > 1 && (codes_stride % 16 || out_stride % (dtype == SD_F32 ? 4 : 8)))) {
+    sd::set_error("%s: rows must be 16-byte aligned", what);
+    return SD_ERR_UNSUPPORTED;
+  }
+  p.items = rows * p.spans;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const dim3 grid(static_cast<unsigned>((p.items + 3) / 4)), block(256);
+  if (dtype == SD_BF16) hipLaunchKernelGGL(rows_from_int8_kernel<__bf16>, grid, block, 0, st, p);
+  else if (dtype == SD_F16) hipLaunchKernelGGL(rows_from_int8_kernel<_Float16>, grid, block, 0, st, p);
+  else hipLaunchKernelGGL(rows_from_int8_kernel<float>, grid, block, 0, st, p);
+  return sd::check_launch(what);
+}

@@ -808,6 +808,153 @@ def w4a16_linear(x: torch.Tensor, qweight: torch.Tensor, scale: torch.Tensor,
     return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
 
 
+# ------------------------------------------------------------------- 8-bit activations
+def _rows8(t: torch.Tensor) -> torch.Tensor:
+    """2-D (rows, width) view with a unit last stride and rows at 16-byte addresses; a copy where
+    they are not."""
+    t2 = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
+    s0, s1 = t2.stride()
+    if s1 != 1 or t2.data_ptr() % 16 or (t2.shape[0] > 1 and (s0 < 0 or s0 * t2.element_size() % 16)):
+        # (not contiguous(): a contiguous view may start anywhere, and stays where it is)
+        t2 = t2.clone(memory_format=torch.contiguous_format)
+    return t2
+
+
+def quantize_rows_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rows of activations in 8 bits: x (..., K) bf16/fp16 -> (codes int8 (..., K), scale fp32
+    (...,)), value = code * scale, scale = max|x| / 127 and code = round_half_even(127 x / max|x|).
+    A row with a NaN or an infinity has scale NaN, a row of zeros scale 0. K a multiple of 16 up
+    to 32768. (``quantize_int8`` makes weights: a bf16 scale, rounded after the codes.)"""
+    x2 = _rows8(x)
+    rows, K = x2.shape
+    dev = _lib.require_device(x2)
+    codes = torch.empty((rows, K), dtype=torch.int8, device=dev)
+    scale = torch.empty(rows, dtype=torch.float32, device=dev)
+    with _lib.on_device(dev):
+        rc = _lib.load().sd_quantize_rows_int8(
+            x2.data_ptr(), x2.stride(0), codes.data_ptr(), K, scale.data_ptr(), rows, K,
+            _lib.dtype_code(x.dtype), _lib.stream_ptr(dev))
+    _lib.check(rc)
+    return (codes, scale) if x.dim() == 2 else (codes.view(x.shape), scale.view(x.shape[:-1]))
+
+
+def rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float,
+                 residual: torch.Tensor | None = None):
+    """``rmsnorm`` whose result goes to 8 bits as ``quantize_rows_int8``'s, without a rounding to 16
+    bits on the way: returns (codes, scale), with ``residual`` (codes, scale, residual_out), where s =
+    x + residual in fp32, residual_out = s rounded to the dtype and the codes are of the norm of s."""
+    x2 = _rows8(x)
+    rows, H = x2.shape
+    dt = x.dtype
+    assert weight.shape == (H,), "weight must be (hidden,)"
+    w = weight if weight.dtype == dt else weight.to(dt)
+    if not w.is_contiguous() or w.data_ptr() % 16:
+        w = w.clone(memory_format=torch.contiguous_format)
+    r2 = ro = None
+    if residual is not None:
+        assert residual.shape == x.shape and residual.dtype == dt
+        r2 = _rows8(residual)
+    dev = _lib.require_device(x2, w, r2)
+    codes = torch.empty((rows, H), dtype=torch.int8, device=dev)
+    scale = torch.empty(rows, dtype=torch.float32, device=dev)
+    if r2 is not None:
+        ro = torch.empty((rows, H), dtype=dt, device=dev)
+    with _lib.on_device(dev):
+        rc = _lib.load().sd_rmsnorm_int8(
+            x2.data_ptr(), x2.stride(0), _ptr(r2), 0 if r2 is None else r2.stride(0), w.data_ptr(),
+            codes.data_ptr(), H, scale.data_ptr(), _ptr(ro), H, rows, H, eps, _lib.dtype_code(dt),
+            _lib.stream_ptr(dev))
+    _lib.check(rc)
+    if x.dim() != 2:
+        codes, scale = codes.view(x.shape), scale.view(x.shape[:-1])
+        ro = None if ro is None else ro.view(x.shape)
+    return (codes, scale) if ro is None else (codes, scale, ro)
+
+
+def dequantize_rows_int8(codes: torch.Tensor, scale: torch.Tensor,
+                         dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values of 8-bit rows: codes (..., K) int8 times scale (...,) fp32, rounded to ``dtype``
+    (bf16, fp16 or fp32). Per-channel int8 weights with their scale in fp32 too."""
+    assert codes.dtype == torch.int8 and scale.dtype == torch.float32
+    assert scale.shape == codes.shape[:-1], f"one scale a row: {tuple(scale.shape)} for {tuple(codes.shape)}"
+    c2 = _rows8(codes)
+    s = _flat(scale, torch.float32)
+    rows, K = c2.shape
+    dev = _lib.require_device(c2, s)
+    out = torch.empty((rows, K), dtype=dtype, device=dev)
+    with _lib.on_device(dev):
+        rc = _lib.load().sd_dequantize_rows_int8(
+            c2.data_ptr(), c2.stride(0), s.data_ptr(), out.data_ptr(), K, rows, K,
+            _lib.dtype_code(dtype), _lib.stream_ptr(dev))
+    _lib.check(rc)
+    return out if codes.dim() == 2 else out.view(codes.shape)
+
+
+# ----------------------------------------------------------------------------- w8a8
+def _w8a8(gated: bool, x, x_scale, qweight, scale, bias, dtype, out):
+    assert x.dtype == torch.int8 and qweight.dtype == torch.int8, \
+        f"x and qweight must be int8, got {x.dtype} and {qweight.dtype}"
+    assert qweight.dim() == 2 and x_scale.dtype == torch.float32
+    wrows, K = qweight.shape
+    assert not gated or wrows % 2 == 0, "qweight must be [gate; up]"
+    N = wrows // 2 if gated else wrows
+    assert x.shape[-1] == K, f"K mismatch: x {tuple(x.shape)} vs w {tuple(qweight.shape)}"
+    assert x_scale.shape == x.shape[:-1], f"one scale a row: {tuple(x_scale.shape)} for {tuple(x.shape)}"
+    assert scale.numel() == wrows, "scale must have one entry per weight row"
+    x2, qw = _rows8(x), _rows8(qweight)
+    M = x2.shape[0]
+    if M > 1 and x2.stride(0) > 1 << 23:
+        x2 = x2.clone(memory_format=torch.contiguous_format)
+    xs = _flat(x_scale, torch.float32)
+    sc = _flat(scale, scale.dtype)
+    b = None
+    if bias is not None:
+        assert bias.shape == (wrows,), "bias must have one entry per weight row"
+        b = _flat(bias, dtype)
+    dev = _lib.require_device(x2, xs, qw, sc, b, out)
+    shape = (*x.shape[:-1], N)
+    if out is None:
+        y = torch.empty((M, N), device=dev, dtype=dtype)
+    else:
+        assert out.shape == shape, f"out must be {shape}, got {tuple(out.shape)}"
+        y = out.view(M, N)
+        assert y.dtype == dtype and (N == 1 or y.stride(1) == 1)
+    if M:
+        lib = _lib.load()
+        with _lib.on_device(dev):
+            # the plan (and so the workspace) depends on the device's compute units
+            ws_bytes = lib.sd_w8a8_workspace_size(M, N, K, gated)
+            ws = _workspace(ws_bytes, dev)
+            rc = (lib.sd_w8a8_gate_up_silu if gated else lib.sd_w8a8_linear)(
+                x2.data_ptr(), x2.stride(0), xs.data_ptr(), qw.data_ptr(), qw.stride(0), sc.data_ptr(),
+                _lib.dtype_code(sc.dtype), _ptr(b), y.data_ptr(), y.stride(0), M, N, K,
+                _lib.dtype_code(dtype), _ptr(ws), ws_bytes, _lib.stream_ptr(dev))
+        _lib.check(rc)
+    return y if x.dim() == 2 else y.view(shape)
+
+
+def w8a8_linear(x: torch.Tensor, x_scale: torch.Tensor, qweight: torch.Tensor, scale: torch.Tensor,
+                bias: torch.Tensor | None = None, dtype: torch.dtype = torch.bfloat16,
+                out: torch.Tensor | None = None) -> torch.Tensor:
+    """y = (x @ qweight^T) * scale * x_scale + bias in 8-bit integers.
+
+    x (..., K) int8 and x_scale (...,) fp32: activations of ``quantize_rows_int8`` or
+    ``rmsnorm_int8``; qweight (N, K) int8 and scale (N,): the weights of ``w8a16_linear``, per
+    channel. K a multiple of 16 below 2^17. Exact integer sums, fp32 scales, one rounding to
+    ``dtype`` (bf16 or fp16); returns (..., N)."""
+    return _w8a8(False, x, x_scale, qweight, scale, bias, dtype, out)
+
+
+def w8a8_gate_up_silu(x: torch.Tensor, x_scale: torch.Tensor, qweight: torch.Tensor,
+                      scale: torch.Tensor, bias: torch.Tensor | None = None,
+                      dtype: torch.dtype = torch.bfloat16,
+                      out: torch.Tensor | None = None) -> torch.Tensor:
+    """silu(gate) * up of the MLP's gate_up projection as ``w8a8_linear``: qweight (2I, K) =
+    [gate; up], scale (2I,); returns (..., I). gate and up are not rounded on the way
+    (``w8a16_gate_up_silu`` keeps the module's own roundings)."""
+    return _w8a8(True, x, x_scale, qweight, scale, bias, dtype, out)
+
+
 def quantize_int8(w: torch.Tensor, group_size: int = 0):
     """Symmetric int8 quantization of a 2-D weight on the GPU (the W8A16
     format's producer, nanovllm/layers/quant.py:123-148): per row (group_size

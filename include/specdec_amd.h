@@ -781,7 +781,8 @@ int sd_dequantize_rows_int8(const int8_t* codes, int64_t codes_stride, const flo
 size_t sd_w8a8_workspace_size(int64_t M, int64_t N, int64_t K, int32_t gated);
 /*
  * The route of a shape on the current device (host only):
- *   K slices | weight rows of a tile << 8 | activation rows of a tile << 20
+ *   K slices | weight rows of a tile << 8 | activation rows of a tile << 20 |
+ *   workgroups a compute unit holds << 32
  * of the tiled kernel; waves | weight rows of a tile << 8 of the kernel for few rows; 0
  * for sizes that the linear refuses.
  */

@@ -32,16 +32,19 @@ def norm_scale(most, s, eps):
     return most / 127 / np.sqrt((s * s).mean(-1) + eps)
 
 
+def _sums(x, w):
+    """Whole numbers below 2^53, so that 64-bit floats hold every partial sum."""
+    return x.astype(np.float64) @ w.astype(np.float64).T
+
+
 def linear32(x, x_scale, w, scale, bias=None):
     """The operator's own arithmetic: exact integer sums, then fp32 products in its order. float32, unrounded."""
-    sums = x.astype(np.int64) @ w.astype(np.int64).T
-    y = sums.astype(np.float32) * scale.astype(np.float32)[None] * x_scale.astype(np.float32)[:, None]
+    y = _sums(x, w).astype(np.float32) * scale.astype(np.float32)[None] * x_scale.astype(np.float32)[:, None]
     return y if bias is None else y + bias.astype(np.float32)[None]
 
 
 def linear64(x, x_scale, w, scale, bias=None):
-    sums = (x.astype(np.int64) @ w.astype(np.int64).T).astype(np.float64)
-    y = sums * scale.astype(np.float64)[None] * x_scale.astype(np.float64)[:, None]
+    y = _sums(x, w) * scale.astype(np.float64)[None] * x_scale.astype(np.float64)[:, None]
     return y if bias is None else y + bias.astype(np.float64)[None]
 
 

@@ -7,10 +7,11 @@
 // are the same bits whatever the other rows, tiles or K slices of the call.
 // The MFMAs take the weights as their rows, so that a lane holds neighbouring outputs of one token.
 //
-// w8a8_rows, few rows: bound by the weights' bytes. 16 weight rows a tile, straight to registers; the waves of a
-// workgroup take the columns in turn and add their sums in LDS.
+// w8a8_rows, few rows: bound by the weights' bytes. 16 weight rows a workgroup, straight to registers.
 // w8a8_gemm, above: tiles in LDS, loaded steps ahead (global_load_lds); K is split over workgroups where the tiles
 // alone leave compute units idle, and w8a8_reduce adds the slices.
+#include <type_traits>
+
 #include "sd_common.h"
 
 namespace {
@@ -49,9 +50,11 @@ __device__ __forceinline__ float output(int32_t sum, float ws, float xs, bool ha
   const float y = static_cast<float>(sum) * ws * xs;
   return has_bias ? y + bias : y;
 }
+// silu(gate) up by the exponential of -|gate|: that of -gate overflows from -89 down, where the result is still 1e-37.
 __device__ __forceinline__ float silu_up(float gate, float up) {
 #pragma clang fp contract(off)
-  return gate / (1.f + expf(-gate)) * up;
+  const float e = expf(-fabsf(gate));
+  return (gate < 0.f ? gate * e : gate) / (1.f + e) * up;
 }
 
 __device__ __forceinline__ i32x4 mfma16(u32x4 a, u32x4 b, i32x4 c) {
@@ -61,104 +64,85 @@ __device__ __forceinline__ i32x16 mfma32(u32x4 a, u32x4 b, i32x16 c) {
   return __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
 }
 
-// Up to 16 XT rows; a workgroup takes NT tiles of 16 weight rows (GATED: the gate's and the up rows of 16 outputs),
-// its waves the stages of 256 columns in turn.
-constexpr int kStage = 256;
+// Up to 16 XT rows. A workgroup takes 16 weight rows (GATED: the gate's and the up rows of 8 outputs), its waves the
+// stages of 128 columns in turn, loaded straight to registers two stages ahead. The activations come from the caches,
+// as many bytes a lane as of weights, which is what bounds it for more rows or many weight rows: 16 x 19456 x 2560
+// takes 14.4 us here, 11.4 in tiles, 1 x 19456 x 2560 10.3 and 11.1. Registers decide how many loads a compute unit
+// has in flight: stages of 256 columns took 10.9 us there, three of them ahead 10.6, two tiles a wave 13.9;
+// nontemporal loads of the weights 13.5.
+constexpr int kStage = 128;
 
-template <typename T, int XT, int NT, bool GATED>
-__global__ __launch_bounds__(1024) void w8a8_rows(Args a) {
-  extern __shared__ __attribute__((aligned(16))) int32_t red[];  // [wave][tile][token][16]
-  constexpr int kCols = GATED ? 16 : 16 * NT;                    // outputs of a workgroup
-  static_assert(!GATED || NT == 2, "a gate tile and an up tile");
+template <typename T, int XT, bool GATED>
+__global__ __launch_bounds__(512) void w8a8_rows(Args a) {
+  extern __shared__ __attribute__((aligned(16))) int32_t red[];  // [wave][token][16]
+  constexpr int kCols = GATED ? 8 : 16;                          // outputs of a workgroup
+  constexpr int kUnits = kStage / 64;
   const int W = blockDim.x >> 6, M = static_cast<int>(a.M);
   const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t n0 = static_cast<int64_t>(blockIdx.x) * kCols;
-  const int8_t* wrow[NT];
-#pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const int64_t n = min(n0 + (GATED ? 0 : 16 * t) + lr, a.N - 1);
-    wrow[t] = a.w + ((GATED && t == 1 ? a.N : 0) + n) * a.ws;
-  }
+  const int64_t n = min(n0 + (GATED ? lr & 7 : lr), a.N - 1) + (GATED && lr >= 8 ? a.N : 0);
+  const int8_t* const wrow = a.w + n * a.ws + 16 * lg;
   const int8_t* xrow[XT];
 #pragma unroll
-  for (int i = 0; i < XT; ++i) xrow[i] = a.x + min(16 * i + lr, M - 1) * a.xs;
-  i32x4 acc[XT][NT];
+  for (int i = 0; i < XT; ++i) xrow[i] = a.x + min(16 * i + lr, M - 1) * a.xs + 16 * lg;
+  i32x4 acc[XT];
 #pragma unroll
-  for (int i = 0; i < XT; ++i)
-#pragma unroll
-    for (int t = 0; t < NT; ++t) acc[i][t] = i32x4{0, 0, 0, 0};
+  for (int i = 0; i < XT; ++i) acc[i] = i32x4{0, 0, 0, 0};
   struct Stage {
-    u32x4 w[NT][4], x[XT][4];
+    u32x4 w[kUnits], x[XT][kUnits];
   };
   const int stages = (a.K + kStage - 1) / kStage;
   auto load = [&](Stage& st, int s) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int k = min(s * kStage + 64 * j + 16 * lg, a.K - 16);  // past K: columns that count nothing
-#pragma unroll
-      for (int t = 0; t < NT; ++t) st.w[t][j] = sd::load16_stream(wrow[t] + k);
+    for (int j = 0; j < kUnits; ++j) {
+      const int k = min(s * kStage + 64 * j, a.K - 16 - 16 * lg);  // past K: columns that count nothing
+      st.w[j] = sd::load16(wrow + k);
 #pragma unroll
       for (int i = 0; i < XT; ++i) st.x[i][j] = sd::load16(xrow[i] + k);
     }
   };
   auto compute = [&](Stage& st, int s) {
-    if (s * kStage + kStage > a.K) {
+    if (s * kStage + kStage > a.K) {  // uniform
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (s * kStage + 64 * j + 16 * lg >= a.K) {
-#pragma unroll
-          for (int i = 0; i < XT; ++i) st.x[i][j] = u32x4{0, 0, 0, 0};
-        }
+      for (int j = 0; j < kUnits; ++j)
+        if (s * kStage + 64 * j + 16 * lg >= a.K) st.w[j] = u32x4{0, 0, 0, 0};
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < kUnits; ++j)
 #pragma unroll
-      for (int i = 0; i < XT; ++i)
-#pragma unroll
-        for (int t = 0; t < NT; ++t) acc[i][t] = mfma16(st.w[t][j], st.x[i][j], acc[i][t]);
+      for (int i = 0; i < XT; ++i) acc[i] = mfma16(st.w[j], st.x[i][j], acc[i]);
   };
   Stage one, two;
   int s = wave;
   if (s < stages) load(one, s);
+  if (s + W < stages) load(two, s + W);
   for (; s < stages; s += 2 * W) {
-    if (s + W < stages) load(two, s + W);
     compute(one, s);
+    if (s + 2 * W < stages) load(one, s + 2 * W);
     if (s + W < stages) {
-      if (s + 2 * W < stages) load(one, s + 2 * W);
       compute(two, s + W);
+      if (s + 3 * W < stages) load(two, s + 3 * W);
     }
   }
-  // ---- the waves' sums meet: lane (lr, lg) holds outputs 4 lg .. 4 lg + 3 of token lr
+  // ---- the waves' sums meet: lane (lr, lg) holds weight rows 4 lg .. 4 lg + 3 of token lr
 #pragma unroll
   for (int i = 0; i < XT; ++i)
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-      *reinterpret_cast<i32x4*>(red + (((wave * NT + t) * XT + i) * 16 + lr) * 16 + 4 * lg) = acc[i][t];
+    *reinterpret_cast<i32x4*>(red + ((wave * XT + i) * 16 + lr) * 16 + 4 * lg) = acc[i];
   __syncthreads();
-  constexpr int kWave = NT * XT * 256;
+  const bool bias = a.bias != nullptr;
   for (int o = tid; o < kCols * M; o += W * 64) {
     const int m = o / kCols, c = o % kCols;
-    const int64_t n = n0 + c;
-    if (n >= a.N) continue;
+    const int64_t out = n0 + c;
+    if (out >= a.N) continue;
     const float xs = a.x_scale[m];
-    auto sum = [&](int t) {
-      const int32_t* r = red + (t * XT * 16 + m) * 16 + (c & 15);
+    auto value = [&](int row, int64_t at) {
       int32_t v = 0;
-      for (int u = 0; u < W; ++u) v += r[u * kWave];
-      return v;
+      for (int u = 0; u < W; ++u) v += red[(u * XT * 16 + m) * 16 + row];
+      return output(v, scale_at(a, at), xs, bias, bias ? sd::from_bits<T>(a.bias[at]) : 0.f);
     };
-    float y;
-    if constexpr (GATED) {
-      const bool bias = a.bias != nullptr;
-      const float g = output(sum(0), scale_at(a, n), xs, bias, bias ? sd::from_bits<T>(a.bias[n]) : 0.f);
-      const float u = output(sum(1), scale_at(a, a.N + n), xs, bias, bias ? sd::from_bits<T>(a.bias[a.N + n]) : 0.f);
-      y = silu_up(g, u);
-    } else {
-      const bool bias = a.bias != nullptr;
-      y = output(sum(c >> 4), scale_at(a, n), xs, bias, bias ? sd::from_bits<T>(a.bias[n]) : 0.f);
-    }
-    a.y[m * a.ys + n] = sd::to_bits<T>(y);
+    const float y = value(c, out);
+    a.y[m * a.ys + out] = sd::to_bits<T>(GATED ? silu_up(y, value(8 + c, a.N + out)) : y);
   }
 }
 
@@ -171,24 +155,28 @@ __device__ __forceinline__ uint32_t lds_addr(const void* l) {
       reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) void*)l)));
 }
 
-// WM x WN waves of MT x NT tiles of 32 tokens x 32 weight rows; S stages of 128 columns in LDS, loaded S - 1 steps
-// ahead. 16-byte unit u of LDS row r stands at u ^ (r % 8): 8 rows' operand reads hit 8 different units. The rows of
-// a weight tile are laid so that a lane's 16 sums of it are neighbours: MFMA row 8 a + 4 h + b is row 16 h + 4 a + b.
-// GATED: the first half of a wave's weight tiles are the gate's, the second the up rows of the same outputs.
+// WM x WN waves of MT x NT tiles of 32 tokens x 32 weight rows; S stages of 128 columns in LDS, loaded S steps ahead.
+// A step is four MFMA depths of 32 columns; the operands of a depth are read while the one before multiplies. Before
+// the last depth the workgroup meets: the next stage has landed (its first operands are read at once) and this one
+// is read by all, so that its place takes the stage S steps on. The MFMAs never wait for a barrier's first reads.
+// LDS: 16-byte unit u of a row stands at u ^ turn, so that 16 rows' operand reads hit 16 different places of 256 bytes
+// (64 banks). MFMA row 8 a + 4 h + b reads weight row 16 h + 4 a + b of its tile: a lane (half h of the wave) then holds
+// sums of 16 neighbouring rows. GATED: rows 0 .. 15 of a tile are the gate's of 16 outputs, 16 .. 31 the up rows.
 constexpr int kBlock = 128;
 
 template <typename T, int WM, int WN, int MT, int NT, int S, bool GATED>
-__global__ __launch_bounds__(WM * WN * 64) void w8a8_gemm(Args a) {
+__global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(WM * WN / 4))) void w8a8_gemm(Args a) {
   constexpr int NW = WM * WN, BM = 32 * MT * WM, BN = 32 * NT * WN;
-  constexpr int BO = GATED ? BN / 2 : BN;  // outputs
+  constexpr int BO = GATED ? BN / 2 : BN;            // outputs
   constexpr int CX = BM / 8 / NW, CW = BN / 8 / NW;  // 1 KB loads (8 rows) of a wave and step
   constexpr int kX = BM * kBlock, kBytes = (BM + BN) * kBlock;
   constexpr int kPitch = 2 * BO + 16;  // of the output tile
   constexpr int kTile = S * kBytes > BM * kPitch ? S * kBytes : BM * kPitch;
+  constexpr int kLoads = CX + CW, kDepths = kBlock / 32;
   static_assert(CX * NW * 8 == BM && CW * NW * 8 == BN, "whole 1 KB loads");
-  static_assert(!GATED || NT % 2 == 0, "as many gate tiles as up tiles");
+  static_assert(S <= 4, "what meet_at counts");
   __shared__ __attribute__((aligned(1024))) uint8_t sm[kTile];
-  __shared__ __attribute__((aligned(16))) float lws[BN], lxs[BM], lbias[BN];
+  __shared__ __attribute__((aligned(16))) float lws[BN], lbias[BN], lxs[BM];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 31, lh = lane >> 5;
@@ -211,56 +199,60 @@ __global__ __launch_bounds__(WM * WN * 64) void w8a8_gemm(Args a) {
   const int b0 = static_cast<int>(static_cast<int64_t>(slice) * blocks / a.slices);
   const int b1 = static_cast<int>(static_cast<int64_t>(slice + 1) * blocks / a.slices);
 
-  // LDS weight row -> output column of the tile (and whether it is an up row)
-  auto col_of = [](int r) {
-    const int q = r % 32, c = 16 * ((q >> 2) & 1) + 4 * (q >> 3) + (q & 3);
-    if constexpr (GATED) return r / (32 * NT) * (16 * NT) + r / 32 % (NT / 2) * 32 + c;
-    else return r - q + c;
-  };
-  auto is_up = [](int r) { return GATED && r / 32 % NT >= NT / 2; };
+  auto x_turn = [](int r) { return (r >> 1) & 7; };
+  auto w_turn = [](int r) { return ((r >> 1) & 3) | ((r >> 4) & 1) << 2; };
+  auto column = [](int r) { return GATED ? (r >> 5) * 16 + (r & 15) : r; };  // of the tile's weight row r
+  auto is_up = [](int r) { return GATED && (r & 16) != 0; };
 
-  // ---- loads: 8 rows an instruction, lane l unit (l % 8) ^ (l / 8) of row l / 8; rows past M or N repeat the last
+  // ---- loads: 8 rows an instruction, lane l 16 bytes of row l / 8; rows past M or N repeat the last
   const int8_t* const xbase = a.x + m0 * a.xs;
   const int8_t* const wbase = a.w + n0 * a.ws;
   const int64_t up = GATED ? a.N * a.ws : 0;
-  const uint32_t unit = 16 * ((lane & 7) ^ (lane >> 3));
+  auto x_unit = [&](int i) { return 16u * ((lane & 7) ^ x_turn((wave * CX + i) * 8 + (lane >> 3))); };
+  auto w_unit = [&](int i) { return 16u * ((lane & 7) ^ w_turn((wave * CW + i) * 8 + (lane >> 3))); };
   uint32_t xoff[CX], woff[CW];
 #pragma unroll
-  for (int i = 0; i < CX; ++i)
-    xoff[i] = static_cast<uint32_t>(min(static_cast<int64_t>((wave * CX + i) * 8 + (lane >> 3)), a.M - 1 - m0)) *
-              static_cast<uint32_t>(a.xs);
+  for (int i = 0; i < CX; ++i) {
+    const int r = (wave * CX + i) * 8 + (lane >> 3);
+    xoff[i] = static_cast<uint32_t>(min(static_cast<int64_t>(r), a.M - 1 - m0)) * static_cast<uint32_t>(a.xs) + x_unit(i);
+  }
 #pragma unroll
-  for (int i = 0; i < CW; ++i)
-    woff[i] = static_cast<uint32_t>(min(static_cast<int64_t>(col_of((wave * CW + i) * 8 + (lane >> 3))), a.N - 1 - n0)) *
-              static_cast<uint32_t>(a.ws);
+  for (int i = 0; i < CW; ++i) {
+    const int r = (wave * CW + i) * 8 + (lane >> 3);
+    woff[i] = static_cast<uint32_t>(min(static_cast<int64_t>(column(r)), a.N - 1 - n0)) * static_cast<uint32_t>(a.ws) +
+              w_unit(i);
+  }
   const uint32_t sm_at = lds_addr(sm);
-  const int blast = max(b1 - 1, b0);  // past the slice: its last block again, so that every step loads as much
-  auto load = [&](int blk, int buf) {
-    blk = min(blk, blast);
+  // The wave's loads [from, to) of a stage; `whole`: none of its columns lies past K (otherwise the last unit of a row
+  // again, columns that count nothing).
+  auto load = [&](int blk, int buf, int from, int to, auto whole) {
     const uint32_t at = sm_at + buf * kBytes;
-    const uint32_t u = min(unit, static_cast<uint32_t>(a.K - 16 - blk * kBlock));  // past K: columns that count nothing
-    const int8_t* xb = xbase + blk * kBlock;
-    const int8_t* wb = wbase + blk * kBlock;
+    const uint32_t last = static_cast<uint32_t>(a.K - 16 - blk * kBlock);
 #pragma unroll
-    for (int i = 0; i < CX; ++i) to_lds16(xb, xoff[i] + u, at + (wave * CX + i) * 1024);
-#pragma unroll
-    for (int i = 0; i < CW; ++i)
-      to_lds16(is_up((wave * CW + i) * 8) ? wb + up : wb, woff[i] + u, at + kX + (wave * CW + i) * 1024);
+    for (int i = 0; i < kLoads; ++i) {
+      if (i < from || i >= to) continue;
+      if (i < CX) {
+        uint32_t off = xoff[i];
+        if constexpr (!decltype(whole)::value) off += min(x_unit(i), last) - x_unit(i);
+        to_lds16(xbase + blk * kBlock, off, at + (wave * CX + i) * 1024);
+      } else {
+        const int c = wave * CW + i - CX;
+        uint32_t off = woff[i - CX];
+        if constexpr (!decltype(whole)::value) off += min(w_unit(i - CX), last) - w_unit(i - CX);
+        to_lds16(wbase + (is_up(c * 8) ? up : 0) + blk * kBlock, off, at + kX + c * 1024);
+      }
+    }
   };
-#pragma unroll
-  for (int i = 0; i < S - 1; ++i) load(b0 + i, i);
-  // the scales, by output column in the order of a wave's tiles
+  // the scales and the bias, in the order of the tile's weight rows
   for (int r = tid; r < BN; r += NW * 64) {
-    // r: wave wn, tile, neighbour
-    const int t = r / 32 % NT;
-    int64_t n;
-    if constexpr (GATED) n = n0 + r / (32 * NT) * (16 * NT) + t % (NT / 2) * 32 + r % 32;
-    else n = n0 + r;
-    n = min(n, a.N - 1) + (GATED && t >= NT / 2 ? a.N : 0);
+    const int64_t n = min(n0 + column(r), a.N - 1) + (is_up(r) ? a.N : 0);
     lws[r] = scale_at(a, n);
     lbias[r] = a.bias ? sd::from_bits<T>(a.bias[n]) : 0.f;
   }
   for (int r = tid; r < BM; r += NW * 64) lxs[r] = a.x_scale[min(m0 + r, a.M - 1)];
+#pragma unroll
+  for (int i = 0; i < S; ++i)
+    if (b0 + i < b1) load(b0 + i, i, 0, kLoads, std::false_type{});
 
   i32x16 acc[MT][NT];
 #pragma unroll
@@ -269,41 +261,65 @@ __global__ __launch_bounds__(WM * WN * 64) void w8a8_gemm(Args a) {
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][t][e] = 0;
-  // operand reads: unit 2 j + lh of row lr of a tile
-  uint32_t at[4];
+  uint32_t x_at[kDepths], w_at[kDepths];  // operand reads: unit 2 j + lh of a row
+  const int wr = 16 * ((lr >> 2) & 1) + 4 * (lr >> 3) + (lr & 3);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) at[j] = lr * kBlock + (((2 * j + lh) ^ (lr & 7)) * 16);
-  constexpr int kLoads = CX + CW;
+  for (int j = 0; j < kDepths; ++j) {
+    x_at[j] = wm * (MT * 32 * kBlock) + lr * kBlock + (((2 * j + lh) ^ x_turn(lr)) * 16);
+    w_at[j] = kX + wn * (NT * 32 * kBlock) + wr * kBlock + (((2 * j + lh) ^ w_turn(wr)) * 16);
+  }
+  u32x4 xf[2][MT], wf[2][NT];
+  // The workgroup meets: all but the newest `stages` stages have landed in every wave's view, and every LDS read so far
+  // is done.
+  auto meet_at = [&](int stages) {
+#define SD_MEET(n) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((n) * kLoads) : "memory")
+    if (stages <= 0) SD_MEET(0);
+    else if (stages == 1) SD_MEET(1);
+    else if (stages == 2) SD_MEET(2);
+    else SD_MEET(3);
+#undef SD_MEET
+  };
+  meet_at(min(S, b1 - b0) - 1);
+#pragma unroll
+  for (int i = 0; i < MT; ++i) xf[0][i] = sd::load16(sm + x_at[0] + i * (32 * kBlock));
+#pragma unroll
+  for (int t = 0; t < NT; ++t) wf[0][t] = sd::load16(sm + w_at[0] + t * (32 * kBlock));
   int buf = 0;
-  for (int blk = b0; blk < b1; ++blk) {
-    // all but the newest S - 2 steps' loads have landed in every wave's view, and the slot of the step before is read
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((S - 2) * kLoads) : "memory");
-    load(blk + S - 1, buf == 0 ? S - 1 : buf - 1);
-    const uint8_t* const lx = sm + buf * kBytes + wm * (MT * 32 * kBlock);
-    const uint8_t* const lw = sm + buf * kBytes + kX + wn * (NT * 32 * kBlock);
+  auto step = [&](int blk, auto middle) {  // middle: the stage S on is a whole one
+    constexpr bool kMiddle = decltype(middle)::value;
+    const int next = buf + 1 == S ? 0 : buf + 1;
     const int left = a.K - blk * kBlock;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      u32x4 xf[MT], wf[NT];
-#pragma unroll
-      for (int i = 0; i < MT; ++i) xf[i] = sd::load16(lx + i * (32 * kBlock) + at[j]);
-#pragma unroll
-      for (int t = 0; t < NT; ++t) wf[t] = sd::load16(lw + t * (32 * kBlock) + at[j]);
-      if (left < kBlock) {  // uniform
+    for (int j = 0; j < kDepths; ++j) {
+      const bool meet = j == kDepths - 1;
+      if (meet) meet_at(kMiddle ? S - 2 : min(S - 2, b1 - 2 - blk));
+      const uint8_t* const from = sm + (meet ? next : buf) * kBytes;
+      const int jn = (j + 1) % kDepths, now = j & 1, then = now ^ 1;
+      if (!kMiddle && left < kBlock) {  // the last columns
         const bool none = 32 * j + 16 * lh >= left;
 #pragma unroll
         for (int t = 0; t < NT; ++t)
-          if (none) wf[t] = u32x4{0, 0, 0, 0};
+          if (none) wf[now][t] = u32x4{0, 0, 0, 0};
       }
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
+      for (int i = 0; i < MT; ++i) {
+        xf[then][i] = sd::load16(from + x_at[jn] + i * (32 * kBlock));
 #pragma unroll
-        for (int t = 0; t < NT; ++t) acc[i][t] = mfma32(wf[t], xf[i], acc[i][t]);
+        for (int t = i * NT / MT; t < (i + 1) * NT / MT; ++t)
+          wf[then][t] = sd::load16(from + w_at[jn] + t * (32 * kBlock));
+        if (meet && (kMiddle || blk + S < b1)) load(blk + S, buf, i * kLoads / MT, (i + 1) * kLoads / MT, middle);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[i][t] = mfma32(wf[now][t], xf[now][i], acc[i][t]);
+        // one row of tiles after another: with the loads and reads all moved ahead of the MFMAs these wait for them
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
-    buf = buf + 1 == S ? 0 : buf + 1;
-  }
-  // the loads that ran ahead land before the stages' LDS is written again, or is another's
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    buf = next;
+  };
+  const int whole = min(b1, a.K / kBlock);
+  int blk = b0;
+  for (; blk + S < whole; ++blk) step(blk, std::true_type{});
+  for (; blk < b1; ++blk) step(blk, std::false_type{});
   const int rows = static_cast<int>(min(static_cast<int64_t>(BM), a.M - m0));
   const int cols = static_cast<int>(min(static_cast<int64_t>(BO), a.N - n0));
   if (a.slices > 1) {  // a lane's 16 sums of a tile
@@ -311,8 +327,8 @@ __global__ __launch_bounds__(WM * WN * 64) void w8a8_gemm(Args a) {
     int32_t* const part = a.part + slice * a.M * width;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const int c0 = (GATED ? wn * (16 * NT) + t % (NT / 2) * 32 : (wn * NT + t) * 32) + 16 * lh;
-      const int64_t n = n0 + c0 + (GATED && t >= NT / 2 ? a.N : 0);
+      const int c0 = GATED ? (wn * NT + t) * 16 : (wn * NT + t) * 32 + 16 * lh;
+      const int64_t n = n0 + c0 + (GATED && lh ? a.N : 0);
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
         const int r = (wm * MT + i) * 32 + lr;
@@ -332,131 +348,221 @@ __global__ __launch_bounds__(WM * WN * 64) void w8a8_gemm(Args a) {
     }
     return;
   }
-  // ---- a lane's 16 neighbouring outputs of a token and tile, through LDS to whole lines
+  // ---- a lane's neighbouring outputs of a token and tile, through LDS to whole lines
   __syncthreads();
-  constexpr int kOut = GATED ? NT / 2 : NT;
   const bool has_bias = a.bias != nullptr;
 #pragma unroll
-  for (int t = 0; t < kOut; ++t) {
+  for (int t = 0; t < NT; ++t) {
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
       const int r = (wm * MT + i) * 32 + lr;
       const float xs = lxs[r];
-      const int at_w = (wn * NT + t) * 32 + 16 * lh;
-      uint32_t o[8];
+      if constexpr (GATED) {
+        // the halves of the wave exchange 8 gates for 8 ups: each has both of 8 outputs
+        const int at_w = (wn * NT + t) * 32 + 8 * lh;
+        uint32_t o[4];
 #pragma unroll
-      for (int e = 0; e < 16; e += 2) {
-        float v[2];
+        for (int e = 0; e < 8; e += 2) {
+          float v[2];
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          v[q] = output(acc[i][t][e + q], lws[at_w + e + q], xs, has_bias, lbias[at_w + e + q]);
-          if constexpr (GATED) {
-            const int up_w = at_w + kOut * 32 + e + q;
-            v[q] = silu_up(v[q], output(acc[i][t + kOut][e + q], lws[up_w], xs, has_bias, lbias[up_w]));
+          for (int q = 0; q < 2; ++q) {
+            const auto z = __builtin_amdgcn_permlane32_swap(static_cast<uint32_t>(acc[i][t][e + q]),
+                                                            static_cast<uint32_t>(acc[i][t][e + q + 8]), false, false);
+            const float g = output(static_cast<int32_t>(z[0]), lws[at_w + e + q], xs, has_bias, lbias[at_w + e + q]);
+            const float u = output(static_cast<int32_t>(z[1]), lws[at_w + 16 + e + q], xs, has_bias,
+                                   lbias[at_w + 16 + e + q]);
+            v[q] = silu_up(g, u);
           }
+          o[e / 2] = sd::pack2<T>(v[0], v[1]);
         }
-        o[e / 2] = sd::pack2<T>(v[0], v[1]);
+        sd::store16(sm + r * kPitch + ((wn * NT + t) * 16 + 8 * lh) * 2, u32x4{o[0], o[1], o[2], o[3]});
+      } else {
+        const int at_w = (wn * NT + t) * 32 + 16 * lh;
+        uint32_t o[8];
+#pragma unroll
+        for (int e = 0; e < 16; e += 2)
+          o[e / 2] = sd::pack2<T>(output(acc[i][t][e], lws[at_w + e], xs, has_bias, lbias[at_w + e]),
+                                  output(acc[i][t][e + 1], lws[at_w + e + 1], xs, has_bias, lbias[at_w + e + 1]));
+        uint8_t* const p = sm + r * kPitch + at_w * 2;
+        sd::store16(p, u32x4{o[0], o[1], o[2], o[3]});
+        sd::store16(p + 16, u32x4{o[4], o[5], o[6], o[7]});
       }
-      uint8_t* const p = sm + r * kPitch + ((wn * kOut + t) * 32 + 16 * lh) * 2;
-      sd::store16(p, u32x4{o[0], o[1], o[2], o[3]});
-      sd::store16(p + 16, u32x4{o[4], o[5], o[6], o[7]});
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
   __syncthreads();
   uint16_t* const y0 = a.y + m0 * a.ys + n0;
+  constexpr int kUnits = BO / 8;
   if (a.wide_y && cols % 8 == 0) {
-    for (int i = tid; i < rows * (BO / 8); i += NW * 64) {
-      const int r = i / (BO / 8), u = i % (BO / 8);
+    for (int i = tid; i < rows * kUnits; i += NW * 64) {
+      const int r = i / kUnits, u = i % kUnits;
       if (u * 8 < cols) sd::store16(y0 + r * a.ys + u * 8, sd::load16(sm + r * kPitch + u * 16));
     }
   } else {
-    for (int i = tid; i < rows * BO; i += NW * 64) {
-      const int r = i / BO, c = i % BO;
-      if (c < cols) y0[r * a.ys + c] = *reinterpret_cast<const uint16_t*>(sm + r * kPitch + c * 2);
+    // rows that start anywhere: the aligned 16 bytes of memory from a row's dwords in LDS, moved by half of one where
+    // the row starts inside a dword; single outputs at the ends (2-byte stores of everything took 7 us a tile)
+    for (int i = tid; i < rows * (kUnits + 1); i += NW * 64) {
+      const int r = i / (kUnits + 1), u = i % (kUnits + 1);
+      uint16_t* const row = y0 + r * a.ys;
+      const int first = 8 * u - static_cast<int>((reinterpret_cast<uintptr_t>(row) & 15) >> 1);
+      if (first >= 0 && first + 8 <= cols) {
+        const uint32_t* const d = reinterpret_cast<const uint32_t*>(sm + r * kPitch) + (first >> 1);
+        const uint32_t shift = (first & 1) * 16;
+        u32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = __builtin_amdgcn_alignbit(d[e + 1], d[e], shift);
+        sd::store16(row + first, v);
+      } else {
+        for (int e = max(first, 0); e < min(first + 8, cols); ++e)
+          row[e] = *reinterpret_cast<const uint16_t*>(sm + r * kPitch + e * 2);
+      }
     }
   }
 }
 
-// Sums of the K slices and the outputs.
-template <typename T, bool GATED> __global__ __launch_bounds__(256) void w8a8_reduce(Args a) {
-  const int64_t all = a.M * a.N, width = GATED ? 2 * a.N : a.N;
+// Sums of the K slices and the outputs; a thread takes V neighbouring outputs of a row (V divides N).
+template <typename T, bool GATED, int V> __global__ __launch_bounds__(256) void w8a8_reduce(Args a) {
+  const int64_t width = GATED ? 2 * a.N : a.N, all = a.M * a.N / V, step = a.M * width;
+  const bool has_bias = a.bias != nullptr;
   for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < all; i += gridDim.x * 256ll) {
-    const int64_t m = i / a.N, n = i - m * a.N;
+    const int64_t m = i * V / a.N, n = i * V - m * a.N;
     const float xs = a.x_scale[m];
-    const bool bias = a.bias != nullptr;
-    auto value = [&](int64_t c) {
-      int32_t s = 0;
-      for (int v = 0; v < a.slices; ++v) s += a.part[(v * a.M + m) * width + c];
-      return output(s, scale_at(a, c), xs, bias, bias ? sd::from_bits<T>(a.bias[c]) : 0.f);
-    };
-    const float y = value(n);
-    a.y[m * a.ys + n] = sd::to_bits<T>(GATED ? silu_up(y, value(a.N + n)) : y);
+    float out[2][V];
+#pragma unroll
+    for (int h = 0; h < (GATED ? 2 : 1); ++h) {
+      const int64_t c = n + (h ? a.N : 0);
+      const int32_t* p = a.part + m * width + c;
+      int32_t sum[V] = {};
+      for (int s = 0; s < a.slices; ++s, p += step) {
+        if constexpr (V == 4) {
+          const i32x4 v = *reinterpret_cast<const i32x4*>(p);
+#pragma unroll
+          for (int e = 0; e < V; ++e) sum[e] += v[e];
+        } else {
+          sum[0] += *p;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        out[h][e] = output(sum[e], scale_at(a, c + e), xs, has_bias, has_bias ? sd::from_bits<T>(a.bias[c + e]) : 0.f);
+    }
+    uint16_t* const y = a.y + m * a.ys + n;
+#pragma unroll
+    for (int e = 0; e < V; ++e) y[e] = sd::to_bits<T>(GATED ? silu_up(out[0][e], out[1][e]) : out[0][e]);
   }
 }
 
-// What runs a shape: w8a8_rows<XT, NT> of W waves (XT > 0), or tiles of bm x bn weight rows and K slices.
+// The tiles there are, with what they were measured to take (us): a round of workgroups `start` + steps x `alone`
+// where each has a compute unit to itself, `full` a step where `per_cu` share it; and, since the whole device multiplies
+// only as fast as its power allows, every workgroup `power_start` + steps x `power` of the device.
+struct Tile {
+  int bm, bn, per_cu;
+  double start, alone, full, power_start, power;
+};
+constexpr Tile kTiles[] = {
+    {256, 256, 1, 10.4, 1.047, 1.047, 0.055, 0.0060}, {192, 256, 1, 7.7, 0.850, 0.850, 0.040, 0.0050},
+    {128, 256, 1, 6.8, 0.568, 0.568, 0.024, 0.0038},  {192, 128, 1, 5.0, 0.517, 0.517, 0.020, 0.0030},
+    {128, 128, 1, 4.4, 0.366, 0.366, 0.014, 0.0024},  {128, 128, 2, 2.4, 0.525, 0.825, 0.006, 0.0022},
+    {64, 128, 2, 2.9, 0.257, 0.504, 0.004, 0.0013},   {32, 64, 4, 2.7, 0.183, 0.357, 0.002, 0.0005},
+};
+
+// What runs a shape: w8a8_rows<XT> of W waves (XT > 0), or a tile and K slices.
 struct Plan {
-  int XT, NT, W;
-  int bm, bn, slices;
+  int XT, W;
+  int tile, slices;
 };
 Plan make_plan(int64_t M, int64_t N, int64_t K, bool gated) {
   Plan pl{};
   const int64_t cus = sd::device_cus();
-  const int64_t wrows = gated ? 2 * N : N, stages = (K + kStage - 1) / kStage;
-  if (M <= 32) {
+  const int64_t wrows = gated ? 2 * N : N, groups = (wrows + 15) / 16, stages = (K + kStage - 1) / kStage;
+  // Few rows: up to 4 always (7 x 19456 x 2560 11.8 us there, 11.2 in tiles of 32 x 64; 16 14.4 and 11.4), up to 16
+  // where weight rows are few (16 x 6144 x 2560 6.8 and 7.6), up to 32 where they and the columns are (32 x 4096 x 1024
+  // 3.8 and 5.2, 32 x 2560 x 4096 7.7 and 8.9, 32 x 6144 x 2560 9.1 and 7.6, 32 x 2560 x 9728 16 and 11.2).
+  if (M <= 4 || (M <= 16 && groups <= 3 * cus) || (M <= 32 && groups <= cus && stages <= 32)) {
     pl.XT = M <= 16 ? 1 : 2;
-    pl.NT = gated ? 2 : 1;
-    const int64_t groups = (wrows + 16 * pl.NT - 1) / (16 * pl.NT);
-    pl.W = 4;
-    while (pl.W < 16 && groups * pl.W < 8 * cus && pl.W < stages) pl.W *= 2;
+    // 8 waves, 4 for very many workgroups (1 x 151936 x 1024 24.5 us, 27.1 with 8)
+    pl.W = groups > 16 * cus ? 4 : 8;
+    if (pl.W > stages) pl.W = static_cast<int>(stages);
     return pl;
   }
+  // The tile and slices of the least time by the figures above (over 262 shapes 1.4% above the fastest of them on
+  // average). Slices cost a launch and their sums' way to memory and back.
   const int64_t blocks = (K + kBlock - 1) / kBlock;
-  auto tiles = [&](int bm, int bn) { return ((M + bm - 1) / bm) * ((wrows + bn - 1) / bn); };
-  pl.bm = pl.bn = 256;
-  if (tiles(256, 256) < 2 * cus) pl.bm = pl.bn = 128;
-  if (tiles(128, 128) < cus) pl.bm = pl.bn = 64;
-  pl.slices = 1;
-  if (tiles(64, 64) < cus) {
-    int64_t s = cus / tiles(64, 64);
-    if (s > blocks / 4) s = blocks / 4;
-    pl.slices = s < 1 ? 1 : s > 16 ? 16 : static_cast<int>(s);
+  double least = 1e30;
+  for (int i = 0; i < static_cast<int>(sizeof(kTiles) / sizeof(kTiles[0])); ++i) {
+    const Tile& t = kTiles[i];
+    const int64_t tiles = ((M + t.bm - 1) / t.bm) * ((wrows + t.bn - 1) / t.bn), slots = t.per_cu * cus;
+    for (int64_t s = 1; s == 1 || (s <= 16 && 4 * s <= blocks && tiles * s <= slots); ++s) {
+      const int64_t steps = (blocks + s - 1) / s, rounds = tiles * s / slots, rest = (tiles * s % slots + cus - 1) / cus;
+      const double more = t.per_cu > 1 ? (t.full - t.alone) / (t.per_cu - 1) : 0;
+      double round = static_cast<double>(rounds) * (t.start + steps * t.full);
+      if (rest) round += t.start + steps * (t.alone + more * (rest - 1));
+      const double power = static_cast<double>(tiles * s) * (t.power_start + steps * t.power);
+      // (neither alone: a smooth maximum, since rounds do not end together)
+      const double r2 = round * round, p2 = power * power, r6 = r2 * r2 * r2, p6 = p2 * p2 * p2;
+      double cost = __builtin_cbrt(__builtin_sqrt(r6 + p6));
+      if (s > 1) cost += 3.4 + 0.16 * s + 1.6e-6 * s * static_cast<double>(M) * wrows;
+      if (cost < least) {
+        least = cost;
+        pl.tile = i;
+        pl.slices = static_cast<int>(s);
+      }
+    }
   }
   return pl;
+}
+
+template <typename T, bool GATED> void launch_tiles(const Args& a, int tile, hipStream_t st) {
+  const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.tiles_m) * a.tiles_n * a.slices));
+#define SD_TILES(i, wm, wn, mt, nt, s)                                                                           \
+  case i:                                                                                                        \
+    static_assert(kTiles[i].bm == 32 * wm * mt && kTiles[i].bn == 32 * wn * nt, "the table's tile");             \
+    hipLaunchKernelGGL((w8a8_gemm<T, wm, wn, mt, nt, s, GATED>), grid, dim3(64 * wm * wn), 0, st, a);            \
+    break
+  switch (tile) {
+    SD_TILES(0, 2, 4, 4, 2, 2);
+    SD_TILES(1, 2, 4, 3, 2, 2);
+    SD_TILES(2, 2, 4, 2, 2, 3);
+    SD_TILES(3, 2, 4, 3, 1, 3);
+    SD_TILES(4, 2, 4, 2, 1, 4);
+    SD_TILES(5, 2, 4, 2, 1, 2);
+    SD_TILES(6, 2, 4, 1, 1, 3);
+    SD_TILES(7, 1, 2, 1, 1, 3);
+  }
+#undef SD_TILES
 }
 
 template <typename T, bool GATED> int launch(Args a, hipStream_t st) {
   const Plan pl = make_plan(a.M, a.N, a.K, GATED);
   if (pl.XT) {
-    const int cols = GATED ? 16 : 16 * pl.NT;
+    const int cols = GATED ? 8 : 16;
     const dim3 grid(static_cast<unsigned>((a.N + cols - 1) / cols)), block(pl.W * 64);
-    const size_t lds = static_cast<size_t>(pl.W) * pl.NT * pl.XT * 1024;
-    constexpr int NT = GATED ? 2 : 1;
-    if (pl.XT == 1) hipLaunchKernelGGL((w8a8_rows<T, 1, NT, GATED>), grid, block, lds, st, a);
-    else hipLaunchKernelGGL((w8a8_rows<T, 2, NT, GATED>), grid, block, lds, st, a);
+    const size_t lds = static_cast<size_t>(pl.W) * pl.XT * 1024;
+    if (pl.XT == 1) hipLaunchKernelGGL((w8a8_rows<T, 1, GATED>), grid, block, lds, st, a);
+    else hipLaunchKernelGGL((w8a8_rows<T, 2, GATED>), grid, block, lds, st, a);
     return sd::check_launch("w8a8");
   }
-  const int bo = GATED ? pl.bn / 2 : pl.bn;
+  const Tile& t = kTiles[pl.tile];
+  const int bo = GATED ? t.bn / 2 : t.bn;
   a.slices = a.part ? pl.slices : 1;  // without its workspace: one slice
-  a.tiles_m = static_cast<int32_t>((a.M + pl.bm - 1) / pl.bm);
+  a.tiles_m = static_cast<int32_t>((a.M + t.bm - 1) / t.bm);
   a.tiles_n = static_cast<int32_t>((a.N + bo - 1) / bo);
-  const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.tiles_m) * a.tiles_n * a.slices)), block(256);
-  if (pl.bm == 256) hipLaunchKernelGGL((w8a8_gemm<T, 2, 2, 4, 4, 2, GATED>), grid, block, 0, st, a);
-  else if (pl.bm == 128) hipLaunchKernelGGL((w8a8_gemm<T, 2, 2, 2, 2, 3, GATED>), grid, block, 0, st, a);
-  else if constexpr (GATED) hipLaunchKernelGGL((w8a8_gemm<T, 2, 1, 1, 2, 4, GATED>), grid, dim3(128), 0, st, a);
-  else hipLaunchKernelGGL((w8a8_gemm<T, 2, 2, 1, 1, 4, GATED>), grid, block, 0, st, a);
+  launch_tiles<T, GATED>(a, pl.tile, st);
   const int rc = sd::check_launch("w8a8");
   if (rc != SD_OK || a.slices == 1) return rc;
-  int64_t wgs = (a.M * a.N + 255) / 256;
+  const int64_t v = a.N % 4 == 0 ? 4 : 1;
+  int64_t wgs = (a.M * a.N / v + 255) / 256;
   if (wgs > 2048) wgs = 2048;
-  hipLaunchKernelGGL((w8a8_reduce<T, GATED>), dim3(static_cast<unsigned>(wgs)), dim3(256), 0, st, a);
+  const dim3 grid(static_cast<unsigned>(wgs)), block(256);
+  if (v == 4) hipLaunchKernelGGL((w8a8_reduce<T, GATED, 4>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((w8a8_reduce<T, GATED, 1>), grid, block, 0, st, a);
   return sd::check_launch("w8a8");
 }
 
-// (a launch takes fewer than 2^32 threads: tiles of 64 x 64 and 256 threads while they are few, of 256 x 256 then)
+// (a launch takes fewer than 2^32 threads; no tile has more than 512 for 64 x 128 weight rows)
 bool sizes_ok(int64_t M, int64_t N, int64_t K) {
   return M <= (1ll << 24) && N <= (1ll << 21) && K < (1ll << 17) &&
-         ((M + 255) / 256) * ((N + 127) / 128) < (1ll << 22);
+         ((M + 63) / 64) * ((N + 63) / 64) < (1ll << 22);
 }
 
 size_t workspace(int64_t M, int64_t N, int64_t K, bool gated) {
@@ -552,8 +658,9 @@ extern "C" size_t sd_w8a8_workspace_size(int64_t M, int64_t N, int64_t K, int32_
 extern "C" int64_t sd_w8a8_plan(int64_t M, int64_t N, int64_t K, int32_t gated) {
   if (M <= 0 || N <= 0 || K <= 0 || K % 16 != 0 || !sizes_ok(M, N, K)) return 0;
   const Plan pl = make_plan(M, N, K, gated != 0);
-  if (pl.XT) return pl.W | 16 * pl.NT << 8;
-  return pl.slices | pl.bn << 8 | static_cast<int64_t>(pl.bm) << 20;
+  if (pl.XT) return pl.W | 16 << 8;
+  const Tile& t = kTiles[pl.tile];
+  return pl.slices | t.bn << 8 | static_cast<int64_t>(t.bm) << 20 | static_cast<int64_t>(t.per_cu) << 32;
 }
 
 extern "C" int sd_w8a8_linear(const int8_t* x, int64_t x_stride_m, const float* x_scale, const int8_t* w,

@@ -3,8 +3,8 @@
 The sums are exact and the three fp32 products and the bias are single operations in a fixed order, so the linear
 equals the oracle's fp32 arithmetic bit for bit. With SiLU, gate and up are those same fp32 values (held against 64
 bits the bound would have to be on |sum| + |bias|, which may cancel to a small gate: dg <= 2^-24 (3 |g - b| + |g|), as
-large as g itself); what is left is the exponential, 2 ulp (2^-22), and its sum, quotient and product, a rounding each:
-2^-24 (4 + 3), and the output's own half step or least value.
+large as g itself); what is left is the exponential of -|gate|, 2 ulp (2^-22), its product with the gate, its sum, the quotient and the
+product with up, a rounding each: 2^-24 (4 + 4), and the output's own half step or least value.
 """
 import numpy as np
 import pytest
@@ -41,7 +41,7 @@ def near(got, x, xs, w, ws, b, kind):
     y = o8.linear32(to_np(x), to_np(xs), to_np(w), to_np(ws.float()), None if b is None else to_np(b.float()))
     want = o8.silu_up(y.astype(np.float64))
     tiny = float(torch.finfo(DTYPES[kind]).tiny) * float(torch.finfo(DTYPES[kind]).eps)
-    tol = np.abs(want) * (float(torch.finfo(DTYPES[kind]).eps) / 2 + 2.0**-24 * 7) + tiny
+    tol = np.abs(want) * (float(torch.finfo(DTYPES[kind]).eps) / 2 + 2.0**-24 * 8) + tiny
     off = np.abs(to_np(got).astype(np.float64) - want)
     assert got.dtype == DTYPES[kind] and got.shape == want.shape
     assert (off <= tol).all(), f"off by {off.max():.3g} where {tol[off > tol].max():.3g} is allowed"
@@ -69,6 +69,35 @@ def test_tiles_and_slices(m, n, k):
     x, xs, w, ws, b = make(m, n, k)
     equal(ops.w8a8_linear(x, xs, w, ws, b), x, xs, w, ws, b, "bf16")
     near(ops.w8a8_gate_up_silu(x, xs, w, ws, b), x, xs, w, ws, b, "bf16")
+
+
+# (gated, rows, outputs, K, (tile rows, weight rows, workgroups a compute unit), in slices)
+ROUTES = [
+    (0, 40, 34, 144, (32, 64, 4), False), (0, 20, 34, 4112, (32, 64, 4), True), (0, 3000, 514, 144, (64, 128, 2), False),
+    (0, 900, 130, 9744, (64, 128, 2), True), (0, 500, 4100, 2064, (128, 128, 1), False),
+    (0, 130, 12000, 144, (128, 128, 2), False), (0, 400, 12000, 4112, (128, 256, 1), False),
+    (0, 500, 8200, 2064, (192, 128, 1), False), (0, 130, 12000, 9744, (192, 128, 1), True),
+    (0, 900, 8200, 1040, (192, 256, 1), False), (0, 1000, 12000, 2064, (256, 256, 1), False),
+    (1, 40, 34, 144, (32, 64, 4), False), (1, 20, 34, 4112, (32, 64, 4), True), (1, 1500, 514, 144, (64, 128, 2), False),
+    (1, 1500, 34, 9744, (64, 128, 2), True), (1, 100, 8200, 2064, (128, 128, 1), False),
+    (1, 70, 8200, 144, (128, 128, 2), False), (1, 200, 8200, 4112, (128, 256, 1), False),
+    (1, 130, 12000, 1040, (192, 128, 1), False), (1, 130, 6000, 9744, (192, 128, 1), True),
+    (1, 900, 4100, 1040, (192, 256, 1), False), (1, 400, 12000, 2064, (256, 256, 1), False),
+]
+
+
+@pytest.mark.parametrize("gated,m,n,k,tile,sliced", ROUTES)
+def test_every_tile(gated, m, n, k, tile, sliced):
+    """Every tile, in slices too, at shapes that end inside it; K ends inside a step. Odd N: rows that start anywhere."""
+    plan = _lib.load().sd_w8a8_plan(m, n, k, gated)
+    if torch.cuda.get_device_properties(0).multi_processor_count == 256:
+        assert ((plan >> 20) & 4095, (plan >> 8) & 4095, plan >> 32) == tile and (plan & 255 > 1) == sliced
+    for cols in (n, n - 1):
+        x, xs, w, ws, b = make(m, cols * (1 + gated), k)
+        if gated:
+            near(ops.w8a8_gate_up_silu(x, xs, w, ws, b), x, xs, w, ws, b, "bf16")
+        else:
+            equal(ops.w8a8_linear(x, xs, w, ws, b), x, xs, w, ws, b, "bf16")
 
 
 @pytest.mark.parametrize("scale_kind", ["bf16", "fp16", "fp32"])
@@ -102,7 +131,7 @@ def test_rows_do_not_depend_on_the_call():
         routes.add(_lib.load().sd_w8a8_plan(m, 1040, 2064, 0))
         assert torch.equal(ops.w8a8_linear(x[:m], xs[:m], w, ws, b), all_rows[:m])
         assert torch.equal(ops.w8a8_gate_up_silu(x[:m], xs[:m], w, ws, b), gated[:m])
-    assert len(routes) > 2
+    assert len(routes) > 1
 
 
 @pytest.mark.parametrize("m", [1, 20, 70])

@@ -772,8 +772,8 @@ int sd_dequantize_rows_int8(const int8_t* codes, int64_t codes_stride, const flo
  *   y       : (M, N) dtype (bf16/f16), row stride y_stride_m (>= N), sharing no byte with
  *             x, x_scale or w
  * K is a multiple of 16 below 2^17: the integer sums are exact (any codes, -128 too).
- * Three fp32 products and one rounding follow; a row's outputs are the same bits
- * whatever M. x_stride_m and w_stride_n <= 2^23 where there is more than one row.
+ * sum * scale in fp32, times x_scale plus bias in one fp32 step, and the rounding
+ * follow; a row's outputs are the same bits whatever M. x_stride_m and w_stride_n <= 2^23 where there is more than one row.
  * workspace: sd_w8a8_workspace_size bytes on the same device, 16-byte aligned (sums of
  * K slices; 0 where one slice runs). Without it (NULL or too small) the call runs in
  * one slice. `gated`: the query is for sd_w8a8_gate_up_silu.
@@ -794,7 +794,8 @@ int sd_w8a8_linear(const int8_t* x, int64_t x_stride_m, const float* x_scale, co
 /*
  * The gated projections of an MLP: w (2 N, K) = [gate; up], scale and bias (2 N,),
  *   y[m, n] = silu(g[m, n]) * u[m, n]
- * with g and u the linear's outputs before their rounding; otherwise as sd_w8a8_linear.
+ * with g and u the linear's outputs before their rounding (0 for g below -87, where silu
+ * is less than 2^-119); otherwise as sd_w8a8_linear.
  */
 int sd_w8a8_gate_up_silu(const int8_t* x, int64_t x_stride_m, const float* x_scale,
                          const int8_t* w, int64_t w_stride_n, const void* scale,

@@ -1,8 +1,8 @@
 """Oracle of the 8-bit activations and the integer linears (numpy).
 
 16-bit inputs arrive as float32 arrays of their exact values. The codes follow from fp32 v and max |v| by one exact
-quotient, so they are compared for equality; scales and outputs in 64 bits, the linear's also by its own three fp32
-products."""
+quotient, so they are compared for equality; scales and outputs in 64 bits, the linear's also by its own fp32
+steps."""
 from __future__ import annotations
 
 import numpy as np
@@ -38,9 +38,11 @@ def _sums(x, w):
 
 
 def linear32(x, x_scale, w, scale, bias=None):
-    """The operator's own arithmetic: exact integer sums, then fp32 products in its order. float32, unrounded."""
-    y = _sums(x, w).astype(np.float32) * scale.astype(np.float32)[None] * x_scale.astype(np.float32)[:, None]
-    return y if bias is None else y + bias.astype(np.float32)[None]
+    """The operator's own arithmetic: exact integer sums, times scale in fp32, then times x_scale plus bias with one
+    rounding to fp32 (through 64 bits of mantissa). float32, not rounded to the output's type."""
+    y = _sums(x, w).astype(np.float32) * scale.astype(np.float32)[None]
+    y = y.astype(np.longdouble) * x_scale.astype(np.longdouble)[:, None]
+    return (y if bias is None else y + bias.astype(np.longdouble)[None]).astype(np.float32)
 
 
 def linear64(x, x_scale, w, scale, bias=None):

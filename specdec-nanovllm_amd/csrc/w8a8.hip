@@ -3,7 +3,7 @@
 //   y[m, n] = (sum_k x[m, k] w[n, k]) ws[n] xs[m] (+ bias[n])
 //   h[m, i] = silu(y[m, i]) y[m, I + i], unrounded y          (gate_up_silu; w has 2 I rows)
 //
-// The sums are exact in 32 bits (K < 2^17), and every route ends in the same three fp32 products: a row's outputs
+// The sums are exact in 32 bits (K < 2^17), and every route ends in the same fp32 steps: a row's outputs
 // are the same bits whatever the other rows, tiles or K slices of the call.
 // The MFMAs take the weights as their rows, so that a lane holds neighbouring outputs of one token.
 //
@@ -44,17 +44,17 @@ __device__ __forceinline__ float scale_at(const Args& a, int64_t n) {
   return a.scale_dtype == SD_F16 ? sd::from_bits<_Float16>(b) : sd::from_bits<__bf16>(b);
 }
 
-// What every route makes of a sum.
-__device__ __forceinline__ float output(int32_t sum, float ws, float xs, bool has_bias, float bias) {
-#pragma clang fp contract(off)
-  const float y = static_cast<float>(sum) * ws * xs;
-  return has_bias ? y + bias : y;
+// What every route makes of a sum: sum ws, rounded, then its product with xs and the bias (0 without one) in one step.
+__device__ __forceinline__ float output(int32_t sum, float ws, float xs, float bias) {
+  return __builtin_fmaf(static_cast<float>(sum) * ws, xs, bias);
 }
-// silu(gate) up by the exponential of -|gate|: that of -gate overflows from -89 down, where the result is still 1e-37.
+// silu(gate) up on the transcendental unit: the exponent's rounding moves the exponential by |gate| 2^-24, v_exp_f32 and
+// v_rcp_f32 by one unit each, far below the output's half step. Below gate = -87, where silu(gate) is less than 2^-119, 0.
+// (With expf and a division the epilogue of a 256 x 256 tile took 9 us, a third of its time.)
 __device__ __forceinline__ float silu_up(float gate, float up) {
 #pragma clang fp contract(off)
-  const float e = expf(-fabsf(gate));
-  return (gate < 0.f ? gate * e : gate) / (1.f + e) * up;
+  const float e = __builtin_amdgcn_exp2f(gate * -1.442695041f);
+  return gate * __builtin_amdgcn_rcpf(1.f + e) * up;
 }
 
 __device__ __forceinline__ i32x4 mfma16(u32x4 a, u32x4 b, i32x4 c) {
@@ -139,7 +139,7 @@ __global__ __launch_bounds__(512) void w8a8_rows(Args a) {
     auto value = [&](int row, int64_t at) {
       int32_t v = 0;
       for (int u = 0; u < W; ++u) v += red[(u * XT * 16 + m) * 16 + row];
-      return output(v, scale_at(a, at), xs, bias, bias ? sd::from_bits<T>(a.bias[at]) : 0.f);
+      return output(v, scale_at(a, at), xs, bias ? sd::from_bits<T>(a.bias[at]) : 0.f);
     };
     const float y = value(c, out);
     a.y[m * a.ys + out] = sd::to_bits<T>(GATED ? silu_up(y, value(8 + c, a.N + out)) : y);
@@ -350,7 +350,6 @@ __global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(WM
   }
   // ---- a lane's neighbouring outputs of a token and tile, through LDS to whole lines
   __syncthreads();
-  const bool has_bias = a.bias != nullptr;
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
 #pragma unroll
@@ -368,9 +367,8 @@ __global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(WM
           for (int q = 0; q < 2; ++q) {
             const auto z = __builtin_amdgcn_permlane32_swap(static_cast<uint32_t>(acc[i][t][e + q]),
                                                             static_cast<uint32_t>(acc[i][t][e + q + 8]), false, false);
-            const float g = output(static_cast<int32_t>(z[0]), lws[at_w + e + q], xs, has_bias, lbias[at_w + e + q]);
-            const float u = output(static_cast<int32_t>(z[1]), lws[at_w + 16 + e + q], xs, has_bias,
-                                   lbias[at_w + 16 + e + q]);
+            const float g = output(static_cast<int32_t>(z[0]), lws[at_w + e + q], xs, lbias[at_w + e + q]);
+            const float u = output(static_cast<int32_t>(z[1]), lws[at_w + 16 + e + q], xs, lbias[at_w + 16 + e + q]);
             v[q] = silu_up(g, u);
           }
           o[e / 2] = sd::pack2<T>(v[0], v[1]);
@@ -381,8 +379,8 @@ __global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(WM
         uint32_t o[8];
 #pragma unroll
         for (int e = 0; e < 16; e += 2)
-          o[e / 2] = sd::pack2<T>(output(acc[i][t][e], lws[at_w + e], xs, has_bias, lbias[at_w + e]),
-                                  output(acc[i][t][e + 1], lws[at_w + e + 1], xs, has_bias, lbias[at_w + e + 1]));
+          o[e / 2] = sd::pack2<T>(output(acc[i][t][e], lws[at_w + e], xs, lbias[at_w + e]),
+                                  output(acc[i][t][e + 1], lws[at_w + e + 1], xs, lbias[at_w + e + 1]));
         uint8_t* const p = sm + r * kPitch + at_w * 2;
         sd::store16(p, u32x4{o[0], o[1], o[2], o[3]});
         sd::store16(p + 16, u32x4{o[4], o[5], o[6], o[7]});
@@ -444,7 +442,7 @@ template <typename T, bool GATED, int V> __global__ __launch_bounds__(256) void 
       }
 #pragma unroll
       for (int e = 0; e < V; ++e)
-        out[h][e] = output(sum[e], scale_at(a, c + e), xs, has_bias, has_bias ? sd::from_bits<T>(a.bias[c + e]) : 0.f);
+        out[h][e] = output(sum[e], scale_at(a, c + e), xs, has_bias ? sd::from_bits<T>(a.bias[c + e]) : 0.f);
     }
     uint16_t* const y = a.y + m * a.ys + n;
 #pragma unroll

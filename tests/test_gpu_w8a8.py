@@ -1,10 +1,11 @@
 """The linears in 8-bit integers (csrc/w8a8.hip through ``ops``) against the oracle.
 
-The sums are exact and the three fp32 products and the bias are single operations in a fixed order, so the linear
-equals the oracle's fp32 arithmetic bit for bit. With SiLU, gate and up are those same fp32 values (held against 64
-bits the bound would have to be on |sum| + |bias|, which may cancel to a small gate: dg <= 2^-24 (3 |g - b| + |g|), as
-large as g itself); what is left is the exponential of -|gate|, 2 ulp (2^-22), its product with the gate, its sum, the quotient and the
-product with up, a rounding each: 2^-24 (4 + 4), and the output's own half step or least value.
+The sums are exact and the fp32 steps single operations in a fixed order, so the linear equals the oracle's fp32
+arithmetic bit for bit. With SiLU, gate and up are those same fp32 values; what is left is exp2(-gate log2(e)): the
+product's rounding, |gate| log2(e) 2^-24, and the constant's, 2^-26 of the same, in the exponent, (1 + 1/4) |gate| 2^-24
+of the exponential, and one unit, 2^-23, of v_exp_f32; the sum's rounding, one unit of v_rcp_f32, two products:
+2^-24 (1.25 |gate| + 2 + 1 + 2 + 2), and the output's own half step or least value. Where the reciprocal is less than
+2^-126 it may be 0: |gate up| 2^-126.
 """
 import numpy as np
 import pytest
@@ -39,9 +40,10 @@ def equal(got, x, xs, w, ws, b, kind):
 
 def near(got, x, xs, w, ws, b, kind):
     y = o8.linear32(to_np(x), to_np(xs), to_np(w), to_np(ws.float()), None if b is None else to_np(b.float()))
+    gate, up = (np.abs(t) for t in np.split(y.astype(np.float64), 2, axis=-1))
     want = o8.silu_up(y.astype(np.float64))
     tiny = float(torch.finfo(DTYPES[kind]).tiny) * float(torch.finfo(DTYPES[kind]).eps)
-    tol = np.abs(want) * (float(torch.finfo(DTYPES[kind]).eps) / 2 + 2.0**-24 * 8) + tiny
+    tol = np.abs(want) * (float(torch.finfo(DTYPES[kind]).eps) / 2 + 2.0**-24 * (1.25 * gate + 7)) + tiny + gate * up * 2.0**-126
     off = np.abs(to_np(got).astype(np.float64) - want)
     assert got.dtype == DTYPES[kind] and got.shape == want.shape
     assert (off <= tol).all(), f"off by {off.max():.3g} where {tol[off > tol].max():.3g} is allowed"

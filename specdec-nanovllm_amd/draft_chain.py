@@ -38,17 +38,24 @@ slot write in one launch), attention and SiLU*mul, one launch each. ``fused`` ch
 nothing there: the linears have no 4-bit form with a norm or SiLU*mul in it, and the
 8-bit ones with a 4-bit cache run without.
 
+``act_bits=8`` holds the activations of every linear in 8 bits with a scale per token
+(int8 weights only): the norms write them, attention's output and the MLP's product are
+quantized by row, and the products are integer ones (``_layer_int8``), in the step and in
+the prefill of the context, which otherwise multiplies by dequantized weights. ``fused``
+changes nothing there either.
+
 ``chain()`` runs ``k`` steps back to back, each feeding its tokens to the next,
 on static buffers, so the whole chain can be captured in one HIP graph.
 """
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
 
 from . import ops
-from .layers.quant import quantize_weight, quantize_weight_int4
+from .layers.quant import int8_linear_a8, quantize_weight, quantize_weight_int4
 
 QWEN3_06B = dict(layers=28, hidden=1024, heads=16, kv_heads=8, head_dim=128, inter=3072,
                  vocab=151936, theta=1e6, eps=1e-6)
@@ -62,11 +69,16 @@ class DraftChain:
                  inter: int = 3072, vocab: int = 151936, theta: float = 1e6, eps: float = 1e-6,
                  block_size: int = 256, seed: int = 0, device="cuda",
                  dtype: torch.dtype = torch.bfloat16, fused: bool = False,
-                 context: str = "prefill", weight_bits: int = 8, kv_bits: int = 16):
+                 context: str = "prefill", weight_bits: int = 8, kv_bits: int = 16,
+                 act_bits: int = 16):
         if weight_bits not in (4, 8) or kv_bits not in (4, 16):
             raise ValueError(f"weights in 4 or 8 bits, cache in 4 or 16: got {weight_bits}, {kv_bits}")
-        self.weight_bits, self.kv_bits = weight_bits, kv_bits
+        if act_bits not in (8, 16) or (act_bits == 8 and weight_bits != 8):
+            raise ValueError(f"activations in 16 bits, or in 8 with weights in 8: got {act_bits}, {weight_bits}")
+        self.weight_bits, self.kv_bits, self.act_bits = weight_bits, kv_bits, act_bits
         self._linear = ops.w4a16_linear if weight_bits == 4 else ops.w8a16_linear
+        if act_bits == 8:
+            self._linear = functools.partial(int8_linear_a8, dtype=dtype)
         self.B, self.ctx_len, self.k = batch, ctx_len, k
         self.fused = fused
         self.L, self.H, self.Hq, self.Hkv, self.D = layers, hidden, heads, kv_heads, head_dim
@@ -159,6 +171,9 @@ class DraftChain:
         B, C, Hq, Hkv, D = self.B, self.ctx_len, self.Hq, self.Hkv, self.D
         if C == 0:
             return
+        if self.act_bits == 8:
+            self._prefill_int8(ids)
+            return
         from .layers.quant import dequantize_weight, dequantize_weight_int4
 
         dequantize = dequantize_weight_int4 if self.weight_bits == 4 else dequantize_weight
@@ -196,6 +211,27 @@ class DraftChain:
             h = lin(torch.nn.functional.silu(gate) * up, lw["down"])
             del q, kk, v, o, x, gate, up
 
+    def _prefill_int8(self, ids: torch.Tensor) -> None:
+        """The prefill with activations in 8 bits: the step's own operators over all rows."""
+        B, C, Hkv, D = self.B, self.ctx_len, self.Hkv, self.D
+        p = torch.arange(C, device=self.dev)
+        slots = (self.block_table.long()[:, p // self.bs] * self.bs + p % self.bs).reshape(-1).to(torch.int32)
+        pos = p.repeat(B)
+        cu = torch.arange(0, (B + 1) * C, C, dtype=torch.int32, device=self.dev)
+        h, residual = self.embed[ids.reshape(-1)], None
+        for li, lw in enumerate(self.layers):
+            def attend(q, kk, v):
+                if self.kv_bits == 4:
+                    q, kk = ops.qk_norm_rope_store_int4(q, kk, v, pos, self.cos_sin, *self.kv4[li], slots,
+                                                        lw["q_norm"], lw["k_norm"], self.eps)
+                    v = v.contiguous()  # strided as the new kk
+                else:
+                    ops.qk_norm_rope(q, kk, pos, self.cos_sin, lw["q_norm"], lw["k_norm"], self.eps, v=v,
+                                     k_cache=self.kv[0, li], v_cache=self.kv[1, li], slot_mapping=slots)
+                return ops.prefill_attention(q, kk, v, cu, cu, C, self.scale)
+
+            h, residual = self._layer_int8(lw, h, residual, attend)
+
     # ------------------------------------------------------------------ neighbours
     def _rms(self, x, w):
         xf = x.float()
@@ -216,6 +252,8 @@ class DraftChain:
     # ----------------------------------------------------------------------- step
     def step(self, s: int) -> torch.Tensor:
         """Draft step s: reads tokens[s], writes tokens[s + 1], returns the logits."""
+        if self.act_bits == 8:
+            return self._step_int8(s)
         if self.weight_bits == 4 or self.kv_bits == 4:
             return self._step_4bit(s)
         if self.fused:
@@ -321,6 +359,41 @@ class DraftChain:
         ops.sample(logits, out=self.tokens[s + 1])
         return logits
 
+    def _layer_int8(self, lw: dict, h: torch.Tensor, residual: torch.Tensor | None, attend):
+        """One layer with activations in 8 bits over the rows of ``h``; ``attend(q, k, v)`` appends and attends."""
+        Hq, Hkv, D, eps, dt = self.Hq, self.Hkv, self.D, self.eps, self.dtype
+        if residual is None:
+            residual, (x, xs) = h, ops.rmsnorm_int8(h, lw["in_norm"], eps)
+        else:
+            x, xs, residual = ops.rmsnorm_int8(h, lw["in_norm"], eps, residual)
+        qkv = ops.w8a8_linear(x, xs, *lw["qkv"], dtype=dt)
+        q, kk, v = (t.unflatten(-1, (-1, D)) for t in qkv.split([Hq * D, Hkv * D, Hkv * D], dim=-1))
+        o = attend(q, kk, v)
+        h = ops.w8a8_linear(*ops.quantize_rows_int8(o.reshape(-1, Hq * D)), *lw["o"], dtype=dt)
+        x, xs, residual = ops.rmsnorm_int8(h, lw["post_norm"], eps, residual)
+        act = ops.w8a8_gate_up_silu(x, xs, *lw["gate_up"], dtype=dt)
+        return ops.w8a8_linear(*ops.quantize_rows_int8(act), *lw["down"], dtype=dt), residual
+
+    def _step_int8(self, s: int) -> torch.Tensor:
+        pos, slots, ctx, eps = self.positions[s], self.slots[s], self.ctx[s], self.eps
+        h, residual = self.embed[self.tokens[s]], None
+        for li, lw in enumerate(self.layers):
+            def attend(q, kk, v):
+                if self.kv_bits == 4:
+                    q, _ = ops.qk_norm_rope_store_int4(q, kk, v, pos, self.cos_sin, *self.kv4[li], slots,
+                                                       lw["q_norm"], lw["k_norm"], eps, key_out=False)
+                    return ops.paged_attention_int4(q, *self.kv4[li], self.block_table, self.scale, context_lens=ctx)
+                ops.qk_norm_rope(q, kk, pos, self.cos_sin, lw["q_norm"], lw["k_norm"], eps, v=v,
+                                 k_cache=self.kv[0, li], v_cache=self.kv[1, li], slot_mapping=slots)
+                return ops.paged_attention(q, self.kv[0, li], self.kv[1, li], self.block_table, self.scale,
+                                           context_lens=ctx)
+
+            h, residual = self._layer_int8(lw, h, residual, attend)
+        x, xs, _ = ops.rmsnorm_int8(h, self.final_norm, eps, residual)
+        logits = ops.w8a8_linear(x, xs, *self.lm_head, dtype=self.dtype)
+        ops.sample(logits, out=self.tokens[s + 1])
+        return logits
+
     def chain(self) -> None:
         for s in range(self.k):
             self.step(s)
@@ -359,6 +432,8 @@ class DraftChain:
                 torch.randn((self.B, self.H), generator=g, device=self.dev).to(self.dtype),
                 torch.randn((self.B, self.Hq * self.D), generator=g, device=self.dev).to(self.dtype),
                 torch.randn((self.B, self.I), generator=g, device=self.dev).to(self.dtype))
+            if self.act_bits == 8:  # (codes, scale), as the norms leave them
+                self._act_static = tuple(ops.quantize_rows_int8(x) for x in self._act_static)
         xh, xo, xi = self._act_static
         for _ in range(self.k):
             for lw in self.layers:

@@ -1,7 +1,8 @@
 """``RMSNorm`` with the reference's interface (nanovllm/layers/layernorm.py:6-47)
 on the HIP kernel ``sd_rmsnorm``: ``forward(x)`` is the plain norm,
 ``forward(x, residual)`` the fused residual add + norm returning
-``(normed, new_residual)``; fp32 arithmetic with the module's bf16 roundings."""
+``(normed, new_residual)``; fp32 arithmetic with the module's bf16 roundings.
+``forward_int8`` gives the norm in 8 bits for a linear with ``quant_act_bits = 8``."""
 from __future__ import annotations
 
 import torch
@@ -21,3 +22,8 @@ class RMSNorm(nn.Module):
         if residual is None:
             return ops.rmsnorm(x, self.weight, self.eps)
         return ops.rmsnorm(x, self.weight, self.eps, residual=residual)
+
+    def forward_int8(self, x: torch.Tensor, residual: torch.Tensor | None = None):
+        """(codes, scale) of the unrounded norm, with ``residual`` ((codes, scale), new_residual)."""
+        codes, scale, *new = ops.rmsnorm_int8(x, self.weight, self.eps, residual)
+        return ((codes, scale), new[0]) if new else (codes, scale)

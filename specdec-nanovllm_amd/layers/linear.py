@@ -3,8 +3,11 @@
 ``LinearBase._apply(x, bias)`` is the one call site of the W8A16 path in the
 reference (linear.py:40-45): an int8 ``weight`` goes to ``int8_linear`` with
 the module's ``weight_scale``/``quant_granularity``/``quant_group_size``, a
-packed 4-bit ``weight`` (uint8) to ``int4_linear``, anything else to ``F.linear``. Tensor-parallel sharding and its all-reduce are
-not part of this single-GPU library (tp_size is 1).
+packed 4-bit ``weight`` (uint8) to ``int4_linear``, anything else to ``F.linear``.
+An int8 module whose ``quant_act_bits`` is 8 (``apply_int8_activations``) goes to
+``int8_linear_a8`` and also takes (codes, scale), activations that are quantized
+already. Tensor-parallel sharding and its all-reduce are not part of this
+single-GPU library (tp_size is 1).
 
 ``nn.Module`` already uses the name ``_apply(fn)`` for ``.to()``/``.cuda()``;
 the reference overrides it with the linear dispatch, which breaks those calls.
@@ -17,7 +20,7 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
-from .quant import int4_linear, int8_linear
+from .quant import int4_linear, int8_linear, int8_linear_a8
 
 
 class LinearBase(nn.Module):
@@ -30,6 +33,7 @@ class LinearBase(nn.Module):
         self.tp_size = 1
         self.quant_granularity = "per_channel"
         self.quant_group_size = 128
+        self.quant_act_bits = 16
         self.weight = nn.Parameter(torch.empty(output_size, input_size))
         if bias:
             self.bias = nn.Parameter(torch.empty(output_size))
@@ -39,6 +43,10 @@ class LinearBase(nn.Module):
     def _apply(self, x, bias=None, *args, **kwargs):
         if callable(x) and not isinstance(x, torch.Tensor):
             return super()._apply(x, *(() if bias is None else (bias,)), *args, **kwargs)
+        if self.weight.dtype == torch.int8 and self.quant_act_bits == 8:
+            return int8_linear_a8(x, self.weight, self.weight_scale, bias)
+        if isinstance(x, tuple):
+            raise TypeError("activations in 8 bits need a module with quant_act_bits = 8 (apply_int8_activations)")
         if self.weight.dtype == torch.int8:
             return int8_linear(x, self.weight, self.weight_scale, bias,
                                self.quant_granularity, self.quant_group_size)

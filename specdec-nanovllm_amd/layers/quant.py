@@ -13,6 +13,9 @@
   (quant.py:31-63).
 * ``apply_int8_quant`` — in-place swap of named linear layers to int8
   (quant.py:66-117).
+* ``int8_linear_a8`` / ``apply_int8_activations`` — the same int8 weights with the
+  activations in 8 bits as well (W8A8, a scale per token: integer products; the
+  reference has no 8-bit activations).
 * ``quantize_weight_int4`` / ``dequantize_weight_int4`` / ``int4_linear`` /
   ``apply_int4_quant`` — the same with 4-bit weights and group scales (W4A16; the
   reference has no 4-bit weights).
@@ -112,6 +115,21 @@ def int8_linear(x: torch.Tensor, qweight: torch.Tensor, scale: torch.Tensor,
     return ops.w8a16_linear(x, qweight, scale, bias, gs)
 
 
+def int8_linear_a8(x, qweight: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor | None = None,
+                   dtype: torch.dtype | None = None):
+    """``int8_linear`` (per channel) with the activations in 8 bits: exact integer sums, then
+    the scales of token and channel.
+
+    x: [..., K] bf16/fp16, quantized here by row, or the (codes, scale) of
+    ``ops.rmsnorm_int8`` or ``ops.quantize_rows_int8``. The result's type is x's, or
+    ``dtype`` (bf16 where neither says). K a multiple of 16.
+    """
+    if not isinstance(x, tuple):
+        dtype = dtype or x.dtype
+        x = ops.quantize_rows_int8(x)
+    return ops.w8a8_linear(*x, qweight, scale, bias, dtype or torch.bfloat16)
+
+
 def quantize_weight_int4(w: torch.Tensor, group_size: int = 128):
     """Symmetric 4-bit quantization of a 2-D weight ``[N, K]`` in groups of ``group_size`` columns (a
     multiple of 32 that divides K), on the weight's device.
@@ -190,8 +208,8 @@ def _swap_to_int4(name: str, mod: nn.Module, group_size: int) -> dict:
                 bytes_after=q.numel() + 2 * s.numel())
 
 
-def _chosen_modules(model: nn.Module, module_names) -> list:
-    """The named ``LinearBase`` submodules with bf16 weights; every name is checked first."""
+def _chosen_modules(model: nn.Module, module_names, dtype: torch.dtype = torch.bfloat16) -> list:
+    """The named ``LinearBase`` submodules with bf16 weights (``dtype``); every name is checked first."""
     from .linear import LinearBase
 
     wanted = set(module_names)
@@ -202,8 +220,8 @@ def _chosen_modules(model: nn.Module, module_names) -> list:
     for name, mod in chosen:
         if not isinstance(mod, LinearBase):
             raise TypeError(f"{name} is a {type(mod).__name__}, not a LinearBase")
-        assert mod.weight.dtype == torch.bfloat16, \
-            f"{name}: weight dtype {mod.weight.dtype} is not bf16"
+        assert mod.weight.dtype == dtype, \
+            f"{name}: weight dtype {mod.weight.dtype} is not {'bf16' if dtype == torch.bfloat16 else dtype}"
     return chosen
 
 
@@ -219,8 +237,31 @@ def apply_int4_quant(model: nn.Module, module_names, group_size: int = 128):
     return [_swap_to_int4(name, mod, group_size) for name, mod in chosen]
 
 
+def _check_act8(name: str, granularity: str, columns: int) -> None:
+    if granularity != "per_channel":
+        raise ValueError(f"{name}: activations in 8 bits need per-channel weight scales, got {granularity}")
+    if columns % 16:
+        raise ValueError(f"{name}: activations in 8 bits need a multiple of 16 columns, got {columns}")
+
+
+def apply_int8_activations(model: nn.Module, module_names, act_bits: int = 8) -> None:
+    """Let the named ``LinearBase`` submodules, whose weights are int8 per channel already
+    (``apply_int8_quant``, or a converted checkpoint's), take their activations in 8 bits:
+    ``LinearBase._apply`` then calls ``int8_linear_a8``, which also accepts (codes, scale)
+    from ``RMSNorm.forward_int8``. ``act_bits=16`` goes back. Same errors as
+    ``apply_int8_quant``, ``ValueError`` for groups or a K that is no multiple of 16;
+    every module is checked before any is changed."""
+    if act_bits not in (8, 16):
+        raise ValueError(f"activations in 8 or 16 bits, got {act_bits}")
+    chosen = _chosen_modules(model, module_names, torch.int8)
+    for name, mod in chosen:
+        _check_act8(name, mod.quant_granularity, mod.weight.shape[1])
+    for _, mod in chosen:
+        mod.quant_act_bits = act_bits
+
+
 def apply_int8_quant(model: nn.Module, module_names, granularity: str = "per_channel",
-                     group_size: int = 128, verbose: bool = False):
+                     group_size: int = 128, verbose: bool = False, act_bits: int = 16):
     """Quantize the named ``LinearBase`` submodules of ``model`` in place
     (the contract of nanovllm/layers/quant.py:66-117).
 
@@ -233,9 +274,18 @@ def apply_int8_quant(model: nn.Module, module_names, granularity: str = "per_cha
     the model lacks, ``TypeError`` for a module that is not a ``LinearBase``,
     ``AssertionError`` for a weight that is not bf16. Every module is checked
     before any is changed, so a refused call leaves the model as it was.
+    ``act_bits=8``: the activations in 8 bits as well, as ``apply_int8_activations``
+    (per channel only).
     """
     chosen = _chosen_modules(model, module_names)
+    if act_bits not in (8, 16):
+        raise ValueError(f"activations in 8 or 16 bits, got {act_bits}")
+    if act_bits == 8:
+        for name, mod in chosen:
+            _check_act8(name, granularity, mod.weight.shape[1])
     report = [_swap_to_int8(name, mod, granularity, group_size) for name, mod in chosen]
+    for _, mod in chosen:
+        mod.quant_act_bits = act_bits
     if verbose:
         for r in report:
             print(f"int8 {r['name']}: {r['shape'][0]}x{r['shape'][1]}, "

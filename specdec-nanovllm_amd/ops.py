@@ -809,15 +809,23 @@ def w4a16_linear(x: torch.Tensor, qweight: torch.Tensor, scale: torch.Tensor,
 
 
 # ------------------------------------------------------------------- 8-bit activations
-def _rows8(t: torch.Tensor) -> torch.Tensor:
-    """2-D (rows, width) view with a unit last stride and rows at 16-byte addresses; a copy where
-    they are not."""
-    t2 = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
-    s0, s1 = t2.stride()
-    if s1 != 1 or t2.data_ptr() % 16 or (t2.shape[0] > 1 and (s0 < 0 or s0 * t2.element_size() % 16)):
+def _rows8(t: torch.Tensor) -> tuple[torch.Tensor, int, int]:
+    """2-D (rows, width) view with a unit last stride and rows at 16-byte addresses, a copy where they are not;
+    with its row stride and address."""
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    s0, s1 = t.stride()
+    p = t.data_ptr()
+    if s1 != 1 or p % 16 or (s0 < 0 or s0 * t.itemsize % 16) and t.shape[0] > 1:
         # (not contiguous(): a contiguous view may start anywhere, and stays where it is)
-        t2 = t2.clone(memory_format=torch.contiguous_format)
-    return t2
+        t = t.clone(memory_format=torch.contiguous_format)
+        s0, p = t.shape[1], t.data_ptr()
+    return t, s0, p
+
+
+def _like(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """An empty row-major tensor of ``t``'s shape (``empty_like`` takes 1 us less than ``empty``)."""
+    return torch.empty_like(t, dtype=dtype) if t.is_contiguous() else torch.empty(t.shape, dtype=dtype, device=t.device)
 
 
 def quantize_rows_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -825,16 +833,17 @@ def quantize_rows_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     (...,)), value = code * scale, scale = max|x| / 127 and code = round_half_even(127 x / max|x|).
     A row with a NaN or an infinity has scale NaN, a row of zeros scale 0. K a multiple of 16 up
     to 32768. (``quantize_int8`` makes weights: a bf16 scale, rounded after the codes.)"""
-    x2 = _rows8(x)
+    x2, x0, xp = _rows8(x)
     rows, K = x2.shape
     dev = _lib.require_device(x2)
-    codes = torch.empty((rows, K), dtype=torch.int8, device=dev)
+    codes = _like(x2, torch.int8)
     scale = torch.empty(rows, dtype=torch.float32, device=dev)
     with _lib.on_device(dev):
         rc = _lib.load().sd_quantize_rows_int8(
-            x2.data_ptr(), x2.stride(0), codes.data_ptr(), K, scale.data_ptr(), rows, K,
-            _lib.dtype_code(x.dtype), _lib.stream_ptr(dev))
-    _lib.check(rc)
+            xp, x0, codes.data_ptr(), K, scale.data_ptr(), rows, K, _lib.dtype_code(x2.dtype),
+            _lib.stream_ptr(dev))
+    if rc:
+        _lib.check(rc)
     return (codes, scale) if x.dim() == 2 else (codes.view(x.shape), scale.view(x.shape[:-1]))
 
 
@@ -843,28 +852,32 @@ def rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float,
     """``rmsnorm`` whose result goes to 8 bits as ``quantize_rows_int8``'s, without a rounding to 16
     bits on the way: returns (codes, scale), with ``residual`` (codes, scale, residual_out), where s =
     x + residual in fp32, residual_out = s rounded to the dtype and the codes are of the norm of s."""
-    x2 = _rows8(x)
+    x2, x0, xp = _rows8(x)
     rows, H = x2.shape
-    dt = x.dtype
+    dt = x2.dtype
     assert weight.shape == (H,), "weight must be (hidden,)"
     w = weight if weight.dtype == dt else weight.to(dt)
-    if not w.is_contiguous() or w.data_ptr() % 16:
+    wp = w.data_ptr()
+    if wp % 16 or not w.is_contiguous():
         w = w.clone(memory_format=torch.contiguous_format)
-    r2 = ro = None
+        wp = w.data_ptr()
+    r2 = ro = rp = rop = None
+    r0 = 0
     if residual is not None:
         assert residual.shape == x.shape and residual.dtype == dt
-        r2 = _rows8(residual)
+        r2, r0, rp = _rows8(residual)
     dev = _lib.require_device(x2, w, r2)
-    codes = torch.empty((rows, H), dtype=torch.int8, device=dev)
+    codes = _like(x2, torch.int8)
     scale = torch.empty(rows, dtype=torch.float32, device=dev)
     if r2 is not None:
-        ro = torch.empty((rows, H), dtype=dt, device=dev)
+        ro = _like(x2, dt)
+        rop = ro.data_ptr()
     with _lib.on_device(dev):
         rc = _lib.load().sd_rmsnorm_int8(
-            x2.data_ptr(), x2.stride(0), _ptr(r2), 0 if r2 is None else r2.stride(0), w.data_ptr(),
-            codes.data_ptr(), H, scale.data_ptr(), _ptr(ro), H, rows, H, eps, _lib.dtype_code(dt),
-            _lib.stream_ptr(dev))
-    _lib.check(rc)
+            xp, x0, rp, r0, wp, codes.data_ptr(), H, scale.data_ptr(), rop, H, rows, H, eps,
+            _lib.dtype_code(dt), _lib.stream_ptr(dev))
+    if rc:
+        _lib.check(rc)
     if x.dim() != 2:
         codes, scale = codes.view(x.shape), scale.view(x.shape[:-1])
         ro = None if ro is None else ro.view(x.shape)
@@ -876,61 +889,70 @@ def dequantize_rows_int8(codes: torch.Tensor, scale: torch.Tensor,
     """The values of 8-bit rows: codes (..., K) int8 times scale (...,) fp32, rounded to ``dtype``
     (bf16, fp16 or fp32). Per-channel int8 weights with their scale in fp32 too."""
     assert codes.dtype == torch.int8 and scale.dtype == torch.float32
-    assert scale.shape == codes.shape[:-1], f"one scale a row: {tuple(scale.shape)} for {tuple(codes.shape)}"
-    c2 = _rows8(codes)
-    s = _flat(scale, torch.float32)
+    shape = codes.shape
+    assert scale.shape == shape[:-1], f"one scale a row: {tuple(scale.shape)} for {tuple(shape)}"
+    c2, c0, cp = _rows8(codes)
+    s = scale if scale.is_contiguous() else scale.contiguous()
     rows, K = c2.shape
     dev = _lib.require_device(c2, s)
-    out = torch.empty((rows, K), dtype=dtype, device=dev)
+    out = _like(c2, dtype)
     with _lib.on_device(dev):
         rc = _lib.load().sd_dequantize_rows_int8(
-            c2.data_ptr(), c2.stride(0), s.data_ptr(), out.data_ptr(), K, rows, K,
-            _lib.dtype_code(dtype), _lib.stream_ptr(dev))
-    _lib.check(rc)
-    return out if codes.dim() == 2 else out.view(codes.shape)
+            cp, c0, s.data_ptr(), out.data_ptr(), K, rows, K, _lib.dtype_code(dtype),
+            _lib.stream_ptr(dev))
+    if rc:
+        _lib.check(rc)
+    return out if len(shape) == 2 else out.view(shape)
 
 
 # ----------------------------------------------------------------------------- w8a8
 def _w8a8(gated: bool, x, x_scale, qweight, scale, bias, dtype, out):
-    assert x.dtype == torch.int8 and qweight.dtype == torch.int8, \
-        f"x and qweight must be int8, got {x.dtype} and {qweight.dtype}"
+    assert x.dtype == qweight.dtype == torch.int8, f"x and qweight must be int8, got {x.dtype} and {qweight.dtype}"
     assert qweight.dim() == 2 and x_scale.dtype == torch.float32
     wrows, K = qweight.shape
-    assert not gated or wrows % 2 == 0, "qweight must be [gate; up]"
-    N = wrows // 2 if gated else wrows
-    assert x.shape[-1] == K, f"K mismatch: x {tuple(x.shape)} vs w {tuple(qweight.shape)}"
-    assert x_scale.shape == x.shape[:-1], f"one scale a row: {tuple(x_scale.shape)} for {tuple(x.shape)}"
+    N = wrows
+    if gated:
+        assert wrows % 2 == 0, "qweight must be [gate; up]"
+        N = wrows // 2
+    xshape = x.shape
+    assert xshape[-1] == K, f"K mismatch: x {tuple(xshape)} vs w {tuple(qweight.shape)}"
+    assert x_scale.shape == xshape[:-1], f"one scale a row: {tuple(x_scale.shape)} for {tuple(xshape)}"
     assert scale.numel() == wrows, "scale must have one entry per weight row"
-    x2, qw = _rows8(x), _rows8(qweight)
+    x2, x0, xp = _rows8(x)
+    qw, w0, wp = _rows8(qweight)
     M = x2.shape[0]
-    if M > 1 and x2.stride(0) > 1 << 23:
-        x2 = x2.clone(memory_format=torch.contiguous_format)
-    xs = _flat(x_scale, torch.float32)
-    sc = _flat(scale, scale.dtype)
+    if M > 1 and x0 > 1 << 23:
+        x2, x0 = x2.clone(memory_format=torch.contiguous_format), K
+        xp = x2.data_ptr()
+    xs = x_scale if x_scale.is_contiguous() else x_scale.contiguous()
+    sc = scale if scale.is_contiguous() else scale.contiguous()
     b = None
     if bias is not None:
         assert bias.shape == (wrows,), "bias must have one entry per weight row"
         b = _flat(bias, dtype)
     dev = _lib.require_device(x2, xs, qw, sc, b, out)
-    shape = (*x.shape[:-1], N)
     if out is None:
         y = torch.empty((M, N), device=dev, dtype=dtype)
+        y0 = N
     else:
+        shape = (*xshape[:-1], N)
         assert out.shape == shape, f"out must be {shape}, got {tuple(out.shape)}"
         y = out.view(M, N)
-        assert y.dtype == dtype and (N == 1 or y.stride(1) == 1)
+        y0, y1 = y.stride()
+        assert y.dtype == dtype and (N == 1 or y1 == 1)
     if M:
         lib = _lib.load()
         with _lib.on_device(dev):
-            # the plan (and so the workspace) depends on the device's compute units
-            ws_bytes = lib.sd_w8a8_workspace_size(M, N, K, gated)
-            ws = _workspace(ws_bytes, dev)
+            # the plan (and so the workspace) depends on the device's compute units; up to 4 rows there is none
+            # (the question takes 1 us)
+            ws_bytes = lib.sd_w8a8_workspace_size(M, N, K, gated) if M > 4 else 0
+            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
             rc = (lib.sd_w8a8_gate_up_silu if gated else lib.sd_w8a8_linear)(
-                x2.data_ptr(), x2.stride(0), xs.data_ptr(), qw.data_ptr(), qw.stride(0), sc.data_ptr(),
-                _lib.dtype_code(sc.dtype), _ptr(b), y.data_ptr(), y.stride(0), M, N, K,
-                _lib.dtype_code(dtype), _ptr(ws), ws_bytes, _lib.stream_ptr(dev))
-        _lib.check(rc)
-    return y if x.dim() == 2 else y.view(shape)
+                xp, x0, xs.data_ptr(), wp, w0, sc.data_ptr(), _lib.dtype_code(sc.dtype), _ptr(b), y.data_ptr(),
+                y0, M, N, K, _lib.dtype_code(dtype), _ptr(ws), ws_bytes, _lib.stream_ptr(dev))
+        if rc:
+            _lib.check(rc)
+    return y if len(xshape) == 2 else y.view(*xshape[:-1], N)
 
 
 def w8a8_linear(x: torch.Tensor, x_scale: torch.Tensor, qweight: torch.Tensor, scale: torch.Tensor,

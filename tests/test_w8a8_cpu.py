@@ -185,3 +185,41 @@ def test_oracle():
     assert o8.linear32(x, one, w, one).tolist() == [[17, -249], [39, -491]] == o8.linear64(x, one, w, one).tolist()
     assert o8.linear32(x, one * 2, w, one, one).tolist() == [[35, -497], [79, -981]]
     assert np.allclose(o8.silu_up(np.array([[0.0, 1.0, 5.0, 2.0]])), [[0, 2 / (1 + np.exp(-1))]])
+
+
+def test_layers_check_before_they_change():
+    from specdec_nanovllm_amd.draft_chain import DraftChain
+    from specdec_nanovllm_amd.layers.linear import ReplicatedLinear
+    from specdec_nanovllm_amd.layers.quant import apply_int8_activations, apply_int8_quant
+
+    m = torch.nn.ModuleDict(dict(a=ReplicatedLinear(64, 8), b=ReplicatedLinear(72, 8), c=torch.nn.Linear(64, 8)))
+    for p in m.parameters():
+        p.data = torch.zeros(p.shape, dtype=torch.bfloat16)
+    for names, kw, error in ((["a", "x"], {}, KeyError), (["a", "c"], {}, TypeError), (["a", "b"], {}, ValueError),
+                             (["a"], dict(granularity="per_group", group_size=64), ValueError)):
+        with pytest.raises(error):
+            apply_int8_quant(m, names, act_bits=8, **kw)
+    with pytest.raises(ValueError, match="8 or 16"):
+        apply_int8_quant(m, ["a"], act_bits=4)
+    assert m["a"].weight.dtype == torch.bfloat16 and m["a"].quant_act_bits == 16
+    with pytest.raises(AssertionError, match="int8"):
+        apply_int8_activations(m, ["a"])
+    for name, k in (("a", 64), ("b", 72)):
+        m[name].weight = torch.nn.Parameter(torch.zeros((8, k), dtype=torch.int8), requires_grad=False)
+        m[name].weight_scale = torch.nn.Parameter(torch.ones(8, dtype=torch.bfloat16), requires_grad=False)
+    with pytest.raises(ValueError, match="multiple of 16"):
+        apply_int8_activations(m, ["a", "b"])
+    assert m["a"].quant_act_bits == 16
+    with pytest.raises(ValueError, match="8 or 16"):
+        apply_int8_activations(m, ["a"], 4)
+    apply_int8_activations(m, ["a"])
+    assert m["a"].quant_act_bits == 8
+    x = torch.zeros((2, 64), dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="ROCm GPU"):  # dispatched to the integer linear, which has no CPU form
+        m["a"](x)
+    apply_int8_activations(m, ["a"], 16)
+    with pytest.raises(TypeError, match="quant_act_bits"):
+        m["a"]((x.to(torch.int8), torch.ones(2)))
+    for bits in (dict(act_bits=4), dict(act_bits=8, weight_bits=4)):
+        with pytest.raises(ValueError, match="8"):
+            DraftChain(1, device="cpu", **bits)

@@ -67,7 +67,7 @@ __device__ __forceinline__ i32x16 mfma32(u32x4 a, u32x4 b, i32x16 c) {
 // Up to 16 XT rows. A workgroup takes 16 weight rows (GATED: the gate's and the up rows of 8 outputs), its waves the
 // stages of 128 columns in turn, loaded straight to registers two stages ahead. The activations come from the caches,
 // as many bytes a lane as of weights, which is what bounds it for more rows or many weight rows: 16 x 19456 x 2560
-// takes 14.4 us here, 11.4 in tiles, 1 x 19456 x 2560 10.3 and 11.1. Registers decide how many loads a compute unit
+// takes 14.2 us here, 11.4 in tiles, 1 x 19456 x 2560 10.3 and 11.1. Registers decide how many loads a compute unit
 // has in flight: stages of 256 columns took 10.9 us there, three of them ahead 10.6, two tiles a wave 13.9;
 // nontemporal loads of the weights 13.5.
 constexpr int kStage = 128;
@@ -156,9 +156,13 @@ __device__ __forceinline__ uint32_t lds_addr(const void* l) {
 }
 
 // WM x WN waves of MT x NT tiles of 32 tokens x 32 weight rows; S stages of 128 columns in LDS, loaded S steps ahead.
-// A step is four MFMA depths of 32 columns; the operands of a depth are read while the one before multiplies. Before
-// the last depth the workgroup meets: the next stage has landed (its first operands are read at once) and this one
-// is read by all, so that its place takes the stage S steps on. The MFMAs never wait for a barrier's first reads.
+// A step is four MFMA depths of 32 columns, whose operands are read three depths ahead, since a small wave's MFMAs of
+// one depth (64 cycles for two tiles) take less time than its reads. After the first depth the workgroup meets: all
+// have read this stage, whose place takes the stage S steps on, and the next stage has landed and is read from here
+// on, so that no MFMA waits for the reads after a barrier. (777 x 2560 x 9728 in tiles of 128 x 128: 33.3 us; 38.1 with
+// operands one depth ahead, 36.2 with the freed stage loaded a step later and no wait for this step's reads, 36.2 with
+// K split between two groups of waves for a third fewer reads. Without any loads 33: waits of eight waves for each
+// other, not memory or LDS, bound that tile.)
 // LDS: 16-byte unit u of a row stands at u ^ turn, so that 16 rows' operand reads hit 16 different places of 256 bytes
 // (64 banks). MFMA row 8 a + 4 h + b reads weight row 16 h + 4 a + b of its tile: a lane (half h of the wave) then holds
 // sums of 16 neighbouring rows. GATED: rows 0 .. 15 of a tile are the gate's of 16 outputs, 16 .. 31 the up rows.
@@ -268,7 +272,7 @@ __global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(WM
     x_at[j] = wm * (MT * 32 * kBlock) + lr * kBlock + (((2 * j + lh) ^ x_turn(lr)) * 16);
     w_at[j] = kX + wn * (NT * 32 * kBlock) + wr * kBlock + (((2 * j + lh) ^ w_turn(wr)) * 16);
   }
-  u32x4 xf[2][MT], wf[2][NT];
+  u32x4 xf[kDepths][MT], wf[kDepths][NT];
   // The workgroup meets: all but the newest `stages` stages have landed in every wave's view, and every LDS read so far
   // is done.
   auto meet_at = [&](int stages) {
@@ -279,37 +283,44 @@ __global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(WM
     else SD_MEET(3);
 #undef SD_MEET
   };
+  constexpr int kAhead = kDepths - 1;  // depths that operands are read ahead
   meet_at(min(S, b1 - b0) - 1);
 #pragma unroll
-  for (int i = 0; i < MT; ++i) xf[0][i] = sd::load16(sm + x_at[0] + i * (32 * kBlock));
+  for (int j = 0; j < kAhead; ++j) {
 #pragma unroll
-  for (int t = 0; t < NT; ++t) wf[0][t] = sd::load16(sm + w_at[0] + t * (32 * kBlock));
+    for (int i = 0; i < MT; ++i) xf[j][i] = sd::load16(sm + x_at[j] + i * (32 * kBlock));
+#pragma unroll
+    for (int t = 0; t < NT; ++t) wf[j][t] = sd::load16(sm + w_at[j] + t * (32 * kBlock));
+  }
   int buf = 0;
   auto step = [&](int blk, auto middle) {  // middle: the stage S on is a whole one
     constexpr bool kMiddle = decltype(middle)::value;
+    constexpr int kMeet = kDepths - kAhead, kParts = MT * kAhead;  // the loads are spread over what follows the meeting
     const int next = buf + 1 == S ? 0 : buf + 1;
     const int left = a.K - blk * kBlock;
 #pragma unroll
     for (int j = 0; j < kDepths; ++j) {
-      const bool meet = j == kDepths - 1;
-      if (meet) meet_at(kMiddle ? S - 2 : min(S - 2, b1 - 2 - blk));
-      const uint8_t* const from = sm + (meet ? next : buf) * kBytes;
-      const int jn = (j + 1) % kDepths, now = j & 1, then = now ^ 1;
+      if (j == kMeet) meet_at(kMiddle ? S - 2 : min(S - 2, b1 - 2 - blk));
+      const uint8_t* const from = sm + (j >= kMeet ? next : buf) * kBytes;
+      const int then = (j + kAhead) % kDepths;
       if (!kMiddle && left < kBlock) {  // the last columns
         const bool none = 32 * j + 16 * lh >= left;
 #pragma unroll
         for (int t = 0; t < NT; ++t)
-          if (none) wf[now][t] = u32x4{0, 0, 0, 0};
+          if (none) wf[j][t] = u32x4{0, 0, 0, 0};
       }
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
-        xf[then][i] = sd::load16(from + x_at[jn] + i * (32 * kBlock));
+        xf[then][i] = sd::load16(from + x_at[then] + i * (32 * kBlock));
 #pragma unroll
         for (int t = i * NT / MT; t < (i + 1) * NT / MT; ++t)
-          wf[then][t] = sd::load16(from + w_at[jn] + t * (32 * kBlock));
-        if (meet && (kMiddle || blk + S < b1)) load(blk + S, buf, i * kLoads / MT, (i + 1) * kLoads / MT, middle);
+          wf[then][t] = sd::load16(from + w_at[then] + t * (32 * kBlock));
+        if (j >= kMeet && (kMiddle || blk + S < b1)) {
+          const int q = (j - kMeet) * MT + i;
+          load(blk + S, buf, q * kLoads / kParts, (q + 1) * kLoads / kParts, middle);
+        }
 #pragma unroll
-        for (int t = 0; t < NT; ++t) acc[i][t] = mfma32(wf[now][t], xf[now][i], acc[i][t]);
+        for (int t = 0; t < NT; ++t) acc[i][t] = mfma32(wf[j][t], xf[j][i], acc[i][t]);
         // one row of tiles after another: with the loads and reads all moved ahead of the MFMAs these wait for them
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -452,16 +463,16 @@ template <typename T, bool GATED, int V> __global__ __launch_bounds__(256) void 
 
 // The tiles there are, with what they were measured to take (us): a round of workgroups `start` + steps x `alone`
 // where each has a compute unit to itself, `full` a step where `per_cu` share it; and, since the whole device multiplies
-// only as fast as its power allows, every workgroup `power_start` + steps x `power` of the device.
+// only as fast as its power allows, a workgroup `power_start` + steps x `power` of the device.
 struct Tile {
   int bm, bn, per_cu;
   double start, alone, full, power_start, power;
 };
 constexpr Tile kTiles[] = {
-    {256, 256, 1, 10.4, 1.047, 1.047, 0.055, 0.0060}, {192, 256, 1, 7.7, 0.850, 0.850, 0.040, 0.0050},
-    {128, 256, 1, 6.8, 0.568, 0.568, 0.024, 0.0038},  {192, 128, 1, 5.0, 0.517, 0.517, 0.020, 0.0030},
-    {128, 128, 1, 4.4, 0.366, 0.366, 0.014, 0.0024},  {128, 128, 2, 2.4, 0.525, 0.825, 0.006, 0.0022},
-    {64, 128, 2, 2.9, 0.257, 0.504, 0.004, 0.0013},   {32, 64, 4, 2.7, 0.183, 0.357, 0.002, 0.0005},
+    {256, 256, 1, 6.0, 1.082, 1.082, 0.037, 0.0057}, {192, 256, 1, 3.9, 0.905, 0.905, 0.032, 0.0043},
+    {128, 256, 1, 5.2, 0.487, 0.487, 0.021, 0.0032}, {192, 128, 1, 4.1, 0.393, 0.393, 0.014, 0.0026},
+    {128, 128, 1, 3.6, 0.295, 0.295, 0.012, 0.0018}, {128, 128, 2, 2.3, 0.515, 0.632, 0.009, 0.0018},
+    {64, 128, 2, 2.3, 0.232, 0.528, 0.006, 0.0008},  {32, 64, 4, 2.3, 0.149, 0.422, 0.000, 0.0004},
 };
 
 // What runs a shape: w8a8_rows<XT> of W waves (XT > 0), or a tile and K slices.
@@ -473,33 +484,36 @@ Plan make_plan(int64_t M, int64_t N, int64_t K, bool gated) {
   Plan pl{};
   const int64_t cus = sd::device_cus();
   const int64_t wrows = gated ? 2 * N : N, groups = (wrows + 15) / 16, stages = (K + kStage - 1) / kStage;
-  // Few rows: up to 4 always (7 x 19456 x 2560 11.8 us there, 11.2 in tiles of 32 x 64; 16 14.4 and 11.4), up to 16
-  // where weight rows are few (16 x 6144 x 2560 6.8 and 7.6), up to 32 where they and the columns are (32 x 4096 x 1024
-  // 3.8 and 5.2, 32 x 2560 x 4096 7.7 and 8.9, 32 x 6144 x 2560 9.1 and 7.6, 32 x 2560 x 9728 16 and 11.2).
-  if (M <= 4 || (M <= 16 && groups <= 3 * cus) || (M <= 32 && groups <= cus && stages <= 32)) {
+  // Few rows: up to 4 always; more where weight rows are few, since every workgroup loads the activations anew (8 x 9000
+  // x 4096 11.7 us there, 11.2 in tiles of 32 x 64, 12 rows 12.9 and 11.2; 16 x 6144 x 2560 6.7 and 6.8, 16 x 2560 x
+  // 4096 6.0 and 8.3; 8 x 19456 x 2560 12.1 and 11.2), past 16 rows where the columns are few too (32 x 2560 x 4096 7.8
+  // and 8.5, 32 x 4096 x 1024 3.9 and 5.0; 32 x 6144 x 2560 9.0 and 6.8, 32 x 2560 x 9728 16 and 10.7).
+  if (M <= 4 || (M <= 8 && groups <= 3 * cus) || (M <= 16 && 2 * groups <= 3 * cus) ||
+      (M <= 32 && groups <= cus && stages <= 32)) {
     pl.XT = M <= 16 ? 1 : 2;
     // 8 waves, 4 for very many workgroups (1 x 151936 x 1024 24.5 us, 27.1 with 8)
     pl.W = groups > 16 * cus ? 4 : 8;
     if (pl.W > stages) pl.W = static_cast<int>(stages);
     return pl;
   }
-  // The tile and slices of the least time by the figures above (over 262 shapes 1.4% above the fastest of them on
-  // average). Slices cost a launch and their sums' way to memory and back.
+  // The tile and slices of the least time by the figures above (over 262 shapes of 17 to 4096 rows 0.6% above the
+  // fastest of them on average, 22% at worst). Slices cost a launch and their sums' way to memory and back.
   const int64_t blocks = (K + kBlock - 1) / kBlock;
   double least = 1e30;
   for (int i = 0; i < static_cast<int>(sizeof(kTiles) / sizeof(kTiles[0])); ++i) {
     const Tile& t = kTiles[i];
     const int64_t tiles = ((M + t.bm - 1) / t.bm) * ((wrows + t.bn - 1) / t.bn), slots = t.per_cu * cus;
+    const double more = t.per_cu > 1 ? (t.full - t.alone) / (t.per_cu - 1) : 0;
     for (int64_t s = 1; s == 1 || (s <= 16 && 4 * s <= blocks && tiles * s <= slots); ++s) {
-      const int64_t steps = (blocks + s - 1) / s, rounds = tiles * s / slots, rest = (tiles * s % slots + cus - 1) / cus;
-      const double more = t.per_cu > 1 ? (t.full - t.alone) / (t.per_cu - 1) : 0;
-      double round = static_cast<double>(rounds) * (t.start + steps * t.full);
-      if (rest) round += t.start + steps * (t.alone + more * (rest - 1));
-      const double power = static_cast<double>(tiles * s) * (t.power_start + steps * t.power);
-      // (neither alone: a smooth maximum, since rounds do not end together)
-      const double r2 = round * round, p2 = power * power, r6 = r2 * r2 * r2, p6 = p2 * p2 * p2;
-      double cost = __builtin_cbrt(__builtin_sqrt(r6 + p6));
-      if (s > 1) cost += 3.4 + 0.16 * s + 1.6e-6 * s * static_cast<double>(M) * wrows;
+      const double steps = static_cast<double>((blocks + s - 1) / s);
+      auto round = [&](int64_t items) {  // (the larger of its two bounds, near where they meet somewhat more than both)
+        const double l = t.start + steps * (t.alone + more * static_cast<double>((items + cus - 1) / cus - 1));
+        const double w = static_cast<double>(items) * (t.power_start + steps * t.power) * 256 / static_cast<double>(cus);
+        return __builtin_sqrt(__builtin_sqrt(l * l * l * l + w * w * w * w));
+      };
+      double cost = static_cast<double>(tiles * s / slots) * round(slots);
+      if (tiles * s % slots) cost += round(tiles * s % slots);
+      if (s > 1) cost += 3.9 + 0.2 * s + 1.7e-6 * s * static_cast<double>(M) * wrows;
       if (cost < least) {
         least = cost;
         pl.tile = i;

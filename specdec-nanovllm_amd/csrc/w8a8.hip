@@ -156,13 +156,16 @@ __device__ __forceinline__ uint32_t lds_addr(const void* l) {
 }
 
 // WM x WN waves of MT x NT tiles of 32 tokens x 32 weight rows; S stages of 128 columns in LDS, loaded S steps ahead.
-// A step is four MFMA depths of 32 columns, whose operands are read three depths ahead, since a small wave's MFMAs of
-// one depth (64 cycles for two tiles) take less time than its reads. After the first depth the workgroup meets: all
+// A step is four MFMA depths of 32 columns, whose operands are read two or three depths ahead, since a small wave's
+// MFMAs of one depth (64 cycles for two tiles) take less time than its reads. Within a step the workgroup meets: all
 // have read this stage, whose place takes the stage S steps on, and the next stage has landed and is read from here
-// on, so that no MFMA waits for the reads after a barrier. (777 x 2560 x 9728 in tiles of 128 x 128: 33.3 us; 38.1 with
-// operands one depth ahead, 36.2 with the freed stage loaded a step later and no wait for this step's reads, 36.2 with
-// K split between two groups of waves for a third fewer reads. Without any loads 33: waits of eight waves for each
-// other, not memory or LDS, bound that tile.)
+// on, so that no MFMA waits for the reads after a barrier. With three stages or more it meets after the first depth,
+// three depths ahead (777 x 2560 x 9728 in tiles of 128 x 128 33.3 us, 38.1 with operands one depth ahead, 40.3 when it
+// meets after the second); with two after the second, which leaves the one stage in flight more time (1300 x 8192 x
+// 8192 in tiles of 256 x 256 87.9 us, 92.5 after the first). Tried at 777 x 2560 x 9728 and no better: the freed stage
+// loaded a step later without a wait for this step's reads (36.2), K split between two groups of waves for a third
+// fewer reads (36.2). Without any loads that tile takes 33: eight waves' waits for each other and for their reads bound
+// it, not memory.
 // LDS: 16-byte unit u of a row stands at u ^ turn, so that 16 rows' operand reads hit 16 different places of 256 bytes
 // (64 banks). MFMA row 8 a + 4 h + b reads weight row 16 h + 4 a + b of its tile: a lane (half h of the wave) then holds
 // sums of 16 neighbouring rows. GATED: rows 0 .. 15 of a tile are the gate's of 16 outputs, 16 .. 31 the up rows.
@@ -283,26 +286,27 @@ __global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(WM
     else SD_MEET(3);
 #undef SD_MEET
   };
-  constexpr int kAhead = kDepths - 1;  // depths that operands are read ahead
+  constexpr int kMeet = S == 2 ? 2 : 1;  // the depth before which the workgroup meets
+  constexpr int kFirst = kDepths - kMeet;  // depths read before the loop
+  auto read = [&](const uint8_t* stage, int j, int i) {  // the operands of depth j: token tile i, and its share of the others
+    xf[j][i] = sd::load16(stage + x_at[j] + i * (32 * kBlock));
+#pragma unroll
+    for (int t = i * NT / MT; t < (i + 1) * NT / MT; ++t) wf[j][t] = sd::load16(stage + w_at[j] + t * (32 * kBlock));
+  };
   meet_at(min(S, b1 - b0) - 1);
 #pragma unroll
-  for (int j = 0; j < kAhead; ++j) {
+  for (int j = 0; j < kFirst; ++j)
 #pragma unroll
-    for (int i = 0; i < MT; ++i) xf[j][i] = sd::load16(sm + x_at[j] + i * (32 * kBlock));
-#pragma unroll
-    for (int t = 0; t < NT; ++t) wf[j][t] = sd::load16(sm + w_at[j] + t * (32 * kBlock));
-  }
+    for (int i = 0; i < MT; ++i) read(sm, j, i);
   int buf = 0;
   auto step = [&](int blk, auto middle) {  // middle: the stage S on is a whole one
     constexpr bool kMiddle = decltype(middle)::value;
-    constexpr int kMeet = kDepths - kAhead, kParts = MT * kAhead;  // the loads are spread over what follows the meeting
+    constexpr int kParts = MT * (kDepths - kMeet);  // the loads are spread over what follows the meeting
     const int next = buf + 1 == S ? 0 : buf + 1;
     const int left = a.K - blk * kBlock;
 #pragma unroll
     for (int j = 0; j < kDepths; ++j) {
       if (j == kMeet) meet_at(kMiddle ? S - 2 : min(S - 2, b1 - 2 - blk));
-      const uint8_t* const from = sm + (j >= kMeet ? next : buf) * kBytes;
-      const int then = (j + kAhead) % kDepths;
       if (!kMiddle && left < kBlock) {  // the last columns
         const bool none = 32 * j + 16 * lh >= left;
 #pragma unroll
@@ -311,10 +315,13 @@ __global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(WM
       }
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
-        xf[then][i] = sd::load16(from + x_at[then] + i * (32 * kBlock));
+        // the rest of this stage with its first depth, so that the reads are old when the workgroup meets
+        if (j == 0) {
 #pragma unroll
-        for (int t = i * NT / MT; t < (i + 1) * NT / MT; ++t)
-          wf[then][t] = sd::load16(from + w_at[then] + t * (32 * kBlock));
+          for (int d = kFirst; d < kDepths; ++d) read(sm + buf * kBytes, d, i);
+        } else if (j >= kMeet) {
+          read(sm + next * kBytes, j - kMeet, i);
+        }
         if (j >= kMeet && (kMiddle || blk + S < b1)) {
           const int q = (j - kMeet) * MT + i;
           load(blk + S, buf, q * kLoads / kParts, (q + 1) * kLoads / kParts, middle);
@@ -469,10 +476,10 @@ struct Tile {
   double start, alone, full, power_start, power;
 };
 constexpr Tile kTiles[] = {
-    {256, 256, 1, 6.0, 1.082, 1.082, 0.037, 0.0057}, {192, 256, 1, 3.9, 0.905, 0.905, 0.032, 0.0043},
-    {128, 256, 1, 5.2, 0.487, 0.487, 0.021, 0.0032}, {192, 128, 1, 4.1, 0.393, 0.393, 0.014, 0.0026},
-    {128, 128, 1, 3.6, 0.295, 0.295, 0.012, 0.0018}, {128, 128, 2, 2.3, 0.515, 0.632, 0.009, 0.0018},
-    {64, 128, 2, 2.3, 0.232, 0.528, 0.006, 0.0008},  {32, 64, 4, 2.3, 0.149, 0.422, 0.000, 0.0004},
+    {256, 256, 1, 7.2, 0.979, 0.979, 0.036, 0.0058}, {192, 256, 1, 5.1, 0.839, 0.839, 0.030, 0.0043},
+    {128, 256, 1, 5.1, 0.506, 0.506, 0.023, 0.0032}, {192, 128, 1, 4.1, 0.408, 0.408, 0.016, 0.0026},
+    {128, 128, 1, 3.4, 0.308, 0.308, 0.013, 0.0019}, {128, 128, 2, 2.3, 0.500, 0.706, 0.009, 0.0017},
+    {64, 128, 2, 2.3, 0.228, 0.523, 0.006, 0.0009},  {32, 64, 4, 2.4, 0.149, 0.440, 0.000, 0.0004},
 };
 
 // What runs a shape: w8a8_rows<XT> of W waves (XT > 0), or a tile and K slices.
@@ -496,7 +503,7 @@ Plan make_plan(int64_t M, int64_t N, int64_t K, bool gated) {
     if (pl.W > stages) pl.W = static_cast<int>(stages);
     return pl;
   }
-  // The tile and slices of the least time by the figures above (over 262 shapes of 17 to 4096 rows 0.6% above the
+  // The tile and slices of the least time by the figures above (over 290 shapes of 17 to 4096 rows 0.8% above the
   // fastest of them on average, 22% at worst). Slices cost a launch and their sums' way to memory and back.
   const int64_t blocks = (K + kBlock - 1) / kBlock;
   double least = 1e30;
@@ -513,7 +520,7 @@ Plan make_plan(int64_t M, int64_t N, int64_t K, bool gated) {
       };
       double cost = static_cast<double>(tiles * s / slots) * round(slots);
       if (tiles * s % slots) cost += round(tiles * s % slots);
-      if (s > 1) cost += 3.9 + 0.2 * s + 1.7e-6 * s * static_cast<double>(M) * wrows;
+      if (s > 1) cost += 3.7 + 0.17 * s + 1.7e-6 * s * static_cast<double>(M) * wrows;
       if (cost < least) {
         least = cost;
         pl.tile = i;

@@ -1,7 +1,8 @@
 """Oracle of the 8-bit activations and the integer linears (numpy).
 
-16-bit inputs arrive as float32 arrays of their exact values. The codes follow from fp32 v and max |v| by one exact
-quotient, so they are compared for equality; scales and outputs in 64 bits, the linear's also by its own fp32
+16-bit inputs arrive as float32 arrays of their exact values. The codes follow from fp32 v and max |v| by one quotient
+rounded to fp32 (of two 16-bit values it is at least 2^-12 from a tie or one, so that this rounding moves no code), so
+they are compared for equality; scales and outputs in 64 bits, the linear's also by its own fp32
 steps."""
 from __future__ import annotations
 
@@ -14,8 +15,7 @@ def codes(v):
     most = np.abs(v).max(-1)
     fine = np.isfinite(most)
     safe = np.where(fine & (most > 0), most, 1.0)
-    # a quotient of two 24-bit numbers is a tie or at least 2^-26 from one: rounding it to 53 bits moves none
-    c = np.rint(127 * np.where(fine[:, None], v, 0) / safe[:, None]).astype(np.int64)
+    c = np.rint((127 * np.where(fine[:, None], v, 0) / safe[:, None]).astype(np.float32)).astype(np.int64)
     return np.where((fine & (most > 0))[:, None], c, 0), np.where(fine, most, np.nan)
 
 

@@ -6,8 +6,8 @@
 //   value = code scale
 //
 // The root mean square cancels out of the codes: the sum of squares and max |v| are one reduction, between
-// which and the codes the row stays in registers. A code is that of the exact quotient of the fp32 v and max |v|;
-// the normalised value itself is never rounded. A row with a NaN or an infinity in v has scale NaN and codes 0,
+// which and the codes the row stays in registers. A code is that of the fp32 quotient of the fp32 v and max |v|; the
+// normalised value itself is never rounded. A row with a NaN or an infinity in v has scale NaN and codes 0,
 // a row of zeros scale 0.
 // Bound by memory: 7 bytes an element with a residual, 3 without either.
 #include <math.h>
@@ -54,31 +54,26 @@ __device__ __forceinline__ float element(const u32x4& v, int i, float (*to)(uint
   return to(static_cast<uint16_t>(v[i / 2] >> (16 * (i & 1))));
 }
 
-// The codes of 8 values. v inv is off by 2^-16 at most (two roundings of up to 127), so that only a quotient
-// that near to a border needs 127 v - r most, which two exact products give.
-__device__ __forceinline__ uint2 codes8(const float (&v)[8], float most, float inv) {
+// The codes of 8 values: the quotient 127 v / most, rounded to fp32, to the nearest whole number (half to even). The
+// product with the rounded 127 / most is off by up to 2^-16; its remainder 127 v - q most, exact in two parts, brings it
+// to the nearest fp32, so that a tie is one and stays one. SHORT: v and most are 16-bit values, whose products are exact
+// in one. No branch: taken only next to a border, the correction cost 1.2 us of a launch of 2.4 (its code came late).
+template <bool SHORT>
+__device__ __forceinline__ uint2 codes8(const float (&v)[8], float most, float inv, float inv1) {
 #pragma clang fp contract(off)
-  float r[8], near = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float q = v[i] * inv;
-    r[i] = rintf(q);
-    near = fmaxf(near, fabsf(q - r[i]));
-  }
-  if (near > 0.5f - 0x1p-14f) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float p = r[i] * most, p_low = fmaf(r[i], most, -p);
-      const float u = 127.f * v[i], u_low = fmaf(127.f, v[i], -u);
-      const float d = (u - p) + (u_low - p_low), half = 0.5f * most;
-      const bool odd = static_cast<int>(r[i]) & 1;
-      if (d > half || (d == half && odd)) r[i] += 1.f;
-      else if (d < -half || (d == -half && odd)) r[i] -= 1.f;
-    }
-  }
   uint32_t b[2] = {0, 0};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) b[i / 4] |= (static_cast<uint32_t>(static_cast<int>(r[i])) & 0xffu) << (8 * (i % 4));
+  for (int i = 0; i < 8; ++i) {
+    float q = v[i] * inv, rem;
+    if constexpr (SHORT) {
+      rem = fmaf(-q, most, 127.f * v[i]);
+    } else {
+      const float p = q * most;
+      rem = fmaf(127.f, v[i], -p) - fmaf(q, most, -p);
+    }
+    q = fmaf(rem, inv1, q);
+    b[i / 4] |= (static_cast<uint32_t>(static_cast<int>(rintf(q))) & 0xffu) << (8 * (i % 4));
+  }
   return uint2{b[0], b[1]};
 }
 
@@ -156,7 +151,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rows_int8_kernel(Params
   }
   // by a power of two into the range where 127 v and the quotient's inverse are finite and normal
   const float to = most < 0x1p-60f ? 0x1p64f : most > 0x1p60f ? 0x1p-64f : 1.f;
-  const float scaled = most * to, inv = 127.f / scaled;
+  const float scaled = most * to, inv = 127.f / scaled, inv1 = inv * (1.f / 127.f);
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     const int e = (c * TPR + t) * 8;
@@ -164,7 +159,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rows_int8_kernel(Params
     float u[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) u[i] = v[c][i] * to;
-    *reinterpret_cast<uint2*>(p.codes + row * p.cs + e) = none ? uint2{0, 0} : codes8(u, scaled, inv);
+    *reinterpret_cast<uint2*>(p.codes + row * p.cs + e) = none ? uint2{0, 0} : codes8<!NORM>(u, scaled, inv, inv1);
   }
 }
 

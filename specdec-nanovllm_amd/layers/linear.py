@@ -24,6 +24,7 @@ from .quant import int4_linear, int8_linear, int8_linear_a8
 
 
 class LinearBase(nn.Module):
+    quant_act_bits = 16  # (of the class: modules saved before it was there have it too)
 
     def __init__(self, input_size: int, output_size: int, bias: bool = False,
                  tp_dim: int | None = None):
@@ -33,7 +34,6 @@ class LinearBase(nn.Module):
         self.tp_size = 1
         self.quant_granularity = "per_channel"
         self.quant_group_size = 128
-        self.quant_act_bits = 16
         self.weight = nn.Parameter(torch.empty(output_size, input_size))
         if bias:
             self.bias = nn.Parameter(torch.empty(output_size))

@@ -730,9 +730,10 @@ int sd_w4a16_linear(const void* x, int64_t x_stride_m, const uint8_t* w, int64_t
  * meet 16-bit activations). A row of activations is held as codes -127 .. 127 and
  * one fp32 scale:
  *   scale = max |v| / 127,  code = round_half_even(127 v / max |v|),  value = code * scale
- * (the quotient rounded to fp32 once). A row with a NaN or an infinity in v has scale NaN and codes 0 (a linear's outputs
- * of that row are NaN); a row of zeros has scale 0. Rows of codes and of 16-bit
- * tensors are 16-byte aligned; columns are a multiple of 16.
+ * (the quotient rounded to fp32 once). A row with a NaN or an infinity in v has scale
+ * NaN and codes 0 (a linear's outputs of that row are NaN); a row of zeros has scale 0.
+ * Rows of codes and of 16-bit tensors are 16-byte aligned; columns are a multiple of 16.
+ * Outputs share no byte with inputs or each other, but for residual_out.
  * ------------------------------------------------------------------------- */
 
 /*
@@ -769,14 +770,15 @@ int sd_dequantize_rows_int8(const int8_t* codes, int64_t codes_stride, const flo
  *   x       : (M, K) codes, row stride x_stride_m;  x_scale : (M,) fp32
  *   w       : (N, K) int8, row stride w_stride_n (the W8A16 linear's per-channel weights)
  *   scale   : (N,) scale_dtype bf16/f16/f32;  bias : (N,) dtype or NULL
- *   y       : (M, N) dtype (bf16/f16), row stride y_stride_m (>= N), sharing no byte with
- *             x, x_scale or w
+ *   y       : (M, N) dtype (bf16/f16), row stride y_stride_m (>= N)
  * K is a multiple of 16 below 2^17: the integer sums are exact (any codes, -128 too).
  * sum * scale in fp32, times x_scale plus bias in one fp32 step, and the rounding
- * follow; a row's outputs are the same bits whatever M. x_stride_m and w_stride_n <= 2^23 where there is more than one row.
+ * follow; a row's outputs are the same bits whatever M. x_stride_m and w_stride_n <= 2^23
+ * where there is more than one row to step over. M <= 2^24, N <= 2^21, and
+ * ceil(M / 64) * ceil(N / 64) < 2^22.
  * workspace: sd_w8a8_workspace_size bytes on the same device, 16-byte aligned (sums of
- * K slices; 0 where one slice runs). Without it (NULL or too small) the call runs in
- * one slice. `gated`: the query is for sd_w8a8_gate_up_silu.
+ * K slices; 0 where one slice runs). Without it (NULL, too small or not aligned) the call
+ * runs in one slice. `gated`: the query is for sd_w8a8_gate_up_silu.
  */
 size_t sd_w8a8_workspace_size(int64_t M, int64_t N, int64_t K, int32_t gated);
 /*

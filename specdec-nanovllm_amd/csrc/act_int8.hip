@@ -257,6 +257,17 @@ int check(const char* what, const Params& p, int32_t dtype, bool residual) {
     sd::set_error("%s: rows must be 16-byte aligned", what);
     return SD_ERR_UNSUPPORTED;
   }
+  const int64_t width = 2 * static_cast<int64_t>(p.K);
+  const sd::Span codes = sd::span_rows(p.codes, p.rows, p.cs, p.K), scale = sd::span_rows(p.scale, p.rows, 4, 4);
+  const sd::Span w = sd::span_rows(p.w, 1, 0, width), res_out = sd::span_rows(p.res_out, p.rows, 2 * p.ros, width);
+  bool shared = codes.overlaps(scale) || res_out.overlaps(w);
+  for (const sd::Span& o : {sd::span_rows(p.x, p.rows, 2 * p.xs, width), sd::span_rows(p.res, p.rows, 2 * p.rs, width),
+                            w, res_out})
+    shared |= codes.overlaps(o) || scale.overlaps(o);
+  if (shared) {
+    sd::set_error("%s: outputs share memory with another argument", what);
+    return SD_ERR_VALUE;
+  }
   return SD_OK;
 }
 
@@ -323,6 +334,12 @@ extern "C" int sd_dequantize_rows_int8(const int8_t* codes, int64_t codes_stride
       (rows > 1 && (codes_stride % 16 || out_stride % (dtype == SD_F32 ? 4 : 8)))) {
     sd::set_error("%s: rows must be 16-byte aligned", what);
     return SD_ERR_UNSUPPORTED;
+  }
+  const int64_t bytes = dtype == SD_F32 ? 4 : 2;
+  const sd::Span o = sd::span_rows(out, rows, bytes * out_stride, bytes * columns);
+  if (o.overlaps(sd::span_rows(codes, rows, codes_stride, columns)) || o.overlaps(sd::span_rows(scale, rows, 4, 4))) {
+    sd::set_error("%s: out shares memory with an input", what);
+    return SD_ERR_VALUE;
   }
   p.items = rows * p.spans;
   hipStream_t st = static_cast<hipStream_t>(stream);

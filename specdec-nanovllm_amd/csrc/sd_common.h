@@ -586,6 +586,14 @@ inline Span span16(const void* p, int64_t rows, int64_t stride, int64_t width) {
   return Span{lo, lo + static_cast<uintptr_t>(((rows - 1) * st + width) * 2)};
 }
 
+// The same of any row-major matrix, in bytes, by a stride of either sign; ends where the address space does.
+inline Span span_rows(const void* p, int64_t rows, int64_t stride_bytes, int64_t width_bytes) {
+  if (!p || rows <= 0 || width_bytes <= 0) return Span{0, 0};
+  const __int128 at = reinterpret_cast<uintptr_t>(p), last = at + static_cast<__int128>(rows - 1) * stride_bytes;
+  const __int128 lo = at < last ? at : last, hi = (at < last ? last : at) + width_bytes;
+  return Span{lo < 0 ? 0 : static_cast<uintptr_t>(lo), hi > UINTPTR_MAX ? UINTPTR_MAX : static_cast<uintptr_t>(hi)};
+}
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // Strides (in elements) the entry points accept: |stride| <= 2^40 keeps every

@@ -590,13 +590,6 @@ size_t workspace(int64_t M, int64_t N, int64_t K, bool gated) {
   return pl.slices > 1 ? static_cast<size_t>(pl.slices) * M * N * (gated ? 2 : 1) * sizeof(int32_t) : 0;
 }
 
-// Bytes of a matrix; ends at the address space's end where strides lead past it.
-sd::Span span(const void* p, int64_t rows, int64_t stride_bytes, int64_t width_bytes) {
-  const uintptr_t lo = reinterpret_cast<uintptr_t>(p);
-  const unsigned __int128 hi = static_cast<unsigned __int128>(rows - 1) * stride_bytes + width_bytes + lo;
-  return sd::Span{lo, hi > UINTPTR_MAX ? UINTPTR_MAX : static_cast<uintptr_t>(hi)};
-}
-
 int run(const char* what, bool gated, Args a, int32_t dtype, void* workspace_p, size_t workspace_bytes, void* stream) {
   sd::clear_error();
   const int64_t M = a.M, N = a.N, wrows = gated ? 2 * N : N;
@@ -635,15 +628,18 @@ int run(const char* what, bool gated, Args a, int32_t dtype, void* workspace_p, 
     sd::set_error("%s: rows of y overlap (stride %lld, %lld columns)", what, (long long)a.ys, (long long)N);
     return SD_ERR_VALUE;
   }
-  const sd::Span y = span(a.y, M, 2 * a.ys, 2 * N);
-  if (span(a.x, M, a.xs, a.K).overlaps(y) || span(a.x_scale, M, 4, 4).overlaps(y) ||
-      span(a.w, wrows, a.ws, a.K).overlaps(y)) {
-    sd::set_error("%s: y shares memory with an input", what);
+  const sd::Span y = sd::span_rows(a.y, M, 2 * a.ys, 2 * N);
+  const int64_t scale_bytes = a.scale_dtype == SD_F32 ? 4 : 2;
+  if (sd::span_rows(a.x, M, a.xs, a.K).overlaps(y) || sd::span_rows(a.x_scale, M, 4, 4).overlaps(y) ||
+      sd::span_rows(a.w, wrows, a.ws, a.K).overlaps(y) || sd::span_rows(a.scale, wrows, scale_bytes, scale_bytes).overlaps(y) ||
+      (a.bias && sd::span_rows(a.bias, wrows, 2, 2).overlaps(y))) {
+    sd::set_error("%s: y shares memory with another argument", what);
     return SD_ERR_VALUE;
   }
   a.wide_y = sd::aligned16(a.y) && a.ys % 8 == 0;
   const size_t need = workspace(M, N, a.K, gated);
-  a.part = need && workspace_p && workspace_bytes >= need ? static_cast<int32_t*>(workspace_p) : nullptr;
+  const bool held = need && workspace_p && workspace_bytes >= need && sd::aligned16(workspace_p);
+  a.part = held ? static_cast<int32_t*>(workspace_p) : nullptr;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (gated) return dtype == SD_BF16 ? launch<__bf16, true>(a, st) : launch<_Float16, true>(a, st);
   return dtype == SD_BF16 ? launch<__bf16, false>(a, st) : launch<_Float16, false>(a, st);

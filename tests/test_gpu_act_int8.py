@@ -80,7 +80,7 @@ def test_ties_go_to_the_even_code(kind):
 
 
 def test_quotients_next_to_a_tie():
-    """Rows whose products with the weight have 24 bits, quotients within 2^-20 of n + 1/2 among them."""
+    """Rows whose products with the weight have 24 bits, quotients within 2^-16 of n + 1/2 among them."""
     g = torch.Generator().manual_seed(3)
     x = torch.randn((64, 4096), generator=g).half().to(DEV)
     w = (torch.rand((4096,), generator=g) + 0.5).half().to(DEV)

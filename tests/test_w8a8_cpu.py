@@ -56,6 +56,14 @@ _REFUSED = [
     ("sd_rmsnorm_int8", {"a13": BF16, "a4": A[2] + 8}, 2, "aligned"),
     ("sd_rmsnorm_int8", {"a13": BF16, "a9": 1020}, 1, "overlap"),
     ("sd_rmsnorm_int8", {"a13": BF16, "a9": 1028}, 2, "aligned"),
+    ("sd_quantize_rows_int8", {"a7": BF16, "a2": A[0] + 2048}, 1, "share memory"),
+    ("sd_quantize_rows_int8", {"a7": BF16, "a4": A[2] + 4, "a2": A[2]}, 1, "share memory"),
+    ("sd_quantize_rows_int8", {"a7": BF16, "a1": -1024, "a2": A[0] - 6144}, 1, "share memory"),
+    ("sd_rmsnorm_int8", {"a13": BF16, "a5": A[1]}, 1, "share memory"),
+    ("sd_rmsnorm_int8", {"a13": BF16, "a7": A[2] + 2044}, 1, "share memory"),
+    ("sd_rmsnorm_int8", {"a13": BF16, "a8": A[4] - 1024}, 1, "share memory"),
+    ("sd_dequantize_rows_int8", {"a7": F32, "a3": A[0] + 4080}, 1, "shares memory"),
+    ("sd_dequantize_rows_int8", {"a7": F32, "a3": A[1] - 16368}, 1, "shares memory"),
     ("sd_dequantize_rows_int8", {}, 2, "dtype"),
     ("sd_dequantize_rows_int8", {"a5": 1 << 26}, 2, "2\\^26"),
     ("sd_dequantize_rows_int8", {"a7": BF16, "a2": None}, 1, "null"),
@@ -83,6 +91,8 @@ for _name in ("sd_w8a8_linear", "sd_w8a8_gate_up_silu"):
         (_name, {**_BF, "a8": A[0] + 1024}, 1, "shares memory"),
         (_name, {**_BF, "a8": A[1] + 8}, 1, "shares memory"),
         (_name, {**_BF, "a8": A[2] + (1 << 20)}, 1, "shares memory"),
+        (_name, {**_BF, "a8": A[3] + 4096}, 1, "shares memory"),
+        (_name, {**_BF, "a7": A[5], "a8": A[5] - 32766}, 1, "shares memory"),
     ]
 
 

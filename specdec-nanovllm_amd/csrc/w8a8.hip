@@ -162,17 +162,21 @@ __device__ __forceinline__ uint32_t lds_addr(const void* l) {
 // on, so that no MFMA waits for the reads after a barrier. With three stages or more it meets after the first depth,
 // three depths ahead (777 x 2560 x 9728 in tiles of 128 x 128 33.3 us, 38.1 with operands one depth ahead, 40.3 when it
 // meets after the second); with two after the second, which leaves the one stage in flight more time (1300 x 8192 x
-// 8192 in tiles of 256 x 256 87.9 us, 92.5 after the first). Tried at 777 x 2560 x 9728 and no better: the freed stage
-// loaded a step later without a wait for this step's reads (36.2), K split between two groups of waves for a third
-// fewer reads (36.2). Without any loads that tile takes 33: eight waves' waits for each other and for their reads bound
-// it, not memory.
+// 8192 in tiles of 256 x 256 87.9 us, 92.5 after the first). Tried at 777 x 2560 x 9728 in 128 x 128 and no better: the
+// freed stage loaded a step later without a wait for this step's reads (36.2), K split between two groups of waves for a
+// third fewer reads (36.2), four waves of 64 x 64 each (33.3).
+// What bounds long K: of those 33.3 us the loads and meetings alone take 32, the MFMAs and meetings alone 26, the reads
+// and meetings alone 25. A compute unit gets 32 KB in 0.23 us where its XCD's L2 holds them and in 0.34 to 0.38 where it
+// does not, with 64 KB in flight or 128 (six stages of 96 x 96, eight of 64 x 64 are no faster than three and four); a
+// wave that reads the lines ahead into the L2 costs more than it gives (a quarter of them: 37 us by vector loads, 100 by
+// scalar ones). So tiles are chosen to give each compute unit the same share.
 // LDS: 16-byte unit u of a row stands at u ^ turn, so that 16 rows' operand reads hit 16 different places of 256 bytes
 // (64 banks). MFMA row 8 a + 4 h + b reads weight row 16 h + 4 a + b of its tile: a lane (half h of the wave) then holds
 // sums of 16 neighbouring rows. GATED: rows 0 .. 15 of a tile are the gate's of 16 outputs, 16 .. 31 the up rows.
 constexpr int kBlock = 128;
 
 template <typename T, int WM, int WN, int MT, int NT, int S, bool GATED>
-__global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(WM * WN / 4))) void w8a8_gemm(Args a) {
+__global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu((WM * WN + 3) / 4))) void w8a8_gemm(Args a) {
   constexpr int NW = WM * WN, BM = 32 * MT * WM, BN = 32 * NT * WN;
   constexpr int BO = GATED ? BN / 2 : BN;            // outputs
   constexpr int CX = BM / 8 / NW, CW = BN / 8 / NW;  // 1 KB loads (8 rows) of a wave and step
@@ -468,18 +472,21 @@ template <typename T, bool GATED, int V> __global__ __launch_bounds__(256) void 
   }
 }
 
-// The tiles there are, with what they were measured to take (us): a round of workgroups `start` + steps x `alone`
-// where each has a compute unit to itself, `full` a step where `per_cu` share it; and, since the whole device multiplies
-// only as fast as its power allows, a workgroup `power_start` + steps x `power` of the device.
+// The tiles there are: 64 x 64 for few tiles of long rows (384 x 2560 x 9728 20.0 us, 23.3 in the others), 96 x 96 where
+// it fills the device and 128 x 128 does not (777 x 2560 x 9728 30.8 and 33.3), 64 x 128 to 256 x 256 by size. Each with
+// what it was measured to take (us): a round of workgroups `start` + steps x `alone` where each has a compute unit to
+// itself, `full` a step where `per_cu` share it; and, since the whole device multiplies only as fast as its power allows,
+// a workgroup `power_start` + steps x `power` of the device.
 struct Tile {
   int bm, bn, per_cu;
   double start, alone, full, power_start, power;
 };
 constexpr Tile kTiles[] = {
-    {256, 256, 1, 7.2, 0.979, 0.979, 0.036, 0.0058}, {192, 256, 1, 5.1, 0.839, 0.839, 0.030, 0.0043},
-    {128, 256, 1, 5.1, 0.506, 0.506, 0.023, 0.0032}, {192, 128, 1, 4.1, 0.408, 0.408, 0.016, 0.0026},
-    {128, 128, 1, 3.4, 0.308, 0.308, 0.013, 0.0019}, {128, 128, 2, 2.3, 0.500, 0.706, 0.009, 0.0017},
-    {64, 128, 2, 2.3, 0.228, 0.523, 0.006, 0.0009},  {32, 64, 4, 2.4, 0.149, 0.440, 0.000, 0.0004},
+    {256, 256, 1, 7.3, 0.969, 0.969, 0.035, 0.0058}, {192, 256, 1, 4.9, 0.841, 0.841, 0.033, 0.0043},
+    {128, 256, 1, 5.0, 0.511, 0.511, 0.023, 0.0032}, {192, 128, 1, 3.9, 0.419, 0.419, 0.018, 0.0026},
+    {128, 128, 1, 3.3, 0.318, 0.318, 0.014, 0.0019}, {96, 96, 1, 3.7, 0.266, 0.266, 0.011, 0.0012},
+    {64, 128, 2, 2.3, 0.234, 0.519, 0.006, 0.0009},  {64, 64, 2, 2.6, 0.171, 0.337, 0.005, 0.0003},
+    {32, 64, 4, 2.4, 0.147, 0.440, 0.000, 0.0004},
 };
 
 // What runs a shape: w8a8_rows<XT> of W waves (XT > 0), or a tile and K slices.
@@ -503,8 +510,8 @@ Plan make_plan(int64_t M, int64_t N, int64_t K, bool gated) {
     if (pl.W > stages) pl.W = static_cast<int>(stages);
     return pl;
   }
-  // The tile and slices of the least time by the figures above (over 290 shapes of 17 to 4096 rows 0.8% above the
-  // fastest of them on average, 22% at worst). Slices cost a launch and their sums' way to memory and back.
+  // The tile and slices of the least time by the figures above (over 336 shapes of 17 to 4096 rows 0.8% above the
+  // fastest of them on average, 21% at worst). Slices cost a launch and their sums' way to memory and back.
   const int64_t blocks = (K + kBlock - 1) / kBlock;
   double least = 1e30;
   for (int i = 0; i < static_cast<int>(sizeof(kTiles) / sizeof(kTiles[0])); ++i) {
@@ -520,7 +527,7 @@ Plan make_plan(int64_t M, int64_t N, int64_t K, bool gated) {
       };
       double cost = static_cast<double>(tiles * s / slots) * round(slots);
       if (tiles * s % slots) cost += round(tiles * s % slots);
-      if (s > 1) cost += 3.7 + 0.17 * s + 1.7e-6 * s * static_cast<double>(M) * wrows;
+      if (s > 1) cost += 3.8 + 0.14 * s + 1.8e-6 * s * static_cast<double>(M) * wrows;
       if (cost < least) {
         least = cost;
         pl.tile = i;
@@ -544,9 +551,10 @@ template <typename T, bool GATED> void launch_tiles(const Args& a, int tile, hip
     SD_TILES(2, 2, 4, 2, 2, 3);
     SD_TILES(3, 2, 4, 3, 1, 3);
     SD_TILES(4, 2, 4, 2, 1, 4);
-    SD_TILES(5, 2, 4, 2, 1, 2);
+    SD_TILES(5, 1, 3, 3, 1, 4);
     SD_TILES(6, 2, 4, 1, 1, 3);
-    SD_TILES(7, 1, 2, 1, 1, 3);
+    SD_TILES(7, 2, 2, 1, 1, 4);
+    SD_TILES(8, 1, 2, 1, 1, 3);
   }
 #undef SD_TILES
 }

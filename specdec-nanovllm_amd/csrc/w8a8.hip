@@ -64,12 +64,25 @@ __device__ __forceinline__ i32x16 mfma32(u32x4 a, u32x4 b, i32x16 c) {
   return __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
 }
 
+// Lanes r < 8 of 16 hold units u of row r and of row r + 8, lanes r >= 8 units u + 4 of row r - 8 and of row r: after the
+// exchange each lane holds units u and u + 4 of its own row.
+__device__ __forceinline__ void own_units(u32x4 (&v)[2]) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int a = static_cast<int>(v[0][e]), b = static_cast<int>(v[1][e]);
+    v[0][e] = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(a, b, 0x128, 0xF, 0xC, false));  // row_ror:8
+    v[1][e] = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(b, a, 0x128, 0xF, 0x3, false));
+  }
+}
+
 // Up to 16 XT rows. A workgroup takes 16 weight rows (GATED: the gate's and the up rows of 8 outputs), its waves the
-// stages of 128 columns in turn, loaded straight to registers two stages ahead. The activations come from the caches,
-// as many bytes a lane as of weights, which is what bounds it for more rows or many weight rows: 16 x 19456 x 2560
-// takes 14.2 us here, 11.4 in tiles, 1 x 19456 x 2560 10.3 and 11.1. Registers decide how many loads a compute unit
-// has in flight: stages of 256 columns took 10.9 us there, three of them ahead 10.6, two tiles a wave 13.9;
-// nontemporal loads of the weights 13.5.
+// stages of 128 columns in turn, loaded straight to registers two stages ahead. A load takes whole lines, of 8 rows, and
+// the lanes exchange halves (of 16 rows by 64 bytes: weights from HBM, 16 x 2560 x 9728 11.9 us and 13.1 so, 1 x 19456 x
+// 2560 11.1 and 11.9; from the caches 1% to 3% the other way, 1 x 4096 x 1024 3.10 and 3.03). The activations come from
+// the caches, as many bytes a lane as of weights, which is what bounds it for more rows or many weight rows: 16 x 19456
+// x 2560 takes 14.3 us here, 11.4 in tiles, 1 x 19456 x 2560 10.4 and 11.0. Registers decide how many loads a compute
+// unit has in flight: stages of 256 columns took 10.9 us there, three of them ahead 10.6, two tiles a wave 13.9;
+// nontemporal loads of the weights 13.5. 12 or 16 waves: within 3% of 8.
 constexpr int kStage = 128;
 
 template <typename T, int XT, bool GATED>
@@ -81,11 +94,15 @@ __global__ __launch_bounds__(512) void w8a8_rows(Args a) {
   const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t n0 = static_cast<int64_t>(blockIdx.x) * kCols;
-  const int64_t n = min(n0 + (GATED ? lr & 7 : lr), a.N - 1) + (GATED && lr >= 8 ? a.N : 0);
-  const int8_t* const wrow = a.w + n * a.ws + 16 * lg;
-  const int8_t* xrow[XT];
+  const int unit = 16 * (lg + 4 * (lr >> 3));
+  const int8_t *wrow[2], *xrow[XT][2];
 #pragma unroll
-  for (int i = 0; i < XT; ++i) xrow[i] = a.x + min(16 * i + lr, M - 1) * a.xs + 16 * lg;
+  for (int j = 0; j < 2; ++j) {
+    const int64_t n = min(n0 + (GATED ? lr & 7 : 8 * j + (lr & 7)), a.N - 1) + (GATED && j ? a.N : 0);
+    wrow[j] = a.w + n * a.ws + unit;
+#pragma unroll
+    for (int i = 0; i < XT; ++i) xrow[i][j] = a.x + min(16 * i + 8 * j + (lr & 7), M - 1) * a.xs + unit;
+  }
   i32x4 acc[XT];
 #pragma unroll
   for (int i = 0; i < XT; ++i) acc[i] = i32x4{0, 0, 0, 0};
@@ -94,15 +111,18 @@ __global__ __launch_bounds__(512) void w8a8_rows(Args a) {
   };
   const int stages = (a.K + kStage - 1) / kStage;
   auto load = [&](Stage& st, int s) {
+    const int k = min(s * kStage, a.K - 16 - unit);  // past K: columns that count nothing
 #pragma unroll
-    for (int j = 0; j < kUnits; ++j) {
-      const int k = min(s * kStage + 64 * j, a.K - 16 - 16 * lg);  // past K: columns that count nothing
-      st.w[j] = sd::load16(wrow + k);
+    for (int j = 0; j < 2; ++j) {
+      st.w[j] = sd::load16(wrow[j] + k);
 #pragma unroll
-      for (int i = 0; i < XT; ++i) st.x[i][j] = sd::load16(xrow[i] + k);
+      for (int i = 0; i < XT; ++i) st.x[i][j] = sd::load16(xrow[i][j] + k);
     }
   };
   auto compute = [&](Stage& st, int s) {
+    own_units(st.w);
+#pragma unroll
+    for (int i = 0; i < XT; ++i) own_units(st.x[i]);
     if (s * kStage + kStage > a.K) {  // uniform
 #pragma unroll
       for (int j = 0; j < kUnits; ++j)

@@ -738,7 +738,7 @@ int sd_w4a16_linear(const void* x, int64_t x_stride_m, const uint8_t* w, int64_t
 
 /*
  * codes (rows, columns) and scale (rows,) of the rows of x (rows, columns) dtype
- * bf16/f16. columns <= 32768, rows < 2^24 (2^22 past 8192 columns).
+ * bf16/f16. columns <= 32768, rows < 2^24 (2^22 past 4096 columns).
  */
 int sd_quantize_rows_int8(const void* x, int64_t x_stride, int8_t* codes, int64_t codes_stride,
                           float* scale, int64_t rows, int32_t columns, int32_t dtype,

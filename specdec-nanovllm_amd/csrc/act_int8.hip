@@ -9,7 +9,8 @@
 // which and the codes the row stays in registers. A code is that of the fp32 quotient of the fp32 v and max |v|; the
 // normalised value itself is never rounded. A row with a NaN or an infinity in v has scale NaN and codes 0,
 // a row of zeros scale 0.
-// Bound by memory: 7 bytes an element with a residual, 3 without either.
+// Bound by memory: 7 bytes an element with a residual, 3 without either (8192 x 2560 with a residual 25 us, 147 MB at
+// 5.9 TB/s from and to the caches; 4001 x 4096 without 10, 49 MB at 4.9); few rows by their latency, 2.3 to 3 us.
 #include <math.h>
 
 #include "sd_common.h"
@@ -78,11 +79,14 @@ __device__ __forceinline__ uint2 codes8(const float (&v)[8], float most, float i
 }
 
 // TPR threads a row (64: four rows a workgroup, no barrier); thread t holds the 8-element chunks t, t + TPR, ...
+// The squares of 64 chunks are summed by a wave, then those sums in order, whichever TPR and C <= 2 the launch took: a
+// row's scale is the same bits whatever the other rows.
 template <typename T, bool NORM, bool RES, int TPR, int C>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rows_int8_kernel(Params p) {
 #pragma clang fp contract(off)
   constexpr int kRows = TPR < 256 ? 256 / TPR : 1;
-  __shared__ float red_sum[TPR / 64];
+  constexpr int kSums = C <= 2 ? C : 1;
+  __shared__ float red_sum[kSums * (TPR / 64)];
   __shared__ uint32_t red_max[TPR / 64];
   const int t = static_cast<int>(threadIdx.x) % TPR;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows +
@@ -99,7 +103,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rows_int8_kernel(Params
     if constexpr (RES) rb[c] = sd::load16(res + e);
     if constexpr (NORM) wb[c] = sd::load16(p.w + e);
   }
-  float v[C][8], sum = 0.f;
+  float v[C][8], sums[kSums] = {};
   uint32_t most_bits = 0;
 #pragma unroll
   for (int c = 0; c < C; ++c) {
@@ -114,7 +118,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rows_int8_kernel(Params
       if (!in) s[i] = 0.f;
       v[c][i] = s[i];
       if constexpr (NORM) {
-        sum += s[i] * s[i];
+        sums[kSums == 1 ? 0 : c] += s[i] * s[i];
         v[c][i] = in ? s[i] * element(wb[c], i, sd::from_bits<T>) : 0.f;
       }
       most_bits = max_u32(most_bits, __float_as_uint(v[c][i]) & 0x7fffffffu);  // NaN above infinity above all else
@@ -123,22 +127,28 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rows_int8_kernel(Params
       sd::store16(p.res_out + row * p.ros + e, u32x4{sd::pack2<T>(s[0], s[1]), sd::pack2<T>(s[2], s[3]),
                                                      sd::pack2<T>(s[4], s[5]), sd::pack2<T>(s[6], s[7])});
   }
-  if constexpr (NORM) sum = sd::xor_sum_down<32>(sum);
+  float sum = 0.f;
+  if constexpr (NORM) {
+#pragma unroll
+    for (int c = 0; c < kSums; ++c) sums[c] = sd::xor_sum_down<32>(sums[c]);
+  }
   most_bits = wave_max(most_bits);
   if constexpr (TPR > 64) {
     const int wave = t >> 6;
     if ((t & 63) == 0) {
-      red_sum[wave] = sum;
+#pragma unroll
+      for (int c = 0; c < kSums; ++c) red_sum[c * (TPR / 64) + wave] = sums[c];
       red_max[wave] = most_bits;
     }
     __syncthreads();
-    sum = 0.f;
     most_bits = 0;
 #pragma unroll
-    for (int i = 0; i < TPR / 64; ++i) {
-      sum += red_sum[i];
-      most_bits = max_u32(most_bits, red_max[i]);
-    }
+    for (int i = 0; i < kSums * (TPR / 64); ++i) sum += red_sum[i];
+#pragma unroll
+    for (int i = 0; i < TPR / 64; ++i) most_bits = max_u32(most_bits, red_max[i]);
+  } else {
+#pragma unroll
+    for (int c = 0; c < kSums; ++c) sum += sums[c];
   }
   const bool none = most_bits >= 0x7f800000u || most_bits == 0;
   const float most = __uint_as_float(most_bits);
@@ -212,11 +222,17 @@ template <typename T, bool NORM, bool RES> void launch(const Params& p, hipStrea
   hipLaunchKernelGGL((rows_int8_kernel<T, NORM, RES, tpr, c>),                                            \
                      dim3(static_cast<unsigned>(tpr < 256 ? (p.rows + 256 / tpr - 1) / (256 / tpr) : p.rows)), \
                      dim3(tpr < 256 ? 256 : tpr), 0, st, p)
+  // A wave a row saves the barrier where rows are short and many, a thread for 8 elements saves steps where they are few
+  // (norm with residual, us): 1 x 1024 2.5 with 256 threads, 2.9 with 64, 4096 x 1024 7.4 and 6.4; 200 x 2560 3.3 with
+  // 512 threads, 3.6 with 256, 777 x 2560 5.0 and 5.3 but 3.6 and 3.5 quantized, 32768 x 2560 112 and 100. Past that 512
+  // threads: 777 x 8192 9.4, 10.2 with 256, 9.9 with 1024; 4096 x 9728 46, 53 with 1024.
   if (p.K <= 512) SD_ROWS_INT8(64, 1);
-  else if (p.K <= 1024) SD_ROWS_INT8(64, 2);
+  else if (p.K <= 1024 && p.rows > 512) SD_ROWS_INT8(64, 2);
+  else if (p.K <= 2048) SD_ROWS_INT8(256, 1);
+  else if (p.K <= 4096 && p.rows <= 512) SD_ROWS_INT8(512, 1);
   else if (p.K <= 4096) SD_ROWS_INT8(256, 2);
-  else if (p.K <= 8192) SD_ROWS_INT8(256, 4);
-  else if (p.K <= 16384) SD_ROWS_INT8(1024, 2);
+  else if (p.K <= 8192) SD_ROWS_INT8(512, 2);
+  else if (p.K <= 16384) SD_ROWS_INT8(512, 4);
   else SD_ROWS_INT8(1024, 4);
 #undef SD_ROWS_INT8
 }
@@ -228,7 +244,7 @@ template <typename T> void launch(const Params& p, hipStream_t st) {
 
 constexpr int kMostColumns = 32768;
 // (a launch takes fewer than 2^32 threads)
-constexpr int64_t most_rows(int32_t columns) { return columns > 8192 ? (1 << 22) - 1 : (1 << 24) - 1; }
+constexpr int64_t most_rows(int32_t columns) { return columns > 4096 ? (1 << 22) - 1 : (1 << 24) - 1; }
 
 // What both entries ask of their sizes and outputs; SD_OK or the refusal.
 int check(const char* what, const Params& p, int32_t dtype, bool residual) {
@@ -237,7 +253,7 @@ int check(const char* what, const Params& p, int32_t dtype, bool residual) {
     return SD_ERR_VALUE;
   }
   if (p.K % 16 != 0 || p.K > kMostColumns || p.rows > most_rows(p.K) || (dtype != SD_BF16 && dtype != SD_F16)) {
-    sd::set_error("%s: columns must be a multiple of 16 up to %d, rows below 2^24 (2^22 past 8192 columns), dtype bf16 "
+    sd::set_error("%s: columns must be a multiple of 16 up to %d, rows below 2^24 (2^22 past 4096 columns), dtype bf16 "
                   "or f16 (%lld rows of %d columns, dtype %d)", what, kMostColumns, (long long)p.rows, p.K, dtype);
     return SD_ERR_UNSUPPORTED;
   }

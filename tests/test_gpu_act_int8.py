@@ -1,8 +1,8 @@
 """Activations in 8 bits (csrc/act_int8.hip through ``ops``) against the oracle.
 
 Codes are equal. A scale without a norm is one correctly rounded division: 2^-24. With the norm, the sum of K squares
-has at most 40 roundings in a row (32 of a thread's, 6 in the wave, 2 to 16 of waves are no more than 40 + 16), half of
-which pass the root, then the mean, eps, root, inverse and two products: (28 + 8) 2^-24.
+has at most 56 roundings in a row (8 or 32 of a thread's, 6 in the wave, 1 to 16 of the waves' sums), half of which pass
+the root, then the mean, eps, root, inverse and two products: (28 + 8) 2^-24.
 """
 import numpy as np
 import pytest
@@ -65,6 +65,16 @@ def test_rows_and_columns(kind, rows, k):
     w, r = weight(k, kind), make(rows, k, kind, seed=5)
     check_norm(x, w, ops.rmsnorm_int8(x, w, EPS))
     check_norm(x, w, ops.rmsnorm_int8(x, w, EPS, r), r)
+
+
+@pytest.mark.parametrize("k", [496, 528, 1024, 1040, 2048, 2064, 4096, 4112, 9728])
+def test_rows_do_not_depend_on_the_call(k):
+    """Few rows take more threads each, sums of squares the same steps."""
+    x, r, w = make(1030, k, "bf16"), make(1030, k, "bf16", seed=5), weight(k, "bf16")
+    want, plain = ops.rmsnorm_int8(x, w, EPS, r), ops.quantize_rows_int8(x)
+    for part in (slice(0, 1), slice(3, 10), slice(17, 529), slice(0, 513), slice(5, 1029)):
+        assert all(torch.equal(a, b[part]) for a, b in zip(ops.rmsnorm_int8(x[part], w, EPS, r[part]), want))
+        assert all(torch.equal(a, b[part]) for a, b in zip(ops.quantize_rows_int8(x[part]), plain))
 
 
 @pytest.mark.parametrize("kind", ["bf16", "fp16"])

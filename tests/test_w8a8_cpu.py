@@ -43,6 +43,7 @@ _REFUSED = [
     ("sd_quantize_rows_int8", {"a6": 32784}, 2, "up to 32768"),
     ("sd_quantize_rows_int8", {"a5": 1 << 24}, 2, "rows below"),
     ("sd_quantize_rows_int8", {"a5": 1 << 22, "a6": 8208}, 2, "rows below"),
+    ("sd_quantize_rows_int8", {"a5": 1 << 22, "a6": 4112}, 2, "rows below"),
     ("sd_quantize_rows_int8", {"a5": -1}, 1, "invalid sizes"),
     ("sd_quantize_rows_int8", {"a6": 0}, 1, "invalid sizes"),
     ("sd_quantize_rows_int8", {"a7": BF16, "a0": None}, 1, "null"),

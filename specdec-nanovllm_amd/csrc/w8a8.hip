@@ -620,7 +620,7 @@ size_t workspace(int64_t M, int64_t N, int64_t K, bool gated) {
 
 int run(const char* what, bool gated, Args a, int32_t dtype, void* workspace_p, size_t workspace_bytes, void* stream) {
   sd::clear_error();
-  const int64_t M = a.M, N = a.N, wrows = gated ? 2 * N : N;
+  const int64_t M = a.M, N = a.N;
   if (M < 0 || N <= 0 || a.K <= 0) {
     sd::set_error("%s: invalid sizes (M=%lld N=%lld K=%d)", what, (long long)M, (long long)N, a.K);
     return SD_ERR_VALUE;
@@ -634,12 +634,13 @@ int run(const char* what, bool gated, Args a, int32_t dtype, void* workspace_p, 
     sd::set_error("%s: dtype must be bf16 or f16, the weight scales' bf16, f16 or f32", what);
     return SD_ERR_UNSUPPORTED;
   }
-  if (!sizes_ok(M, N, a.K) || (M > 1 && a.xs > (1ll << 23)) || (wrows > 1 && a.ws > (1ll << 23))) {
+  if (!sizes_ok(M, N, a.K) || (M > 1 && a.xs > (1ll << 23)) || ((gated || N > 1) && a.ws > (1ll << 23))) {
     sd::set_error("%s: M=%lld N=%lld K=%d (strides %lld, %lld) too large", what, (long long)M, (long long)N, a.K,
                   (long long)a.xs, (long long)a.ws);
     return SD_ERR_UNSUPPORTED;
   }
   if (M == 0) return SD_OK;
+  const int64_t wrows = gated ? 2 * N : N;  // (N at most 2^21)
   if (!a.x || !a.x_scale || !a.w || !a.scale || !a.y) {
     sd::set_error("%s: null pointer argument", what);
     return SD_ERR_VALUE;

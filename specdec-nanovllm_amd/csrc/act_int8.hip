@@ -62,7 +62,7 @@ __device__ __forceinline__ float element(const u32x4& v, int i, float (*to)(uint
 template <bool SHORT>
 __device__ __forceinline__ uint2 codes8(const float (&v)[8], float most, float inv, float inv1) {
 #pragma clang fp contract(off)
-  uint32_t b[2] = {0, 0};
+  uint32_t b[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     float q = v[i] * inv, rem;
@@ -73,9 +73,12 @@ __device__ __forceinline__ uint2 codes8(const float (&v)[8], float most, float i
       rem = fmaf(127.f, v[i], -p) - fmaf(q, most, -p);
     }
     q = fmaf(rem, inv1, q);
-    b[i / 4] |= (static_cast<uint32_t>(static_cast<int>(rintf(q))) & 0xffu) << (8 * (i % 4));
+    b[i] = __float_as_uint(q + 0x1.8p23f);  // the whole number nearest to q, in the low byte
   }
-  return uint2{b[0], b[1]};
+  uint32_t h[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) h[i] = __builtin_amdgcn_perm(b[2 * i + 1], b[2 * i], 0x0c0c0400u);
+  return uint2{h[0] | h[1] << 16, h[2] | h[3] << 16};
 }
 
 // TPR threads a row (64: four rows a workgroup, no barrier); thread t holds the 8-element chunks t, t + TPR, ...
@@ -107,23 +110,21 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rows_int8_kernel(Params
   uint32_t most_bits = 0;
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    if (c * TPR * 8 >= p.K) break;  // uniform
     const int e = (c * TPR + t) * 8;
-    const bool in = e < p.K;
+    if (e >= p.K) break;  // (whole waves, mostly)
     float s[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       s[i] = element(xb[c], i, sd::from_bits<T>);
       if constexpr (RES) s[i] = s[i] + element(rb[c], i, sd::from_bits<T>);
-      if (!in) s[i] = 0.f;
       v[c][i] = s[i];
       if constexpr (NORM) {
-        sums[kSums == 1 ? 0 : c] += s[i] * s[i];
-        v[c][i] = in ? s[i] * element(wb[c], i, sd::from_bits<T>) : 0.f;
+        sums[kSums == 1 ? 0 : c] = fmaf(s[i], s[i], sums[kSums == 1 ? 0 : c]);
+        v[c][i] = s[i] * element(wb[c], i, sd::from_bits<T>);
       }
       most_bits = max_u32(most_bits, __float_as_uint(v[c][i]) & 0x7fffffffu);  // NaN above infinity above all else
     }
-    if (RES && in)
+    if constexpr (RES)
       sd::store16(p.res_out + row * p.ros + e, u32x4{sd::pack2<T>(s[0], s[1]), sd::pack2<T>(s[2], s[3]),
                                                      sd::pack2<T>(s[4], s[5]), sd::pack2<T>(s[6], s[7])});
   }
@@ -162,14 +163,17 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rows_int8_kernel(Params
   // by a power of two into the range where 127 v and the quotient's inverse are finite and normal
   const float to = most < 0x1p-60f ? 0x1p64f : most > 0x1p60f ? 0x1p-64f : 1.f;
   const float scaled = most * to, inv = 127.f / scaled, inv1 = inv * (1.f / 127.f);
+  if (to != 1.f) {  // uniform: of the row
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[c][i] *= to;
+  }
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     const int e = (c * TPR + t) * 8;
     if (e >= p.K) break;
-    float u[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) u[i] = v[c][i] * to;
-    *reinterpret_cast<uint2*>(p.codes + row * p.cs + e) = none ? uint2{0, 0} : codes8<!NORM>(u, scaled, inv, inv1);
+    *reinterpret_cast<uint2*>(p.codes + row * p.cs + e) = none ? uint2{0, 0} : codes8<!NORM>(v[c], scaled, inv, inv1);
   }
 }
 

@@ -9,8 +9,9 @@
 // which and the codes the row stays in registers. A code is that of the fp32 quotient of the fp32 v and max |v|; the
 // normalised value itself is never rounded. A row with a NaN or an infinity in v has scale NaN and codes 0,
 // a row of zeros scale 0.
-// Bound by memory: 7 bytes an element with a residual, 3 without either (8192 x 2560 with a residual 25 us, 147 MB at
-// 5.9 TB/s from and to the caches; 4001 x 4096 without 10, 49 MB at 4.9); few rows by their latency, 2.3 to 3 us.
+// Bound by memory: 7 bytes an element with a residual, 3 without either (8192 x 2560 with a residual 24 us, 147 MB at
+// 6.2 TB/s from and to the caches; 4001 x 4096 without 9.9, 49 MB at 5.0), with vector issue close behind (14 of those
+// 24 us); few rows by their latency, 2.2 to 3 us.
 #include <math.h>
 
 #include "sd_common.h"
@@ -227,9 +228,9 @@ template <typename T, bool NORM, bool RES> void launch(const Params& p, hipStrea
                      dim3(static_cast<unsigned>(tpr < 256 ? (p.rows + 256 / tpr - 1) / (256 / tpr) : p.rows)), \
                      dim3(tpr < 256 ? 256 : tpr), 0, st, p)
   // A wave a row saves the barrier where rows are short and many, a thread for 8 elements saves steps where they are few
-  // (norm with residual, us): 1 x 1024 2.5 with 256 threads, 2.9 with 64, 4096 x 1024 7.4 and 6.4; 200 x 2560 3.3 with
-  // 512 threads, 3.6 with 256, 777 x 2560 5.0 and 5.3 but 3.6 and 3.5 quantized, 32768 x 2560 112 and 100. Past that 512
-  // threads: 777 x 8192 9.4, 10.2 with 256, 9.9 with 1024; 4096 x 9728 46, 53 with 1024.
+  // (norm with residual, us): 1 x 1024 2.5 with 256 threads, 2.7 with 64, 4096 x 1024 6.9 and 6.1; 1 x 2560 2.6 with 512
+  // threads, 2.8 with 256, 200 x 2560 3.2 and 3.4, 32768 x 2560 107 and 101. Past that 512 threads: 777 x 8192 8.8, 9.6
+  // with 256, 9.8 with 1024; 777 x 9728 10.8, 11.2 with 1024.
   if (p.K <= 512) SD_ROWS_INT8(64, 1);
   else if (p.K <= 1024 && p.rows > 512) SD_ROWS_INT8(64, 2);
   else if (p.K <= 2048) SD_ROWS_INT8(256, 1);

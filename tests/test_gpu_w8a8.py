@@ -77,18 +77,20 @@ def test_tiles_and_slices(m, n, k):
 ROUTES = [
     (0, 40, 34, 144, (32, 64, 4), False), (0, 40, 34, 1040, (32, 64, 4), False), (0, 20, 34, 9744, (32, 64, 4), True),
     (0, 40, 8200, 528, (64, 64, 2), False), (0, 40, 8200, 1040, (64, 64, 2), False),
-    (0, 2000, 34, 9744, (64, 64, 2), True), (0, 40, 8200, 144, (64, 128, 2), False),
-    (0, 70, 8200, 1040, (64, 128, 2), False), (0, 70, 2050, 9744, (64, 128, 2), True),
-    (0, 190, 12000, 1040, (96, 96, 1), False), (0, 200, 8200, 1040, (128, 128, 1), False),
-    (0, 400, 12000, 144, (128, 256, 1), False), (0, 400, 12000, 1040, (128, 256, 1), False),
-    (0, 500, 8200, 144, (192, 128, 1), False), (0, 500, 8200, 1040, (192, 128, 1), False),
-    (0, 900, 8200, 144, (192, 256, 1), False), (0, 900, 8200, 1040, (192, 256, 1), False),
-    (0, 1000, 12000, 144, (256, 256, 1), False), (0, 1000, 12000, 1040, (256, 256, 1), False),
-    (1, 40, 34, 144, (32, 64, 4), False), (1, 40, 34, 1040, (32, 64, 4), False), (1, 20, 34, 9744, (32, 64, 4), True),
+    (0, 1500, 34, 9744, (64, 64, 2), True), (0, 40, 8200, 144, (64, 128, 2), False),
+    (0, 100, 8200, 1040, (64, 128, 2), False), (0, 2000, 1030, 1040, (96, 96, 1), False),
+    (0, 70, 8200, 9744, (96, 96, 1), True), (0, 200, 8200, 1040, (128, 128, 1), False),
+    (0, 100, 8200, 9744, (128, 128, 1), True), (0, 400, 12000, 144, (128, 256, 1), False),
+    (0, 400, 12000, 1040, (128, 256, 1), False), (0, 500, 8200, 144, (192, 128, 1), False),
+    (0, 500, 8200, 1040, (192, 128, 1), False), (0, 900, 8200, 144, (192, 256, 1), False),
+    (0, 900, 8200, 1040, (192, 256, 1), False), (0, 1000, 12000, 144, (256, 256, 1), False),
+    (0, 1000, 12000, 1040, (256, 256, 1), False), (1, 40, 34, 144, (32, 64, 4), False),
+    (1, 40, 34, 1040, (32, 64, 4), False), (1, 20, 34, 9744, (32, 64, 4), True),
     (1, 40, 4100, 528, (64, 64, 2), False), (1, 40, 4100, 1040, (64, 64, 2), False),
-    (1, 900, 34, 9744, (64, 64, 2), True), (1, 16, 8200, 144, (64, 128, 2), False),
-    (1, 16, 8200, 1040, (64, 128, 2), False), (1, 70, 1030, 9744, (64, 128, 2), True),
-    (1, 70, 8200, 1040, (96, 96, 1), False), (1, 100, 8200, 1040, (128, 128, 1), False),
+    (1, 700, 34, 9744, (64, 64, 2), True), (1, 16, 8200, 144, (64, 128, 2), False),
+    (1, 40, 8200, 1040, (64, 128, 2), False), (1, 70, 12000, 528, (96, 96, 1), False),
+    (1, 70, 8200, 1040, (96, 96, 1), False), (1, 70, 4100, 9744, (96, 96, 1), True),
+    (1, 100, 8200, 1040, (128, 128, 1), False), (1, 100, 4100, 9744, (128, 128, 1), True),
     (1, 200, 8200, 144, (128, 256, 1), False), (1, 200, 8200, 1040, (128, 256, 1), False),
     (1, 130, 12000, 144, (192, 128, 1), False), (1, 130, 12000, 1040, (192, 128, 1), False),
     (1, 900, 4100, 144, (192, 256, 1), False), (1, 400, 8200, 1040, (192, 256, 1), False),

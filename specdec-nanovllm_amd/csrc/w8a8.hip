@@ -522,7 +522,8 @@ Plan make_plan(int64_t M, int64_t N, int64_t K, bool gated) {
   // Few rows: up to 4 always; more where weight rows are few, since every workgroup loads the activations anew (8 x 9000
   // x 4096 11.7 us there, 11.2 in tiles of 32 x 64, 12 rows 12.9 and 11.2; 16 x 6144 x 2560 6.7 and 6.8, 16 x 2560 x
   // 4096 6.0 and 8.3; 8 x 19456 x 2560 12.1 and 11.2), past 16 rows where the columns are few too (32 x 2560 x 4096 7.8
-  // and 8.5, 32 x 4096 x 1024 3.9 and 5.0; 32 x 6144 x 2560 9.0 and 6.8, 32 x 2560 x 9728 16 and 10.7).
+  // and 8.5, 32 x 4096 x 1024 3.9 and 5.0; 32 x 6144 x 2560 9.0 and 6.8, 32 x 2560 x 9728 16 and 10.7). Weights in the
+  // caches; from HBM the limits would lie somewhat higher (8 x 9000 x 4096 12.8 and 13.5, 16 x 19456 x 2560 15.7 and 14.8).
   if (M <= 4 || (M <= 8 && groups <= 3 * cus) || (M <= 16 && 2 * groups <= 3 * cus) ||
       (M <= 32 && groups <= cus && stages <= 32)) {
     pl.XT = M <= 16 ? 1 : 2;

@@ -256,6 +256,8 @@ def apply_int8_activations(model: nn.Module, module_names, act_bits: int = 8) ->
     chosen = _chosen_modules(model, module_names, torch.int8)
     for name, mod in chosen:
         _check_act8(name, mod.quant_granularity, mod.weight.shape[1])
+        if getattr(mod, "weight_scale", None) is None or mod.weight_scale.numel() != mod.weight.shape[0]:
+            raise ValueError(f"{name}: activations in 8 bits need one weight scale a row")
     for _, mod in chosen:
         mod.quant_act_bits = act_bits
 

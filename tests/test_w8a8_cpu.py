@@ -223,6 +223,13 @@ def test_layers_check_before_they_change():
     assert m["a"].quant_act_bits == 16
     with pytest.raises(ValueError, match="8 or 16"):
         apply_int8_activations(m, ["a"], 4)
+    scale = m["a"].weight_scale
+    for other in (None, torch.nn.Parameter(torch.ones((8, 2)), requires_grad=False)):  # of groups, whatever the name says
+        m["a"].weight_scale = other
+        with pytest.raises(ValueError, match="one weight scale a row"):
+            apply_int8_activations(m, ["a"])
+    m["a"].weight_scale = scale
+    assert m["a"].quant_act_bits == 16
     apply_int8_activations(m, ["a"])
     assert m["a"].quant_act_bits == 8
     x = torch.zeros((2, 64), dtype=torch.bfloat16)

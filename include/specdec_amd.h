@@ -747,7 +747,8 @@ int sd_quantize_rows_int8(const void* x, int64_t x_stride, int8_t* codes, int64_
 /*
  * RMSNorm whose result is quantized unrounded: s = x (+ residual) in fp32,
  *   v = s * rsqrt(mean(s^2) + eps) * weight,  residual_out = dtype(s)
- * residual and residual_out may both be NULL; residual_out may be x or residual.
+ * residual may be NULL; residual_out is written only with a residual. residual_out may be
+ * x or residual (the same address and row stride), otherwise its rows share no byte with theirs.
  * Limits as sd_quantize_rows_int8. A row whose squares' sum leaves fp32 gives
  * zeros, as in sd_rmsnorm.
  */

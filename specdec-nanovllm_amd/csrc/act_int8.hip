@@ -251,6 +251,26 @@ constexpr int kMostColumns = 32768;
 // (a launch takes fewer than 2^32 threads)
 constexpr int64_t most_rows(int32_t columns) { return columns > 4096 ? (1 << 22) - 1 : (1 << 24) - 1; }
 
+// Whether rows of residual_out (stride `os` >= K) share a byte with other rows of `in`, or with their own shifted: a
+// workgroup loads a row before it stores it, another's rows at any time. Exact, so that rows may lie between rows.
+bool meets_rows(const uint16_t* out, int64_t os, const uint16_t* in, int64_t is, int64_t rows, int64_t K) {
+  if (in == out && (rows == 1 || is == os)) return false;
+  if (!sd::span_rows(out, rows, 2 * os, 2 * K).overlaps(sd::span_rows(in, rows, 2 * is, 2 * K))) return false;
+  if (rows == 1) return true;
+  const __int128 step = 2 * os, width = 2 * K;
+  const __int128 first = static_cast<__int128>(reinterpret_cast<uintptr_t>(in)) - reinterpret_cast<uintptr_t>(out);
+  auto near_row = [&](__int128 at, int64_t least) {  // bytes at .. at + width and one of the rows `least` .. rows - 1
+    __int128 j = at / step - (at % step < 0);
+    for (int i = 0; i < 2; ++i, ++j)
+      if (j >= least && j < rows && at - j * step < width && j * step - at < width) return true;
+    return false;
+  };
+  if (is == os) return near_row(first, 1 - rows);  // every row's place is that of the first
+  for (int64_t i = 0; i < rows; ++i)
+    if (near_row(first + static_cast<__int128>(i) * 2 * is, 0)) return true;
+  return false;
+}
+
 // What both entries ask of their sizes and outputs; SD_OK or the refusal.
 int check(const char* what, const Params& p, int32_t dtype, bool residual) {
   if (p.rows < 0 || p.K <= 0) {
@@ -285,6 +305,8 @@ int check(const char* what, const Params& p, int32_t dtype, bool residual) {
   for (const sd::Span& o : {sd::span_rows(p.x, p.rows, 2 * p.xs, width), sd::span_rows(p.res, p.rows, 2 * p.rs, width),
                             w, res_out})
     shared |= codes.overlaps(o) || scale.overlaps(o);
+  if (residual)
+    shared |= meets_rows(p.res_out, p.ros, p.x, p.xs, p.rows, p.K) || meets_rows(p.res_out, p.ros, p.res, p.rs, p.rows, p.K);
   if (shared) {
     sd::set_error("%s: outputs share memory with another argument", what);
     return SD_ERR_VALUE;

@@ -730,8 +730,9 @@ int sd_w4a16_linear(const void* x, int64_t x_stride_m, const uint8_t* w, int64_t
  * meet 16-bit activations). A row of activations is held as codes -127 .. 127 and
  * one fp32 scale:
  *   scale = max |v| / 127,  code = round_half_even(127 v / max |v|),  value = code * scale
- * (the quotient rounded to fp32 once). A row with a NaN or an infinity in v has scale
- * NaN and codes 0 (a linear's outputs of that row are NaN); a row of zeros has scale 0.
+ * (the quotient rounded to fp32 once). A row with a NaN or an infinity in v (of a norm: in
+ * s or weight, not only in their product) has scale NaN and codes 0 (a linear's outputs of
+ * that row are NaN); a row of zeros has scale 0.
  * Rows of codes and of 16-bit tensors are 16-byte aligned; columns are a multiple of 16.
  * Outputs share no byte with inputs or each other, but for residual_out.
  * ------------------------------------------------------------------------- */

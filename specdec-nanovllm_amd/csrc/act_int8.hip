@@ -7,12 +7,14 @@
 //
 // The root mean square cancels out of the codes: the sum of squares and max |v| are one reduction, between
 // which and the codes the row stays in registers. A code is that of the fp32 quotient of the fp32 v and max |v|; the
-// normalised value itself is never rounded. A row with a NaN or an infinity in v has scale NaN and codes 0,
-// a row of zeros scale 0.
+// normalised value itself is never rounded. A row with a NaN or an infinity in s or w has scale NaN and codes 0, a row of
+// zeros scale 0. Where only the product leaves fp32 (bf16 s and w) it is formed again 2^128 smaller.
 // Bound by memory: 7 bytes an element with a residual, 3 without either (8192 x 2560 with a residual 24 us, 147 MB at
 // 6.2 TB/s from and to the caches; 4001 x 4096 without 9.9, 49 MB at 5.0), with vector issue close behind (14 of those
 // 24 us); few rows by their latency, 2.2 to 3 us.
 #include <math.h>
+
+#include <type_traits>
 
 #include "sd_common.h"
 
@@ -82,6 +84,18 @@ __device__ __forceinline__ uint2 codes8(const float (&v)[8], float most, float i
   return uint2{h[0] | h[1] << 16, h[2] | h[3] << 16};
 }
 
+// Maximum over the threads of a row; `red` may be in use by the row's other waves.
+template <int TPR> __device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t* red, int t) {
+  v = wave_max(v);
+  if constexpr (TPR > 64) {
+    __syncthreads();
+    if ((t & 63) == 0) red[t >> 6] = v;
+    __syncthreads();
+    v = wave_max(red[t % (TPR / 64)]);
+  }
+  return v;
+}
+
 // TPR threads a row (64: four rows a workgroup, no barrier); thread t holds the 8-element chunks t, t + TPR, ...
 // The squares of 64 chunks are summed by a wave, then those sums in order, whichever TPR and C <= 2 the launch took: a
 // row's scale is the same bits whatever the other rows.
@@ -90,6 +104,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rows_int8_kernel(Params
 #pragma clang fp contract(off)
   constexpr int kRows = TPR < 256 ? 256 / TPR : 1;
   constexpr int kSums = C <= 2 ? C : 1;
+  constexpr bool kWide = NORM && std::is_same<T, __bf16>::value;  // (fp16 products stay below 2^34)
   __shared__ float red_sum[kSums * (TPR / 64)];
   __shared__ uint32_t red_max[TPR / 64];
   const int t = static_cast<int>(threadIdx.x) % TPR;
@@ -109,11 +124,25 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rows_int8_kernel(Params
   }
   float v[C][8], sums[kSums] = {};
   uint32_t most_bits = 0;
+  // Chunk c's products 2^128 smaller. Exact where it counts: where s or w is below 2^-62 the product is far below half a
+  // level of a row that left fp32.
+  [[maybe_unused]] uint32_t smaller = 0;  // the chunks that are
+  [[maybe_unused]] auto again = [&](int c, int e) {
+    const u32x4 xa = RES ? xb[c] : sd::load16(x + e), wa = sd::load16(p.w + e);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float s = element(xa, i, sd::from_bits<T>);
+      if constexpr (RES) s = s + element(rb[c], i, sd::from_bits<T>);
+      v[c][i] = s * 0x1p-64f * (element(wa, i, sd::from_bits<T>) * 0x1p-64f);
+    }
+    smaller |= 1u << c;
+  };
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     const int e = (c * TPR + t) * 8;
     if (e >= p.K) break;  // (whole waves, mostly)
     float s[8];
+    uint32_t bits = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       s[i] = element(xb[c], i, sd::from_bits<T>);
@@ -123,11 +152,25 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rows_int8_kernel(Params
         sums[kSums == 1 ? 0 : c] = fmaf(s[i], s[i], sums[kSums == 1 ? 0 : c]);
         v[c][i] = s[i] * element(wb[c], i, sd::from_bits<T>);
       }
-      most_bits = max_u32(most_bits, __float_as_uint(v[c][i]) & 0x7fffffffu);  // NaN above infinity above all else
+      bits = max_u32(bits, __float_as_uint(v[c][i]) & 0x7fffffffu);  // NaN above infinity above all else
     }
+    most_bits = max_u32(most_bits, bits);
     if constexpr (RES)
       sd::store16(p.res_out + row * p.ros + e, u32x4{sd::pack2<T>(s[0], s[1]), sd::pack2<T>(s[2], s[3]),
                                                      sd::pack2<T>(s[4], s[5]), sd::pack2<T>(s[6], s[7])});
+    if constexpr (kWide && RES && C > 2)
+      if (bits == 0x7f800000u) again(c, e);
+  }
+  // With a residual, s has to be formed again from what was loaded: residual_out may have taken its place in memory. Of
+  // four chunks each for itself, since keeping all of them to here takes registers (777 x 9728 12.0 us, 10.9 so).
+  if constexpr (kWide && RES && C <= 2) {
+    if (most_bits == 0x7f800000u) {
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        if ((c * TPR + t) * 8 >= p.K) break;
+        again(c, (c * TPR + t) * 8);
+      }
+    }
   }
   float sum = 0.f;
   if constexpr (NORM) {
@@ -143,20 +186,43 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rows_int8_kernel(Params
       red_max[wave] = most_bits;
     }
     __syncthreads();
-    most_bits = 0;
 #pragma unroll
     for (int i = 0; i < kSums * (TPR / 64); ++i) sum += red_sum[i];
+    if constexpr (TPR == 1024) {
+      most_bits = wave_max(red_max[t % 16]);  // (16 more registers would leave one row a compute unit instead of two)
+    } else {
+      most_bits = 0;
 #pragma unroll
-    for (int i = 0; i < TPR / 64; ++i) most_bits = max_u32(most_bits, red_max[i]);
+      for (int i = 0; i < TPR / 64; ++i) most_bits = max_u32(most_bits, red_max[i]);
+    }
   } else {
 #pragma unroll
     for (int c = 0; c < kSums; ++c) sum += sums[c];
+  }
+  [[maybe_unused]] float up = 1.f;  // v is 1 / up^2 of the product
+  if constexpr (kWide) {
+    if (most_bits == 0x7f800000u) {  // uniform: of the row. All its products 2^128 smaller; an infinity of s or w stays one
+      uint32_t bits = 0;
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const int e = (c * TPR + t) * 8;
+        if (e >= p.K) break;
+        if constexpr (!RES) again(c, e);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (!(smaller >> c & 1)) v[c][i] = v[c][i] * 0x1p-64f * 0x1p-64f;
+          bits = max_u32(bits, __float_as_uint(v[c][i]) & 0x7fffffffu);
+        }
+      }
+      most_bits = row_max<TPR>(bits, red_max, t);
+      up = 0x1p64f;
+    }
   }
   const bool none = most_bits >= 0x7f800000u || most_bits == 0;
   const float most = __uint_as_float(most_bits);
   if (t == 0) {
     float scale = most / 127.f;
-    if constexpr (NORM) scale = scale * (1.f / sqrtf(sum / static_cast<float>(p.K) + p.eps));
+    if constexpr (NORM) scale = scale * (1.f / sqrtf(sum / static_cast<float>(p.K) + p.eps)) * up * up;
     if (most_bits == 0) scale = 0.f;
     if (most_bits >= 0x7f800000u) scale = __uint_as_float(0x7fc00000u);
     p.scale[row] = scale;

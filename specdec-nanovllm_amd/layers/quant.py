@@ -122,7 +122,7 @@ def int8_linear_a8(x, qweight: torch.Tensor, scale: torch.Tensor, bias: torch.Te
 
     x: [..., K] bf16/fp16, quantized here by row, or the (codes, scale) of
     ``ops.rmsnorm_int8`` or ``ops.quantize_rows_int8``. The result's type is x's, or
-    ``dtype`` (bf16 where neither says). K a multiple of 16.
+    ``dtype`` (bf16 where neither says). K a multiple of 16 up to 32768.
     """
     if not isinstance(x, tuple):
         dtype = dtype or x.dtype
@@ -237,11 +237,18 @@ def apply_int4_quant(model: nn.Module, module_names, group_size: int = 128):
     return [_swap_to_int4(name, mod, group_size) for name, mod in chosen]
 
 
-def _check_act8(name: str, granularity: str, columns: int) -> None:
+# What ``ops.quantize_rows_int8`` and ``ops.w8a8_linear`` take.
+MOST_COLUMNS_ACT8, MOST_OUTPUTS_ACT8 = 32768, 1 << 21
+
+
+def _check_act8(name: str, granularity: str, outputs: int, columns: int) -> None:
     if granularity != "per_channel":
         raise ValueError(f"{name}: activations in 8 bits need per-channel weight scales, got {granularity}")
     if columns % 16:
         raise ValueError(f"{name}: activations in 8 bits need a multiple of 16 columns, got {columns}")
+    if columns > MOST_COLUMNS_ACT8 or outputs > MOST_OUTPUTS_ACT8:
+        raise ValueError(f"{name}: activations in 8 bits go to {MOST_COLUMNS_ACT8} columns and {MOST_OUTPUTS_ACT8} outputs, "
+                         f"got {columns} and {outputs}")
 
 
 def apply_int8_activations(model: nn.Module, module_names, act_bits: int = 8) -> None:
@@ -249,13 +256,13 @@ def apply_int8_activations(model: nn.Module, module_names, act_bits: int = 8) ->
     (``apply_int8_quant``, or a converted checkpoint's), take their activations in 8 bits:
     ``LinearBase._apply`` then calls ``int8_linear_a8``, which also accepts (codes, scale)
     from ``RMSNorm.forward_int8``. ``act_bits=16`` goes back. Same errors as
-    ``apply_int8_quant``, ``ValueError`` for groups or a K that is no multiple of 16;
-    every module is checked before any is changed."""
+    ``apply_int8_quant``, ``ValueError`` for groups, for a K that is no multiple of 16 or above
+    32768 and for more than 2^21 outputs; every module is checked before any is changed."""
     if act_bits not in (8, 16):
         raise ValueError(f"activations in 8 or 16 bits, got {act_bits}")
     chosen = _chosen_modules(model, module_names, torch.int8)
     for name, mod in chosen:
-        _check_act8(name, mod.quant_granularity, mod.weight.shape[1])
+        _check_act8(name, mod.quant_granularity, *mod.weight.shape)
         if getattr(mod, "weight_scale", None) is None or mod.weight_scale.numel() != mod.weight.shape[0]:
             raise ValueError(f"{name}: activations in 8 bits need one weight scale a row")
     for _, mod in chosen:
@@ -284,7 +291,7 @@ def apply_int8_quant(model: nn.Module, module_names, granularity: str = "per_cha
         raise ValueError(f"activations in 8 or 16 bits, got {act_bits}")
     if act_bits == 8:
         for name, mod in chosen:
-            _check_act8(name, granularity, mod.weight.shape[1])
+            _check_act8(name, granularity, *mod.weight.shape)
     report = [_swap_to_int8(name, mod, granularity, group_size) for name, mod in chosen]
     for _, mod in chosen:
         mod.quant_act_bits = act_bits

@@ -1,0 +1,33 @@
+"""Modules with activations in 8 bits: what ``apply_int8_quant`` and ``apply_int8_activations`` accept can run."""
+import pytest
+import torch
+
+from specdec_nanovllm_amd.layers.linear import ReplicatedLinear
+from specdec_nanovllm_amd.layers.quant import apply_int8_activations, apply_int8_quant
+
+
+def model(dtype=torch.int8, **shapes):
+    """{name: (outputs, columns)} as modules with zero weights; int8 ones with a scale a row."""
+    m = torch.nn.ModuleDict({name: ReplicatedLinear(1, 1) for name in shapes})
+    for name, shape in shapes.items():
+        m[name].weight = torch.nn.Parameter(torch.zeros(shape, dtype=dtype), requires_grad=False)
+        if dtype == torch.int8:
+            m[name].weight_scale = torch.nn.Parameter(torch.ones(shape[0], dtype=torch.bfloat16), requires_grad=False)
+    return m
+
+
+# quantize_rows_int8 takes up to 32768 columns, w8a8_linear up to 2^21 outputs
+@pytest.mark.parametrize("shape,says", [((8, 32784), "32768"), ((8, 40960), "32768"), (((1 << 21) + 1, 16), "2097152")])
+def test_sizes_that_cannot_run_are_refused_before_a_change(shape, says):
+    for dtype, call in ((torch.int8, apply_int8_activations), (torch.bfloat16, lambda *a: apply_int8_quant(*a, act_bits=8))):
+        m = model(dtype, a=(8, 64), b=shape)
+        with pytest.raises(ValueError, match=says):
+            call(m, ["a", "b"])
+        assert m["a"].quant_act_bits == m["b"].quant_act_bits == 16
+        assert m["a"].weight.dtype == m["b"].weight.dtype == dtype
+
+
+def test_the_largest_sizes_are_taken():
+    m = model(a=(8, 32768), b=(1 << 21, 16))
+    apply_int8_activations(m, ["a", "b"])
+    assert m["a"].quant_act_bits == m["b"].quant_act_bits == 8

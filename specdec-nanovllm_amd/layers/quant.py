@@ -255,13 +255,13 @@ def apply_int8_activations(model: nn.Module, module_names, act_bits: int = 8) ->
     """Let the named ``LinearBase`` submodules, whose weights are int8 per channel already
     (``apply_int8_quant``, or a converted checkpoint's), take their activations in 8 bits:
     ``LinearBase._apply`` then calls ``int8_linear_a8``, which also accepts (codes, scale)
-    from ``RMSNorm.forward_int8``. ``act_bits=16`` goes back. Same errors as
-    ``apply_int8_quant``, ``ValueError`` for groups, for a K that is no multiple of 16 or above
+    from ``RMSNorm.forward_int8``. ``act_bits=16`` goes back, whatever the int8 weights. Same
+    errors as ``apply_int8_quant``, with 8 bits ``ValueError`` for groups, for a K that is no multiple of 16 or above
     32768 and for more than 2^21 outputs; every module is checked before any is changed."""
     if act_bits not in (8, 16):
         raise ValueError(f"activations in 8 or 16 bits, got {act_bits}")
     chosen = _chosen_modules(model, module_names, torch.int8)
-    for name, mod in chosen:
+    for name, mod in chosen if act_bits == 8 else ():
         _check_act8(name, mod.quant_granularity, *mod.weight.shape)
         if getattr(mod, "weight_scale", None) is None or mod.weight_scale.numel() != mod.weight.shape[0]:
             raise ValueError(f"{name}: activations in 8 bits need one weight scale a row")

@@ -31,3 +31,17 @@ def test_the_largest_sizes_are_taken():
     m = model(a=(8, 32768), b=(1 << 21, 16))
     apply_int8_activations(m, ["a", "b"])
     assert m["a"].quant_act_bits == m["b"].quant_act_bits == 8
+
+
+def test_any_int8_module_goes_back_to_16_bits():
+    """Also one whose weights were replaced since, by group scales or a K that 8 bits do not take."""
+    m = model(a=(8, 64), b=(8, 64))
+    apply_int8_activations(m, ["a", "b"])
+    m["a"].quant_granularity, m["a"].quant_group_size = "per_group", 32
+    m["a"].weight_scale = torch.nn.Parameter(torch.ones((8, 2), dtype=torch.bfloat16), requires_grad=False)
+    m["b"].weight = torch.nn.Parameter(torch.zeros((8, 72), dtype=torch.int8), requires_grad=False)
+    for names in (["a"], ["b"]):
+        with pytest.raises(ValueError):
+            apply_int8_activations(m, names)
+    apply_int8_activations(m, ["a", "b"], act_bits=16)
+    assert m["a"].quant_act_bits == m["b"].quant_act_bits == 16

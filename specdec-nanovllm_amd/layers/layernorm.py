@@ -25,5 +25,7 @@ class RMSNorm(nn.Module):
 
     def forward_int8(self, x: torch.Tensor, residual: torch.Tensor | None = None):
         """(codes, scale) of the unrounded norm, with ``residual`` ((codes, scale), new_residual)."""
-        codes, scale, *new = ops.rmsnorm_int8(x, self.weight, self.eps, residual)
-        return ((codes, scale), new[0]) if new else (codes, scale)
+        if residual is None:
+            return ops.rmsnorm_int8(x, self.weight, self.eps)
+        codes, scale, new = ops.rmsnorm_int8(x, self.weight, self.eps, residual)
+        return ops.int8_rows(codes, scale, x.dtype), new

@@ -121,13 +121,12 @@ def int8_linear_a8(x, qweight: torch.Tensor, scale: torch.Tensor, bias: torch.Te
     the scales of token and channel.
 
     x: [..., K] bf16/fp16, quantized here by row, or the (codes, scale) of
-    ``ops.rmsnorm_int8`` or ``ops.quantize_rows_int8``. The result's type is x's, or
-    ``dtype`` (bf16 where neither says). K a multiple of 16 up to 32768.
+    ``ops.rmsnorm_int8`` or ``ops.quantize_rows_int8``. The result's type is x's, or that the
+    rows came from (``ops.Int8Rows``), or ``dtype`` (bf16 where nothing says). K a multiple of 16 up to 32768.
     """
     if not isinstance(x, tuple):
-        dtype = dtype or x.dtype
         x = ops.quantize_rows_int8(x)
-    return ops.w8a8_linear(*x, qweight, scale, bias, dtype or torch.bfloat16)
+    return ops.w8a8_linear(*x, qweight, scale, bias, dtype or getattr(x, "dtype", torch.bfloat16))
 
 
 def quantize_weight_int4(w: torch.Tensor, group_size: int = 128):

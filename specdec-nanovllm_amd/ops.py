@@ -828,7 +828,19 @@ def _like(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     return torch.empty_like(t, dtype=dtype) if t.is_contiguous() else torch.empty(t.shape, dtype=dtype, device=t.device)
 
 
-def quantize_rows_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+class Int8Rows(tuple):
+    """(codes, scale) of rows in 8 bits that know the type they came from, ``dtype``, which a layer's
+    linear gives its outputs."""
+    dtype = torch.bfloat16
+
+
+def int8_rows(codes: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype) -> Int8Rows:
+    rows = Int8Rows((codes, scale))
+    rows.dtype = dtype
+    return rows
+
+
+def quantize_rows_int8(x: torch.Tensor) -> Int8Rows:
     """Rows of activations in 8 bits: x (..., K) bf16/fp16 -> (codes int8 (..., K), scale fp32
     (...,)), value = code * scale, scale = max|x| / 127 and code = round_half_even(127 x / max|x|).
     A row with a NaN or an infinity has scale NaN, a row of zeros scale 0. K a multiple of 16 up
@@ -844,7 +856,9 @@ def quantize_rows_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
             _lib.stream_ptr(dev))
     if rc:
         _lib.check(rc)
-    return (codes, scale) if x.dim() == 2 else (codes.view(x.shape), scale.view(x.shape[:-1]))
+    if x.dim() != 2:
+        codes, scale = codes.view(x.shape), scale.view(x.shape[:-1])
+    return int8_rows(codes, scale, x.dtype)
 
 
 def rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float,
@@ -881,7 +895,7 @@ def rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float,
     if x.dim() != 2:
         codes, scale = codes.view(x.shape), scale.view(x.shape[:-1])
         ro = None if ro is None else ro.view(x.shape)
-    return (codes, scale) if ro is None else (codes, scale, ro)
+    return int8_rows(codes, scale, dt) if ro is None else (codes, scale, ro)
 
 
 def dequantize_rows_int8(codes: torch.Tensor, scale: torch.Tensor,

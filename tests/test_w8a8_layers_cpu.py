@@ -45,3 +45,35 @@ def test_any_int8_module_goes_back_to_16_bits():
             apply_int8_activations(m, names)
     apply_int8_activations(m, ["a", "b"], act_bits=16)
     assert m["a"].quant_act_bits == m["b"].quant_act_bits == 16
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_quantized_rows_keep_their_type(monkeypatch, dtype):
+    """(codes, scale) from a norm or of a tensor: the linear's outputs have the type that the rows came from."""
+    import copy
+    import pickle
+
+    from specdec_nanovllm_amd import _lib, ops
+    from specdec_nanovllm_amd.layers.layernorm import RMSNorm
+    from specdec_nanovllm_amd.layers.quant import int8_linear_a8
+
+    class NoLaunch:
+        def __getattr__(self, name):
+            return lambda *args: 0
+
+    monkeypatch.setattr(_lib, "load", NoLaunch)
+    monkeypatch.setattr(_lib, "require_device", lambda *t: torch.device("cpu"))
+    monkeypatch.setattr(_lib, "on_device", lambda dev: torch.no_grad())
+    monkeypatch.setattr(_lib, "stream_ptr", lambda dev: 0)
+    m = model(a=(8, 64))
+    apply_int8_activations(m, ["a"])
+    norm, x = RMSNorm(64).to(dtype), torch.zeros((2, 64), dtype=dtype)
+    rows = [ops.quantize_rows_int8(x), norm.forward_int8(x), norm.forward_int8(x, x)[0],
+            norm.forward_int8(x.view(1, 2, 64))]
+    rows += [copy.deepcopy(rows[0]), pickle.loads(pickle.dumps(rows[1]))]
+    for r in rows:
+        assert isinstance(r, tuple) and len(r) == 2
+        assert m["a"](r).dtype == int8_linear_a8(r, m["a"].weight, m["a"].weight_scale).dtype == dtype
+        assert int8_linear_a8(r, m["a"].weight, m["a"].weight_scale, dtype=torch.bfloat16).dtype == torch.bfloat16
+    assert m["a"](x).dtype == dtype
+    assert m["a"](tuple(rows[0])).dtype == torch.bfloat16  # where nothing says

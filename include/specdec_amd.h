@@ -779,8 +779,8 @@ int sd_dequantize_rows_int8(const int8_t* codes, int64_t codes_stride, const flo
  * where there is more than one row to step over. M <= 2^24, N <= 2^21, and
  * ceil(M / 64) * ceil(N / 64) < 2^22.
  * workspace: sd_w8a8_workspace_size bytes on the same device, 16-byte aligned (sums of
- * K slices; 0 where one slice runs). Without it (NULL, too small or not aligned) the call
- * runs in one slice. `gated`: the query is for sd_w8a8_gate_up_silu.
+ * K slices; 0 where one slice runs, as for M <= 4 with K <= 16384). Without it (NULL, too small
+ * or not aligned) the call runs in one slice. `gated`: the query is for sd_w8a8_gate_up_silu.
  */
 size_t sd_w8a8_workspace_size(int64_t M, int64_t N, int64_t K, int32_t gated);
 /*

@@ -510,11 +510,14 @@ constexpr Tile kTiles[] = {
     {32, 64, 4, 2.4, 0.149, 0.440, 0.0000, 0.00040},
 };
 
-// What runs a shape: w8a8_rows<XT> of W waves (XT > 0), or a tile and K slices.
+// What runs a shape: w8a8_rows<XT> of W waves (slices 0), or a tile and K slices; with XT > 0 the former where there is
+// no workspace for the slices.
 struct Plan {
   int XT, W;
   int tile, slices;
 };
+// Up to 4 rows of up to so many columns need no workspace (what a caller may know without asking).
+constexpr int64_t kLongSum = 16384;
 Plan make_plan(int64_t M, int64_t N, int64_t K, bool gated) {
   Plan pl{};
   const int64_t cus = sd::device_cus();
@@ -524,13 +527,21 @@ Plan make_plan(int64_t M, int64_t N, int64_t K, bool gated) {
   // 4096 6.0 and 8.3; 8 x 19456 x 2560 12.1 and 11.2), past 16 rows where the columns are few too (32 x 2560 x 4096 7.8
   // and 8.5, 32 x 4096 x 1024 3.9 and 5.0; 32 x 6144 x 2560 9.0 and 6.8, 32 x 2560 x 9728 16 and 10.7). Weights in the
   // caches; from HBM the limits would lie somewhat higher (8 x 9000 x 4096 12.8 and 13.5, 16 x 19456 x 2560 15.7 and 14.8).
-  if (M <= 4 || (M <= 8 && groups <= 3 * cus) || (M <= 16 && 2 * groups <= 3 * cus) ||
-      (M <= 32 && groups <= cus && stages <= 32)) {
+  const bool few = M <= 4 || (M <= 8 && groups <= 3 * cus) || (M <= 16 && 2 * groups <= 3 * cus) ||
+                   (M <= 32 && groups <= cus && stages <= 32);
+  // Long sums of few weight rows: a workgroup walks its stages alone, which takes 0.52 to 0.82 us for 8 of them, while other
+  // compute units have nothing; tiles in K slices use them all (16 x 512 x 65536 58.2 us there, 18.4 in tiles, 16 x 2560
+  // x 28672 27.6 and 18.8, 1 x 1024 x 65536 37.6 and 19.3, 16 x 5120 x 9728 20.0 and 14.7). The figures of the tiles, of
+  // more rows, are too good for so few by half; the last microseconds are the gated sums' addition. Asked only where it
+  // may matter: 10 rounds of 8 stages are 11 us in either (16 x 2560 x 9728 11.1 and 10.3, weights from HBM 11.8 and 13.2).
+  const int64_t rounds = (stages + 7) / 8 * ((groups + cus - 1) / cus);
+  const bool either = few && 2 * groups <= 3 * cus && rounds > 10 && M <= 16 && (M > 4 || K > kLongSum);
+  if (few) {
     pl.XT = M <= 16 ? 1 : 2;
     // 8 waves, 4 for very many workgroups (1 x 151936 x 1024 24.5 us, 27.1 with 8)
     pl.W = groups > 16 * cus ? 4 : 8;
     if (pl.W > stages) pl.W = static_cast<int>(stages);
-    return pl;
+    if (!either) return pl;
   }
   // The tile and slices of the least time by the figures above. Over 336 shapes of 17 to 4096 rows its choice takes 0.6%
   // more than the fastest of them on average, 13% at worst, with weights in the caches, 1.6% and 20% with weights from
@@ -558,6 +569,9 @@ Plan make_plan(int64_t M, int64_t N, int64_t K, bool gated) {
       }
     }
   }
+  if (either && 2.9 + static_cast<double>(rounds) * (0.52 + 0.019 * static_cast<double>(M)) <=
+                    1.45 * least + (gated ? 2 : 0))
+    pl.slices = 0;
   return pl;
 }
 
@@ -582,9 +596,8 @@ template <typename T, bool GATED> void launch_tiles(const Args& a, int tile, hip
 #undef SD_TILES
 }
 
-template <typename T, bool GATED> int launch(Args a, hipStream_t st) {
-  const Plan pl = make_plan(a.M, a.N, a.K, GATED);
-  if (pl.XT) {
+template <typename T, bool GATED> int launch(Args a, const Plan& pl, hipStream_t st) {
+  if (pl.slices == 0 || (pl.XT && pl.slices > 1 && !a.part)) {
     const int cols = GATED ? 8 : 16;
     const dim3 grid(static_cast<unsigned>((a.N + cols - 1) / cols)), block(pl.W * 64);
     const size_t lds = static_cast<size_t>(pl.W) * pl.XT * 1024;
@@ -615,9 +628,7 @@ bool sizes_ok(int64_t M, int64_t N, int64_t K) {
          ((M + 63) / 64) * ((N + 63) / 64) < (1ll << 22);
 }
 
-size_t workspace(int64_t M, int64_t N, int64_t K, bool gated) {
-  if (M <= 0 || N <= 0 || K <= 0 || !sizes_ok(M, N, K)) return 0;
-  const Plan pl = make_plan(M, N, K, gated);
+size_t workspace(const Plan& pl, int64_t M, int64_t N, bool gated) {
   return pl.slices > 1 ? static_cast<size_t>(pl.slices) * M * N * (gated ? 2 : 1) * sizeof(int32_t) : 0;
 }
 
@@ -669,12 +680,13 @@ int run(const char* what, bool gated, Args a, int32_t dtype, void* workspace_p, 
     return SD_ERR_VALUE;
   }
   a.wide_y = sd::aligned16(a.y) && a.ys % 8 == 0;
-  const size_t need = workspace(M, N, a.K, gated);
+  const Plan pl = make_plan(M, N, a.K, gated);
+  const size_t need = workspace(pl, M, N, gated);
   const bool held = need && workspace_p && workspace_bytes >= need && sd::aligned16(workspace_p);
   a.part = held ? static_cast<int32_t*>(workspace_p) : nullptr;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (gated) return dtype == SD_BF16 ? launch<__bf16, true>(a, st) : launch<_Float16, true>(a, st);
-  return dtype == SD_BF16 ? launch<__bf16, false>(a, st) : launch<_Float16, false>(a, st);
+  if (gated) return dtype == SD_BF16 ? launch<__bf16, true>(a, pl, st) : launch<_Float16, true>(a, pl, st);
+  return dtype == SD_BF16 ? launch<__bf16, false>(a, pl, st) : launch<_Float16, false>(a, pl, st);
 }
 
 Args args_of(const int8_t* x, int64_t xs, const float* x_scale, const int8_t* w, int64_t ws, const void* scale,
@@ -699,13 +711,14 @@ Args args_of(const int8_t* x, int64_t xs, const float* x_scale, const int8_t* w,
 }  // namespace
 
 extern "C" size_t sd_w8a8_workspace_size(int64_t M, int64_t N, int64_t K, int32_t gated) {
-  return workspace(M, N, K, gated != 0);
+  if (M <= 0 || N <= 0 || K <= 0 || !sizes_ok(M, N, K)) return 0;
+  return workspace(make_plan(M, N, K, gated != 0), M, N, gated != 0);
 }
 
 extern "C" int64_t sd_w8a8_plan(int64_t M, int64_t N, int64_t K, int32_t gated) {
   if (M <= 0 || N <= 0 || K <= 0 || K % 16 != 0 || !sizes_ok(M, N, K)) return 0;
   const Plan pl = make_plan(M, N, K, gated != 0);
-  if (pl.XT) return pl.W | 16 << 8;
+  if (pl.slices == 0) return pl.W | 16 << 8;
   const Tile& t = kTiles[pl.tile];
   return pl.slices | t.bn << 8 | static_cast<int64_t>(t.bm) << 20 | static_cast<int64_t>(t.per_cu) << 32;
 }

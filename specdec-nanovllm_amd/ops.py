@@ -958,9 +958,9 @@ def _w8a8(gated: bool, x, x_scale, qweight, scale, bias, dtype, out):
     if M:
         lib = _lib.load()
         with _lib.on_device(dev):
-            # the plan (and so the workspace) depends on the device's compute units; up to 4 rows there is none
-            # (the question takes 1 us)
-            ws_bytes = lib.sd_w8a8_workspace_size(M, N, K, gated) if M > 4 else 0
+            # the plan (and so the workspace) depends on the device's compute units; up to 4 rows of up to 16384
+            # columns there is none (the question takes 1 us, 2 to 3 where tiles are compared)
+            ws_bytes = lib.sd_w8a8_workspace_size(M, N, K, gated) if M > 4 or K > 16384 else 0
             ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
             rc = (lib.sd_w8a8_gate_up_silu if gated else lib.sd_w8a8_linear)(
                 xp, x0, xs.data_ptr(), wp, w0, sc.data_ptr(), _lib.dtype_code(sc.dtype), _ptr(b), y.data_ptr(),

@@ -828,15 +828,18 @@ def _like(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     return torch.empty_like(t, dtype=dtype) if t.is_contiguous() else torch.empty(t.shape, dtype=dtype, device=t.device)
 
 
+_BF16 = torch.bfloat16
+
+
 class Int8Rows(tuple):
     """(codes, scale) of rows in 8 bits that know the type they came from, ``dtype``, which a layer's
     linear gives its outputs."""
-    dtype = torch.bfloat16
+    dtype = _BF16
 
 
 def int8_rows(codes: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype) -> Int8Rows:
     rows = Int8Rows((codes, scale))
-    if dtype is not torch.bfloat16:  # (an attribute of its own takes 0.1 us)
+    if dtype is not _BF16:  # (an attribute of its own takes 0.1 us)
         rows.dtype = dtype
     return rows
 
@@ -848,18 +851,19 @@ def quantize_rows_int8(x: torch.Tensor) -> Int8Rows:
     to 32768. (``quantize_int8`` makes weights: a bf16 scale, rounded after the codes.)"""
     x2, x0, xp = _rows8(x)
     rows, K = x2.shape
+    dt = x2.dtype
     dev = _lib.require_device(x2)
     codes = _like(x2, torch.int8)
     scale = torch.empty(rows, dtype=torch.float32, device=dev)
     with _lib.on_device(dev):
         rc = _lib.load().sd_quantize_rows_int8(
-            xp, x0, codes.data_ptr(), K, scale.data_ptr(), rows, K, _lib.dtype_code(x2.dtype),
+            xp, x0, codes.data_ptr(), K, scale.data_ptr(), rows, K, _lib.dtype_code(dt),
             _lib.stream_ptr(dev))
     if rc:
         _lib.check(rc)
-    if x.dim() != 2:
+    if x2 is not x and x.dim() != 2:
         codes, scale = codes.view(x.shape), scale.view(x.shape[:-1])
-    return int8_rows(codes, scale, x.dtype)
+    return Int8Rows((codes, scale)) if dt is _BF16 else int8_rows(codes, scale, dt)
 
 
 def rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float,
@@ -893,10 +897,12 @@ def rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float,
             _lib.dtype_code(dt), _lib.stream_ptr(dev))
     if rc:
         _lib.check(rc)
-    if x.dim() != 2:
+    if x2 is not x and x.dim() != 2:
         codes, scale = codes.view(x.shape), scale.view(x.shape[:-1])
         ro = None if ro is None else ro.view(x.shape)
-    return int8_rows(codes, scale, dt) if ro is None else (codes, scale, ro)
+    if ro is not None:
+        return codes, scale, ro
+    return Int8Rows((codes, scale)) if dt is _BF16 else int8_rows(codes, scale, dt)
 
 
 def dequantize_rows_int8(codes: torch.Tensor, scale: torch.Tensor,

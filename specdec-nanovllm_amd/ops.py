@@ -984,7 +984,8 @@ def w8a8_linear(x: torch.Tensor, x_scale: torch.Tensor, qweight: torch.Tensor, s
     x (..., K) int8 and x_scale (...,) fp32: activations of ``quantize_rows_int8`` or
     ``rmsnorm_int8``; qweight (N, K) int8 and scale (N,): the weights of ``w8a16_linear``, per
     channel. K a multiple of 16 below 2^17. Exact integer sums, fp32 scales, one rounding to
-    ``dtype`` (bf16 or fp16); returns (..., N)."""
+    ``dtype`` (bf16 or fp16); returns (..., N). Rows that do not start at 16-byte addresses are
+    copied first, in every call, weights too: keep those aligned."""
     return _w8a8(False, x, x_scale, qweight, scale, bias, dtype, out)
 
 

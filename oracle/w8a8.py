@@ -3,8 +3,8 @@
 16-bit inputs arrive as float32 arrays of their exact values. The codes follow from fp32 v and max |v| by one quotient
 rounded to fp32. Of two 16-bit values, a 2^i and b 2^j with whole a and b below 2^11, the quotient 127 a / (b 2^f) is a
 tie (2 n + 1) / 2 or differs from it by at least 1 / (b 2^(f + 1)), that is by 1 / (254 a) > 2^-19 of itself; fp32 moves
-it by 2^-24 at most, so that this rounding moves no code. So they are compared for equality; scales and outputs in 64 bits, the linear's also by its own fp32
-steps."""
+it by 2^-24 at most, so that this rounding moves no code. So they are compared for equality; scales and outputs in 64
+bits, the linear's also by its own fp32 steps."""
 from __future__ import annotations
 
 import numpy as np

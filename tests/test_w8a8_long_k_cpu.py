@@ -5,9 +5,11 @@ import torch
 
 from specdec_nanovllm_amd import _lib
 
-pytestmark = pytest.mark.skipif(
-    torch.cuda.is_available() and torch.cuda.get_device_properties(0).multi_processor_count != 256,
-    reason="the routes of 256 compute units")
+
+@pytest.fixture(autouse=True)
+def of_256_compute_units():
+    if torch.cuda.device_count() and torch.cuda.get_device_properties(0).multi_processor_count != 256:
+        pytest.skip("the routes of 256 compute units")
 
 
 def route(m, n, k, gated=0):
